@@ -185,7 +185,8 @@ const char* lunara_last_error_string(void);
 /* Synchronizes `stream`, then returns the device error word (0 = none) and
  * clears it when `clear` is non-zero. Codes: 0x1xx GEMM, 0x2xx attention
  * (a bounded wait ran out), 0x301 gather index out of range, 0x4xx the
- * self-tests of lunara_b200_selftest.h.
+ * self-tests of lunara_b200_selftest.h, 0x5xx the decoder operators of
+ * lunara_b200_decoder.h.
  * The word is one per device and sticky: a kernel on any stream of the
  * current device sets it (the first failure wins) and it stays set until a
  * caller clears it. Only `stream` is synchronized, so a caller that launched

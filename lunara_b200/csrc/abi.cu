@@ -20,8 +20,8 @@ namespace lunara {
 __device__ unsigned int g_device_error_word = 0;
 
 namespace {
-
 thread_local char g_last_error[512] = "";
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -40,6 +40,8 @@ int from_cuda(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return ok();
   return fail(LUNARA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
 }
+
+namespace {
 
 bool valid_dtype(int d) { return d == LUNARA_F16 || d == LUNARA_BF16 || d == LUNARA_F32; }
 bool valid_act(int a) { return a >= LUNARA_ACT_NONE && a <= LUNARA_ACT_TANH; }

@@ -33,6 +33,10 @@ enum DeviceErrorSite : unsigned int {
   kErrAttnMma = 0x202,
   kErrAttnSoftmax = 0x203,
   kErrGatherIndex = 0x301,
+  kErrRotaryPosition = 0x501,  // position outside the rotary table
+  kErrCachePage = 0x502,       // page number outside the cache
+  kErrCachePosition = 0x503,   // position outside the page table
+  kErrPagedWait = 0x504,       // a bounded wait of the paged attention ran out
   kErrSelftestWait = 0x401,   // the bounded-wait self-test kernel (never set by a product kernel)
 };
 

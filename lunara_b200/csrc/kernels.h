@@ -12,6 +12,12 @@ namespace lunara {
 
 int device_num_sms();
 
+// Status of an entry point: keeps a message for lunara_last_error_string()
+// and returns the code (fail), clears it (ok), or does either by a CUDA result.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int ok();
+int from_cuda(cudaError_t e, const char* what);
+
 // Launch with programmatic stream serialization: the kernel may be scheduled
 // before its predecessor in the stream has finished and waits for it in
 // pdl_wait() (common.cuh). Used for every kernel of the hot path.

@@ -1,0 +1,723 @@
+// Rotary positions, per-head query/key norms with the rotation, and appending
+// to and reading from the paged key/value cache: kernels that move rows of one
+// head's elements ("rows") once, bound by HBM when there are many tokens and by
+// memory latency in a decode step.
+//
+// Mathematics. A pair (a, b) of a row at position p becomes
+//   (a cos - b sin, b cos + a sin),  (cos, sin) = table[p][pair]
+// with pairs (i, i + rot/2) or (2i, 2i + 1), elements from rot on unchanged;
+// the norm before it is x * rsqrt(mean(x^2) + eps) * w. All of it in fp32 with
+// one rounding at the end. The rotation's products and sums are rounded one by
+// one (no contraction into FMAs), so that the 4-bit codes made from them are
+// the same in any implementation of the definition.
+//
+// Work split. A lane holds the two 8-element vectors of one "unit" of a row
+// (both halves of 8 pairs, or 16 neighbouring elements), so a pair never
+// crosses lanes, rotation in place is safe and every access is 16 bytes. The
+// (cos, sin) of its 8 pairs stay in registers while the lane walks over kHeads
+// heads of the token: the fp32 table (64 bytes per lane) is read once for
+// them instead of once per head.
+#include "kernels.h"
+#include "paged.cuh"
+
+namespace lunara {
+namespace {
+
+constexpr int kThreads = 128;
+
+// 8 consecutive elements (16-byte aligned) as floats, and back.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const float2 a = Io<T>::unpack2(u.x), b = Io<T>::unpack2(u.y), c = Io<T>::unpack2(u.z), d = Io<T>::unpack2(u.w);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint4 u;
+    u.x = Io<T>::pack2(f[0], f[1]);
+    u.y = Io<T>::pack2(f[2], f[3]);
+    u.z = Io<T>::pack2(f[4], f[5]);
+    u.w = Io<T>::pack2(f[6], f[7]);
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+}
+
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+  const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+  a = x;
+}
+
+// One group of heads: strided rows in, strided rows or cache slots out.
+struct RowSet {
+  const void* src;
+  void* dst;
+  int64_t sb, sh, ss;      // source strides (batch, head, seq)
+  int64_t db, dh, ds;      // destination strides; paged: db = page, dh = head, ds = slot (dim)
+  const void* weight;      // norm weight or NULL
+  int heads;
+  int rotate, paged;
+};
+
+struct RowsParams {
+  RowSet set[3];
+  int group_end[3];        // head groups of sets 0..i, cumulated
+  // positions: given, or from the sequences
+  const void* positions;
+  int position_bytes;
+  int64_t position_batch_stride;
+  Seqs seqs;
+  int num_pages;
+  const float* table;
+  int64_t table_positions;
+  int rot, dim, units, lanes_log2;
+  int tokens, seq;         // tokens = batch * seq
+  int inverse;
+  float eps;
+  unsigned int* err;
+};
+
+// Where a token stands: its batch index and seq index in the views, its
+// position, and (paged) its page and slot.
+struct TokenPlace {
+  int b, s, page, slot;
+  int64_t pos;
+  bool owned;    // false: nothing of the token is touched
+  bool valid;    // false: its rows are zero, nothing goes to the cache
+};
+
+template <bool PAGED>
+__device__ __forceinline__ TokenPlace place_token(const RowsParams& p, int token, bool needs_table) {
+  TokenPlace t;
+  t.owned = token < p.tokens;
+  t.valid = false;
+  t.page = -1;
+  t.slot = 0;
+  t.pos = 0;
+  t.b = 0;
+  t.s = token;
+  if (!t.owned) return t;
+  if constexpr (PAGED) {
+    int seq;
+    t.owned = find_token(p.seqs, token, seq, t.pos);
+    if (!t.owned || t.pos < 0) return t;
+    t.page = find_page(p.seqs, seq, t.pos, p.num_pages, t.slot, p.err);
+    t.valid = t.page >= 0;
+  } else {
+    t.b = token / p.seq;
+    t.s = token - t.b * p.seq;
+    const int64_t i = t.b * p.position_batch_stride + t.s;
+    t.pos = p.position_bytes == 8 ? static_cast<const int64_t*>(p.positions)[i]
+                                  : static_cast<const int32_t*>(p.positions)[i];
+    t.valid = true;
+  }
+  if (t.valid && needs_table && (t.pos < 0 || t.pos >= p.table_positions)) {
+    atomicCAS(p.err, 0u, static_cast<unsigned>(kErrRotaryPosition));
+    t.valid = false;
+  }
+  return t;
+}
+
+template <typename T, int LAYOUT, bool NORM, bool PAGED, int HEADS>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowsParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lanes = 1 << p.lanes_log2;
+  const int gid = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
+  const int u = static_cast<int>(threadIdx.x) & (lanes - 1);
+  int which = 0;
+  while (which < 2 && static_cast<int>(blockIdx.y) >= p.group_end[which]) ++which;
+  const RowSet& set = p.set[which];
+  const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.group_end[which - 1] : 0)) * HEADS;
+  const int nh = min(HEADS, set.heads - h0);
+  const TokenPlace t = place_token<PAGED>(p, gid, p.rot > 0);
+  const bool rotate = set.rotate && 16 * u < p.rot;
+  const bool active = t.owned && u < p.units;
+  int o0, o1;
+  if (LAYOUT == LUNARAD_ROTARY_HALF && 16 * u < p.rot) {
+    o0 = 8 * u;
+    o1 = p.rot / 2 + 8 * u;
+  } else {
+    o0 = 16 * u;
+    o1 = o0 + 8;
+  }
+  const T* src = static_cast<const T*>(set.src) + t.b * set.sb + t.s * set.ss + h0 * set.sh;
+  float a[HEADS][8], b[HEADS][8];
+  if (active && t.valid) {
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+      if (h < nh) {
+        load8(src + h * set.sh + o0, a[h]);
+        load8(src + h * set.sh + o1, b[h]);
+      }
+  }
+  float cs[16];
+  if (active && t.valid && rotate) {
+    const float4* row = reinterpret_cast<const float4*>(p.table + t.pos * p.rot + 16 * u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = __ldg(row + i);
+      cs[4 * i] = v.x; cs[4 * i + 1] = v.y; cs[4 * i + 2] = v.z; cs[4 * i + 3] = v.w;
+    }
+    if (p.inverse) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cs[2 * i + 1] = -cs[2 * i + 1];
+    }
+  }
+  if constexpr (NORM) {
+    float w0[8], w1[8];
+    if (active && set.weight != nullptr) {
+      load8(static_cast<const T*>(set.weight) + o0, w0);
+      load8(static_cast<const T*>(set.weight) + o1, w1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w0[i] = w1[i] = 1.f;
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      float ss = 0.f;
+      if (active && t.valid && h < nh) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(a[h][i], a[h][i], fmaf(b[h][i], b[h][i], ss));
+      }
+      for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss / static_cast<float>(p.dim) + p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[h][i] = a[h][i] * r * w0[i];
+        b[h][i] = b[h][i] * r * w1[i];
+      }
+    }
+  }
+  if (!active) return;
+  T* dst = static_cast<T*>(set.dst);
+  if (set.paged) {
+    if (!t.valid) return;
+    dst += t.page * set.db + h0 * set.dh + t.slot * set.ds;
+  } else {
+    dst += t.b * set.db + t.s * set.ds + h0 * set.dh;
+  }
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    if (h < nh) {
+      if (!t.valid) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[h][i] = b[h][i] = 0.f;
+      } else if (rotate) {
+        if (LAYOUT == LUNARAD_ROTARY_HALF) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) turn(a[h][i], b[h][i], cs[2 * i], cs[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            turn(a[h][2 * i], a[h][2 * i + 1], cs[2 * i], cs[2 * i + 1]);
+            turn(b[h][2 * i], b[h][2 * i + 1], cs[8 + 2 * i], cs[8 + 2 * i + 1]);
+          }
+        }
+      }
+      store8(dst + h * set.dh + o0, a[h]);
+      store8(dst + h * set.dh + o1, b[h]);
+    }
+  }
+}
+
+// Any head dimension, alignment and rot: one warp per row, lanes over pairs
+// and then over the elements behind rot, element by element.
+template <typename T, bool NORM, bool PAGED>
+__global__ void __launch_bounds__(kThreads) rows_any_kernel(const __grid_constant__ RowsParams p, int layout) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int token = static_cast<int>(blockIdx.x) * (kThreads / 32) + (static_cast<int>(threadIdx.x) >> 5);
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  int which = 0;
+  while (which < 2 && static_cast<int>(blockIdx.y) >= p.group_end[which]) ++which;
+  const RowSet& set = p.set[which];
+  const int h = static_cast<int>(blockIdx.y) - (which ? p.group_end[which - 1] : 0);
+  const TokenPlace t = place_token<PAGED>(p, token, p.rot > 0);
+  if (!t.owned || (set.paged && !t.valid)) return;
+  const T* src = static_cast<const T*>(set.src) + t.b * set.sb + t.s * set.ss + h * set.sh;
+  T* dst = static_cast<T*>(set.dst) +
+           (set.paged ? t.page * set.db + t.slot * set.ds : t.b * set.db + t.s * set.ds) + h * set.dh;
+  if (!t.valid) {
+    for (int d = lane; d < p.dim; d += 32) dst[d] = Io<T>::from_f(0.f);
+    return;
+  }
+  float r = 1.f;
+  const T* w = static_cast<const T*>(set.weight);
+  if constexpr (NORM) {
+    float ss = 0.f;
+    for (int d = lane; d < p.dim; d += 32) {
+      const float x = Io<T>::to_f(src[d]);
+      ss = fmaf(x, x, ss);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    r = rsqrtf(ss / static_cast<float>(p.dim) + p.eps);
+  }
+  auto value = [&](int d) {
+    float x = Io<T>::to_f(src[d]);
+    if constexpr (NORM) x = x * r * (w != nullptr ? Io<T>::to_f(w[d]) : 1.f);
+    return x;
+  };
+  const int rot = set.rotate ? p.rot : 0;
+  for (int i = lane; i < rot / 2; i += 32) {
+    const int d0 = layout == LUNARAD_ROTARY_HALF ? i : 2 * i;
+    const int d1 = layout == LUNARAD_ROTARY_HALF ? rot / 2 + i : 2 * i + 1;
+    float a = value(d0), b = value(d1);
+    const float* cs = p.table + (t.pos * (p.rot / 2) + i) * 2;
+    turn(a, b, cs[0], p.inverse ? -cs[1] : cs[1]);
+    dst[d0] = Io<T>::from_f(a);
+    dst[d1] = Io<T>::from_f(b);
+  }
+  for (int d = rot + lane; d < p.dim; d += 32) dst[d] = Io<T>::from_f(value(d));
+}
+
+// ------------------------------------------------- append to a 4-bit cache --
+// A thread makes the 16 elements of one scale block: rotates them (reading the
+// partner elements of the half layout as well; they are in L1 from the lane
+// that owns them), takes their largest magnitude, the e4m3 scale and the codes,
+// and writes 8 bytes of codes and one scale byte. Query rows go the same way
+// and are stored unquantised.
+struct QuantParams {
+  RowsParams r;
+  void* scales[3];
+  int64_t sc_page[3], sc_head[3];
+  float inv_gain[3];
+  int blocks;   // dim / 16
+};
+
+// code = e2m1(y / s), the quotient rounded to nearest as IEEE division does:
+// with r = RN(1/s), q0 = RN(y r) and the exact remainder y - q0 s, RN(q0 +
+// remainder * r) is the correctly rounded quotient (Markstein, 1990; s has 4
+// significant bits, so the all-ones exception of the theorem cannot arise, and
+// y / s <= 7 while y is finite, so nothing over- or underflows that matters).
+__device__ __forceinline__ float quotient(float y, float s, float r) {
+  const float q0 = __fmul_rn(y, r);
+  return __fmaf_rn(__fmaf_rn(-q0, s, y), r, q0);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) append_e2m1_kernel(const __grid_constant__ QuantParams q, int layout) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const RowsParams& p = q.r;
+  const int lanes = 1 << p.lanes_log2;
+  const int token = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
+  const int u = static_cast<int>(threadIdx.x) & (lanes - 1);
+  int which = 0;
+  while (which < 2 && static_cast<int>(blockIdx.y) >= p.group_end[which]) ++which;
+  const RowSet& set = p.set[which];
+  const int h = static_cast<int>(blockIdx.y) - (which ? p.group_end[which - 1] : 0);
+  const TokenPlace t = place_token<true>(p, token, p.rot > 0);
+  if (!t.owned || u >= q.blocks || (set.paged && !t.valid)) return;
+  const T* src = static_cast<const T*>(set.src) + t.s * set.ss + h * set.sh;
+  const int d0 = 16 * u;
+  float y[16];
+  if (!t.valid) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = 0.f;
+  } else {
+    const int rot = set.rotate ? p.rot : 0;
+    const float* row = p.table + t.pos * p.rot;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int d = d0 + 8 * c;
+        float x[8];
+        load8(src + d, x);
+        if (d < rot) {
+          if (layout == LUNARAD_ROTARY_HALF) {
+            const bool first = d < rot / 2;
+            float z[8];
+            load8(src + (first ? d + rot / 2 : d - rot / 2), z);
+            const float* cs = row + 2 * (first ? d : d - rot / 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a = first ? x[i] : z[i], b = first ? z[i] : x[i];
+              turn(a, b, __ldg(cs + 2 * i), __ldg(cs + 2 * i + 1));
+              x[i] = first ? a : b;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], __ldg(row + d + 2 * i), __ldg(row + d + 2 * i + 1));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[8 * c + i] = x[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = d0 + i;
+        float x = Io<T>::to_f(src[d]);
+        if (d < rot) {
+          const bool first = layout == LUNARAD_ROTARY_HALF ? d < rot / 2 : (d & 1) == 0;
+          const int other = layout == LUNARAD_ROTARY_HALF ? (first ? d + rot / 2 : d - rot / 2) : (d ^ 1);
+          const int pair = layout == LUNARAD_ROTARY_HALF ? (first ? d : d - rot / 2) : d >> 1;
+          const float z = Io<T>::to_f(src[other]);
+          float a = first ? x : z, b = first ? z : x;
+          turn(a, b, row[2 * pair], row[2 * pair + 1]);
+          x = first ? a : b;
+        }
+        y[i] = x;
+      }
+    }
+  }
+  if (!set.paged) {
+    T* dst = static_cast<T*>(set.dst) + t.s * set.ds + h * set.dh + d0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 8) {
+      if constexpr (VEC) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = y[i + j];
+        store8(dst + i, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dst[i + j] = Io<T>::from_f(y[i + j]);
+      }
+    }
+    return;
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    y[i] = __fmul_rn(y[i], q.inv_gain[which]);
+    amax = fmax_nan(amax, fabsf(y[i]));
+  }
+  const uint32_t sb = float_to_e4m3(__fdiv_rn(amax, 6.0f));   // saturates at 448, keeps NaN
+  const float s = e4m3_to_float(sb);
+  uint32_t w[2] = {0u, 0u};
+  if (s > 0.f) {
+    const float r = __frcp_rn(s);
+    const bool finite = amax < 1e30f;   // beyond, the quotient's remainder may overflow
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float lo = finite ? quotient(y[i], s, r) : __fdiv_rn(y[i], s);
+      const float hi = finite ? quotient(y[i + 1], s, r) : __fdiv_rn(y[i + 1], s);
+      w[i >> 3] |= float2_to_e2m1x2(lo, hi) << (4 * (i & 7));
+    }
+  }
+  uint8_t* dst = static_cast<uint8_t*>(set.dst) + t.page * set.db + h * set.dh + t.slot * set.ds + 8 * u;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  static_cast<uint8_t*>(q.scales[which])[t.page * q.sc_page[which] + h * q.sc_head[which] +
+                                         static_cast<int64_t>(t.slot) * q.blocks + u] = static_cast<uint8_t>(sb);
+}
+
+// --------------------------------------------------------------- read back --
+struct ReadParams {
+  Seqs seqs;
+  const void* src[2];
+  const void* scales[2];
+  int64_t page_stride[2], head_stride[2], sc_page[2], sc_head[2];
+  float gain[2];
+  void* dst[2];
+  int heads, dim, units, lanes_log2, num_pages, tokens;
+  unsigned int* err;
+};
+
+// blockIdx.y = head, blockIdx.z = 0 keys / 1 values; a lane moves 16 elements.
+template <typename T, bool E2M1, bool VEC>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lanes = 1 << p.lanes_log2;
+  const int token = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
+  const int u0 = static_cast<int>(threadIdx.x) & (lanes - 1);
+  if (token >= p.tokens) return;
+  const int h = static_cast<int>(blockIdx.y), kv = static_cast<int>(blockIdx.z);
+  int seq, slot = 0, page = -1;
+  int64_t pos;
+  if (!find_token(p.seqs, token, seq, pos)) return;
+  if (pos >= 0) page = find_page(p.seqs, seq, pos, p.num_pages, slot, p.err);
+  T* dst = static_cast<T*>(p.dst[kv]) + (static_cast<int64_t>(token) * p.heads + h) * p.dim;
+  const int64_t at = page * p.page_stride[kv] + h * p.head_stride[kv];
+  for (int u = u0; u < p.units; u += lanes) {
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = 0.f;
+    if constexpr (E2M1) {
+      if (page >= 0) {
+        const uint8_t* c = static_cast<const uint8_t*>(p.src[kv]) + at + static_cast<int64_t>(slot) * (p.dim / 2) + 8 * u;
+        const uint32_t sb = static_cast<const uint8_t*>(p.scales[kv])[page * p.sc_page[kv] + h * p.sc_head[kv] +
+                                                                      static_cast<int64_t>(slot) * (p.dim / 16) + u];
+        const uint2 w = *reinterpret_cast<const uint2*>(c);
+        const float s = __fmul_rn(e4m3_to_float(sb), p.gain[kv]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 v = __half22float2(e2m1x2_to_half2(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFu));
+          f[2 * i] = __fmul_rn(v.x, s);
+          f[2 * i + 1] = __fmul_rn(v.y, s);
+        }
+      }
+    }
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 8) {
+        float x[8];
+        if constexpr (E2M1) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = f[i + j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = 0.f;
+          if (page >= 0) load8(static_cast<const T*>(p.src[kv]) + at + static_cast<int64_t>(slot) * p.dim + 16 * u + i, x);
+        }
+        store8(dst + 16 * u + i, x);
+      }
+    } else {
+      for (int i = 0; i < 16 && 16 * u + i < p.dim; ++i) {
+        if constexpr (E2M1) dst[16 * u + i] = Io<T>::from_f(f[i]);
+        else dst[16 * u + i] = page >= 0 ? static_cast<const T*>(p.src[kv])[at + static_cast<int64_t>(slot) * p.dim + 16 * u + i]
+                                         : Io<T>::from_f(0.f);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------- host --
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int log2_ceil(int n) {
+  int l = 0;
+  while ((1 << l) < n) ++l;
+  return l;
+}
+
+// Whether the 16-byte row kernel takes the sets: whole units, 16-byte aligned rows.
+bool rows_vector_ok(const RowsParams& p, int n_sets, int elem) {
+  if (p.dim % 16 != 0 || p.rot % 16 != 0 || p.dim > 512) return false;
+  if (p.rot > 0 && !al16(p.table)) return false;
+  const int64_t vec = 16 / elem;
+  for (int i = 0; i < n_sets; ++i) {
+    const RowSet& s = p.set[i];
+    if (!al16(s.src) || !al16(s.dst) || !al16(s.weight)) return false;
+    const int64_t st[6] = {s.sb, s.sh, s.ss, s.db, s.dh, s.ds};
+    for (int64_t v : st)
+      if (v % vec != 0) return false;
+  }
+  return true;
+}
+
+void set_groups(RowsParams& p, int n_sets, int per) {
+  int end = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (i < n_sets) end += (p.set[i].heads + per - 1) / per;
+    p.group_end[i] = end;
+  }
+}
+
+constexpr int kHeads = 4;
+
+template <typename T, bool NORM, bool PAGED>
+cudaError_t run_rows(RowsParams p, int n_sets, int layout, cudaStream_t s) {
+  p.err = device_error_word();
+  if (p.err == nullptr) return cudaErrorInvalidDevice;
+  if (!rows_vector_ok(p, n_sets, sizeof(T))) {
+    set_groups(p, n_sets, 1);
+    const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, kThreads / 32)), p.group_end[2]);
+    return launch_pdl(rows_any_kernel<T, NORM, PAGED>, grid, dim3(kThreads), 0, s, p, layout);
+  }
+  p.units = p.dim / 16;
+  p.lanes_log2 = log2_ceil(p.units);
+  const int per_block = kThreads >> p.lanes_log2;
+  const unsigned gx = static_cast<unsigned>(ceil_div64(p.tokens, per_block));
+  set_groups(p, n_sets, 1);
+  const bool few = static_cast<int64_t>(gx) * p.group_end[2] <= int64_t{device_num_sms()} * 16;
+  if (!few) set_groups(p, n_sets, kHeads);
+  const dim3 grid(gx, p.group_end[2]);
+  if (layout == LUNARAD_ROTARY_HALF)
+    return few ? launch_pdl(rows_kernel<T, LUNARAD_ROTARY_HALF, NORM, PAGED, 1>, grid, dim3(kThreads), 0, s, p)
+               : launch_pdl(rows_kernel<T, LUNARAD_ROTARY_HALF, NORM, PAGED, kHeads>, grid, dim3(kThreads), 0, s, p);
+  return few ? launch_pdl(rows_kernel<T, LUNARAD_ROTARY_INTERLEAVED, NORM, PAGED, 1>, grid, dim3(kThreads), 0, s, p)
+             : launch_pdl(rows_kernel<T, LUNARAD_ROTARY_INTERLEAVED, NORM, PAGED, kHeads>, grid, dim3(kThreads), 0, s, p);
+}
+
+template <bool NORM, bool PAGED>
+cudaError_t run_rows_dtype(const RowsParams& p, int n_sets, int layout, int64_t dtype, cudaStream_t s) {
+  if (dtype == LUNARA_F16) return run_rows<__half, NORM, PAGED>(p, n_sets, layout, s);
+  if (dtype == LUNARA_BF16) return run_rows<__nv_bfloat16, NORM, PAGED>(p, n_sets, layout, s);
+  return run_rows<float, NORM, PAGED>(p, n_sets, layout, s);
+}
+
+void set_rotary(RowsParams& p, const lunarad_rotary_table& r) {
+  p.table = r.table;
+  p.table_positions = r.positions;
+  p.rot = static_cast<int>(r.rot);
+}
+
+RowSet view_set(const lunarad_view& in, const lunarad_view& out, const void* weight, int64_t heads) {
+  RowSet s{};
+  s.src = in.data;
+  s.sb = in.batch_stride;
+  s.sh = in.head_stride;
+  s.ss = in.seq_stride;
+  s.dst = const_cast<void*>(out.data);
+  s.db = out.batch_stride;
+  s.dh = out.head_stride;
+  s.ds = out.seq_stride;
+  s.weight = weight;
+  s.heads = static_cast<int>(heads);
+  s.rotate = 1;
+  return s;
+}
+
+template <typename T>
+cudaError_t run_quant(QuantParams q, int n_sets, int layout, cudaStream_t s) {
+  RowsParams& p = q.r;
+  p.err = device_error_word();
+  if (p.err == nullptr) return cudaErrorInvalidDevice;
+  q.blocks = p.dim / 16;
+  p.lanes_log2 = log2_ceil(q.blocks);
+  const int per_block = kThreads >> p.lanes_log2;
+  set_groups(p, n_sets, 1);
+  const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, per_block)), p.group_end[2]);
+  bool vec = p.rot % 16 == 0;
+  const int64_t e = 16 / sizeof(T);
+  for (int i = 0; i < n_sets; ++i) {
+    const RowSet& r = p.set[i];
+    vec = vec && al16(r.src) && r.sh % e == 0 && r.ss % e == 0;
+    if (!r.paged) vec = vec && al16(r.dst) && r.dh % e == 0 && r.ds % e == 0;
+  }
+  return vec ? launch_pdl(append_e2m1_kernel<T, true>, grid, dim3(kThreads), 0, s, q, layout)
+             : launch_pdl(append_e2m1_kernel<T, false>, grid, dim3(kThreads), 0, s, q, layout);
+}
+
+template <typename T>
+cudaError_t run_read(ReadParams p, bool e2m1, cudaStream_t s) {
+  p.err = device_error_word();
+  if (p.err == nullptr) return cudaErrorInvalidDevice;
+  p.units = (p.dim + 15) / 16;
+  p.lanes_log2 = log2_ceil(p.units);
+  if (p.lanes_log2 > 5) p.lanes_log2 = 5;
+  const int per_block = kThreads >> p.lanes_log2;
+  const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, per_block)), p.heads, 2);
+  const int64_t e = 16 / sizeof(T);
+  bool vec = p.dim % 16 == 0;
+  for (int i = 0; i < 2; ++i) {
+    vec = vec && al16(p.dst[i]);
+    if (!e2m1) vec = vec && al16(p.src[i]) && p.page_stride[i] % e == 0 && p.head_stride[i] % e == 0;
+  }
+  if (e2m1)
+    return vec ? launch_pdl(read_kernel<T, true, true>, grid, dim3(kThreads), 0, s, p)
+               : launch_pdl(read_kernel<T, true, false>, grid, dim3(kThreads), 0, s, p);
+  return vec ? launch_pdl(read_kernel<T, false, true>, grid, dim3(kThreads), 0, s, p)
+             : launch_pdl(read_kernel<T, false, false>, grid, dim3(kThreads), 0, s, p);
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const lunarad_rotary_args& a, cudaStream_t stream) {
+  RowsParams p{};
+  p.set[0] = view_set(a.x, a.y, nullptr, a.heads);
+  p.positions = a.positions;
+  p.position_bytes = static_cast<int>(a.position_bytes);
+  p.position_batch_stride = a.position_batch_stride;
+  set_rotary(p, a.rotary);
+  p.dim = static_cast<int>(a.dim);
+  p.tokens = static_cast<int>(a.batch * a.seq);
+  p.seq = static_cast<int>(a.seq);
+  p.inverse = a.inverse != 0;
+  return run_rows_dtype<false, false>(p, 1, static_cast<int>(a.rotary.layout), a.dtype, stream);
+}
+
+cudaError_t launch_qk_norm_rotary(const lunarad_qk_norm_rotary_args& a, cudaStream_t stream) {
+  RowsParams p{};
+  p.set[0] = view_set(a.q, a.q_out, a.q_weight, a.q_heads);
+  p.set[1] = view_set(a.k, a.k_out, a.k_weight, a.k_heads);
+  p.positions = a.positions;
+  p.position_bytes = static_cast<int>(a.position_bytes);
+  p.position_batch_stride = a.position_batch_stride;
+  set_rotary(p, a.rotary);
+  p.dim = static_cast<int>(a.dim);
+  p.tokens = static_cast<int>(a.batch * a.seq);
+  p.seq = static_cast<int>(a.seq);
+  p.eps = static_cast<float>(a.eps);
+  return run_rows_dtype<true, false>(p, 2, static_cast<int>(a.rotary.layout), a.dtype, stream);
+}
+
+cudaError_t launch_kv_append(const lunarad_kv_append_args& a, cudaStream_t stream) {
+  const lunarad_cache& c = *a.cache;
+  const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
+  QuantParams q{};
+  RowsParams& p = q.r;
+  const lunarad_view none{};
+  int n = 0;
+  auto cache_set = [&](const lunarad_view& in, void* pages, int64_t ps, int64_t hs, void* scales, int64_t sps,
+                       int64_t shs, double gain, bool rotate) {
+    RowSet s = view_set(in, none, nullptr, c.kv_heads);
+    s.sb = 0;
+    s.dst = pages;
+    s.db = ps;
+    s.dh = hs;
+    s.ds = e2m1 ? c.dim / 2 : c.dim;
+    s.rotate = rotate && a.rotary.rot > 0;
+    s.paged = 1;
+    q.scales[n] = scales;
+    q.sc_page[n] = sps;
+    q.sc_head[n] = shs;
+    q.inv_gain[n] = 1.0f / static_cast<float>(gain);
+    p.set[n++] = s;
+  };
+  cache_set(a.k, c.k, c.k_page_stride, c.k_head_stride, c.k_scales, c.ks_page_stride, c.ks_head_stride, c.k_gain, true);
+  cache_set(a.v, c.v, c.v_page_stride, c.v_head_stride, c.v_scales, c.vs_page_stride, c.vs_head_stride, c.v_gain, false);
+  if (a.q_heads > 0) {
+    RowSet s = view_set(a.q, a.q_out, nullptr, a.q_heads);
+    s.sb = s.db = 0;
+    p.set[n++] = s;
+  }
+  p.seqs = make_seqs(a.seqs, c.page_size);
+  p.num_pages = static_cast<int>(c.num_pages);
+  set_rotary(p, a.rotary);
+  p.dim = static_cast<int>(c.dim);
+  p.tokens = static_cast<int>(a.seqs.tokens);
+  p.seq = p.tokens;
+  const int layout = static_cast<int>(a.rotary.layout);
+  if (!e2m1) return run_rows_dtype<false, true>(p, n, layout, a.dtype, stream);
+  if (a.dtype == LUNARA_F16) return run_quant<__half>(q, n, layout, stream);
+  if (a.dtype == LUNARA_BF16) return run_quant<__nv_bfloat16>(q, n, layout, stream);
+  return run_quant<float>(q, n, layout, stream);
+}
+
+cudaError_t launch_kv_read(const lunarad_kv_read_args& a, cudaStream_t stream) {
+  const lunarad_cache& c = *a.cache;
+  ReadParams p{};
+  p.seqs = make_seqs(a.seqs, c.page_size);
+  p.src[0] = c.k;
+  p.src[1] = c.v;
+  p.scales[0] = c.k_scales;
+  p.scales[1] = c.v_scales;
+  p.page_stride[0] = c.k_page_stride;
+  p.page_stride[1] = c.v_page_stride;
+  p.head_stride[0] = c.k_head_stride;
+  p.head_stride[1] = c.v_head_stride;
+  p.sc_page[0] = c.ks_page_stride;
+  p.sc_page[1] = c.vs_page_stride;
+  p.sc_head[0] = c.ks_head_stride;
+  p.sc_head[1] = c.vs_head_stride;
+  p.gain[0] = static_cast<float>(c.k_gain);
+  p.gain[1] = static_cast<float>(c.v_gain);
+  p.dst[0] = a.k_out;
+  p.dst[1] = a.v_out;
+  p.heads = static_cast<int>(c.kv_heads);
+  p.dim = static_cast<int>(c.dim);
+  p.num_pages = static_cast<int>(c.num_pages);
+  p.tokens = static_cast<int>(a.seqs.tokens);
+  const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
+  if (a.dtype == LUNARA_F16) return run_read<__half>(p, e2m1, stream);
+  if (a.dtype == LUNARA_BF16) return run_read<__nv_bfloat16>(p, e2m1, stream);
+  return run_read<float>(p, e2m1, stream);
+}
+
+}  // namespace lunara

@@ -23,6 +23,9 @@ ACT_NONE, ACT_RELU, ACT_GELU_ERF, ACT_GELU_TANH, ACT_SIGMOID, ACT_TANH = range(6
 BIN_ADD, BIN_MUL = 0, 1
 # lunara_b_layout
 B_KN, B_NK = 0, 1
+# lunarad_rotary_layout and the cache kind beside lunara_dtype
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+KIND_E2M1 = 16
 
 # Every exported symbol with its ctypes signature; the header declares exactly these.
 _p, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
@@ -58,6 +61,18 @@ SIGNATURES = {
     "lunara_version": ([], _i),
 }
 
+# Decoder operators, declared in include/lunara_b200_decoder.h: a struct of
+# arguments (packed by the caller) and a stream.
+_args = ctypes.c_char_p
+DECODER_SIGNATURES = {
+    "lunarad_rotary": ([_args, _p], _i),
+    "lunarad_qk_norm_rotary": ([_args, _p], _i),
+    "lunarad_kv_append": ([_args, _p], _i),
+    "lunarad_kv_read": ([_args, _p], _i),
+    "lunarad_paged_attention": ([_args, _p], _i),
+    "lunarad_paged_attention_workspace": ([_args], _i64),
+}
+
 # Internal self-test entry points, declared in include/lunara_b200_selftest.h
 # (not part of the kernel ABI; used by the tests only).
 SELFTEST_SIGNATURES = {
@@ -87,7 +102,7 @@ def load(path: os.PathLike | str | None = None) -> ctypes.CDLL:
         raise ImportError(
             f"lunara_b200 kernel library not found at {p}; build it with `python -m lunara_b200.build`")
     lib = ctypes.CDLL(str(p))
-    for name, (argtypes, restype) in {**SIGNATURES, **SELFTEST_SIGNATURES}.items():
+    for name, (argtypes, restype) in {**SIGNATURES, **DECODER_SIGNATURES, **SELFTEST_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = restype
@@ -102,6 +117,11 @@ def check(rc: int) -> None:
         if rc == ERR_INVALID_ARG:
             raise ValueError(f"[lunara status {rc}] {msg}")
         raise LunaraError(rc, msg)
+
+
+def address_of(packed: bytes) -> int:
+    """Address of a packed struct; valid as long as the caller keeps the bytes object."""
+    return ctypes.cast(ctypes.c_char_p(packed), ctypes.c_void_p).value
 
 
 def i64_array(values) -> ctypes.Array:

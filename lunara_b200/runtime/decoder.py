@@ -1,0 +1,344 @@
+"""Torch-facing decoder operators over the C ABI of ``include/lunara_b200_decoder.h``:
+rotary positions, per-head query/key norms with the rotation, the paged key/value cache
+and attention over it.
+
+As in ``lunara_b200.runtime.ops`` (which re-exports these), torch owns every buffer and
+the work is enqueued on torch's current stream, of the tensors' device. Shape errors raise
+``AssertionError``, library errors ``ValueError`` or ``LunaraError``. The operators are
+inference operators: they record no autograd graph (``rotary(..., inverse=True)`` is the
+gradient of ``rotary``).
+
+Ragged batches: the tokens of all sequences stand one behind the other;
+``seq_starts`` int32 [batch + 1] says where each sequence's begin, ``seq_lens`` int32
+[batch] how long each sequence is with them, ``page_table`` int32 [batch, max_pages] which
+page holds its positions ``page_size * i`` onwards. Token ``i`` of ``n`` has position
+``seq_len - n + i``; a negative one marks padding (written nowhere, zero in outputs).
+Tokens behind ``seq_starts[batch]`` belong to no sequence; their output rows are left as
+they were. All three live on the device, so a captured graph follows their contents. What
+is wrong in them (a page outside the cache, a position outside the tables) is kept as a
+device error (``ops.device_error()``) and treated as padding, never as an access out of
+bounds.
+"""
+from __future__ import annotations
+
+import math
+import struct
+from typing import Dict, Optional, Tuple
+
+import torch
+
+from lunara_b200.runtime import _lib
+from lunara_b200.runtime.kv_cache import PagedKVCache
+
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+_LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
+
+# The argument structs of the header: 8-byte fields, packed in one go (a ctypes.Structure
+# filled field by field costs several microseconds more per call).
+_ROTARY = struct.Struct("21q")
+_QK_NORM = struct.Struct("31qd")
+_APPEND = struct.Struct("30q")
+_READ = struct.Struct("11q")
+_ATTENTION = struct.Struct("22qd")
+
+
+def _dtype_code(t: torch.Tensor) -> int:
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"unsupported dtype {t.dtype}; expected float16, bfloat16 or float32") from None
+
+
+def _layout_code(layout: str) -> int:
+    try:
+        return _LAYOUTS[layout]
+    except KeyError:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}") from None
+
+
+def _check_device(device: torch.device, *ts: Optional[torch.Tensor]) -> None:
+    assert device.type == "cuda", "lunara kernels take CUDA tensors"
+    for t in ts:
+        if t is not None:
+            assert t.device == device, f"all tensors must be on {device}, got {t.device}"
+
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    lib = _lib.load()
+    if torch._C._cuda_getDevice() != device.index:
+        with torch.cuda.device(device):
+            return _call(name, args, device)
+    rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        _lib.check(rc)
+
+
+def _unit(t: torch.Tensor, name: str) -> None:
+    assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs a unit inner stride"
+
+
+def _view(t: torch.Tensor) -> Tuple[int, int, int, int]:
+    """lunarad_view of [batch, heads, seq, dim], or of [tokens, heads, dim]."""
+    st = t.stride()
+    if len(st) == 4:
+        return t.data_ptr(), st[0], st[1], st[2]
+    return t.data_ptr(), 0, st[1], st[0]
+
+
+def _writable(t: torch.Tensor, name: str) -> None:
+    for n, s in zip(t.shape, t.stride()):
+        assert s != 0 or n <= 1, f"{name} is an expanded view; it cannot be written"
+
+
+# ───────────────────────────────────────────────────────────── rotary ──
+
+def rotary_table(positions: int, rot_dim: int, base: float = 10000.0, scaling: Optional[Dict[str, float]] = None,
+                 device="cuda") -> torch.Tensor:
+    """The (cos, sin) table ``[positions, rot_dim / 2, 2]`` float32 that the rotary operators
+    read, computed in 64 bits (angles of far positions lose their digits in 32).
+
+    Frequency i is ``base ** (-2 i / rot_dim)``. ``scaling`` stretches a context:
+
+    * ``{"type": "linear", "factor": f}``: every frequency divided by f;
+    * ``{"type": "ntk", "factor": f}``: the base times ``f ** (rot_dim / (rot_dim - 2))``, which
+      keeps the fastest frequency and divides the slowest by f;
+    * ``{"type": "yarn", "factor": f, "original_positions": n, "beta_fast": 32, "beta_slow": 1,
+      "amplitude": a}``: frequencies that turn more than beta_fast times over the n original
+      positions are kept, those below beta_slow turns divided by f, with a linear ramp between;
+      cos and sin times a (default ``0.1 ln f + 1``).
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even and positive, got {rot_dim}")
+    if positions < 1:
+        raise ValueError(f"positions must be positive, got {positions}")
+    if not base > 1.0:
+        raise ValueError(f"base must be above 1, got {base}")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64, device=device)
+    amplitude = 1.0
+    kind = "none" if scaling is None else scaling.get("type")
+    if kind not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling type {kind!r}")
+    factor = 1.0 if kind == "none" else float(scaling["factor"])
+    if not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError(f"scaling factor must be at least 1, got {factor}")
+    if kind == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs a rot_dim above 2")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freq = base ** (-2.0 * i / rot_dim)
+    if kind == "linear":
+        freq = freq / factor
+    elif kind == "yarn":
+        original = float(scaling["original_positions"])
+        if not original > 0:
+            raise ValueError(f"original_positions must be positive, got {original}")
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        # The index whose frequency turns `turns` times over the original positions.
+        index = lambda turns: rot_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot_dim - 1)
+        ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        amplitude = float(scaling.get("amplitude", 0.1 * math.log(factor) + 1.0))
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.stack((angle.cos() * amplitude, angle.sin() * amplitude), dim=-1).to(torch.float32).contiguous()
+
+
+def _table(table: Optional[torch.Tensor], dim: int, layout: str) -> Tuple[int, int, int, int]:
+    code = _layout_code(layout)
+    if table is None:
+        return 0, 0, 0, code
+    assert table.dim() == 3 and table.shape[2] == 2 and table.dtype == torch.float32 and table.is_contiguous(), \
+        "table must be a contiguous float32 [positions, rot_dim / 2, 2] (rotary_table)"
+    rot = 2 * table.shape[1]
+    assert rot <= dim, f"the table rotates {rot} elements of a head of {dim}"
+    return table.data_ptr(), table.shape[0], rot, code
+
+
+def _positions(positions: torch.Tensor, batch: int, seq: int, rank: int) -> Tuple[int, int, int]:
+    if positions.dtype == torch.int64:
+        size = 8
+    else:
+        assert positions.dtype == torch.int32, "positions must be int32 or int64"
+        size = 4
+    shape = positions.shape
+    if len(shape) == 1:
+        assert shape[0] == seq, f"positions must be [{seq}], got {tuple(shape)}"
+        stride = 0
+    else:
+        assert rank == 4 and shape == (batch, seq), f"positions must be [{seq}] or [{batch}, {seq}], got {tuple(shape)}"
+        stride = positions.stride(0)
+    assert positions.stride(-1) == 1 or seq <= 1, "positions need a unit inner stride"
+    return positions.data_ptr(), size, stride
+
+
+def _dense(x: torch.Tensor, name: str) -> Tuple[int, int, int, int]:
+    """(batch, heads, seq, dim) of [B, H, S, D] or [tokens, H, D]."""
+    assert x.dim() in (3, 4), f"{name} must be [B, H, S, D] or [tokens, H, D]"
+    _unit(x, name)
+    s = x.shape
+    return (s[0], s[1], s[2], s[3]) if len(s) == 4 else (1, s[1], s[0], s[2])
+
+
+def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    assert out.shape == like.shape and out.dtype == like.dtype, f"{name} must be {tuple(like.shape)} {like.dtype}"
+    _unit(out, name)
+    _writable(out, name)
+    return out
+
+
+def rotary(X: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, layout: str = "half",
+           inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate the heads of X, [B, H, S, D] or [tokens, H, D] (any strides, unit inner one).
+
+    The pair (a, b) of frequency i becomes ``(a cos - b sin, b cos + a sin)`` with (cos, sin)
+    = ``table[position, i]``: elements (i, i + rot/2) in the "half" layout, (2i, 2i + 1) in the
+    "interleaved" one; elements from rot on pass through. fp32 arithmetic, one rounding.
+    ``positions`` int32 or int64, [S] or [B, S] ([tokens] for a 3-D X). ``out`` may be X.
+    ``inverse`` turns back (the gradient). A position outside the table records a device
+    error and its row is zero-filled."""
+    batch, heads, seq, dim = _dense(X, "X")
+    rot = _table(table, dim, layout)
+    assert table is not None, "rotary needs a table"
+    pos = _positions(positions, batch, seq, X.dim())
+    code = _dtype_code(X)
+    _check_device(X.device, positions, table, out)
+    out = _output(out, X, "out")
+    _call("lunarad_rotary", _ROTARY.pack(*_view(X), *_view(out), *pos, *rot, batch, heads, seq, dim, 1 if inverse else 0,
+                                         code), X.device)
+    return out
+
+
+def _weight(w: Optional[torch.Tensor], like: torch.Tensor, dim: int, name: str) -> int:
+    if w is None:
+        return 0
+    assert w.shape == (dim,) and w.dtype == like.dtype and w.is_contiguous(), f"{name} must be [{dim}] {like.dtype}, contiguous"
+    return w.data_ptr()
+
+
+def qk_norm_rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, table: Optional[torch.Tensor],
+                   q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   layout: str = "half", out_q: Optional[torch.Tensor] = None,
+                   out_k: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Normalise every head of Q and K, ``x / sqrt(mean(x^2) + eps) * weight``, and rotate it, in
+    one launch. Q [B, Hq, S, D] and K [B, Hk, S, D], or [tokens, H, D], any strides (views of a
+    fused projection); weights [D] or None; ``table=None`` normalises only. Statistics and
+    rotation in fp32, one rounding. Outputs may be the inputs."""
+    batch, q_heads, seq, dim = _dense(Q, "Q")
+    kb, k_heads, ks, kd = _dense(K, "K")
+    assert K.dim() == Q.dim() and (kb, ks, kd) == (batch, seq, dim), "Q and K must agree in batch, positions and head dim"
+    assert Q.dtype == K.dtype, "Q and K must share a dtype"
+    rot = _table(table, dim, layout)
+    pos = _positions(positions, batch, seq, Q.dim())
+    code = _dtype_code(Q)
+    _check_device(Q.device, K, positions, table, q_weight, k_weight, out_q, out_k)
+    wq, wk = _weight(q_weight, Q, dim, "q_weight"), _weight(k_weight, Q, dim, "k_weight")
+    out_q, out_k = _output(out_q, Q, "out_q"), _output(out_k, K, "out_k")
+    _call("lunarad_qk_norm_rotary", _QK_NORM.pack(*_view(Q), *_view(K), *_view(out_q), *_view(out_k), wq, wk, *pos, *rot, batch,
+                                                  q_heads, k_heads, seq, dim, code, eps), Q.device)
+    return out_q, out_k
+
+
+# ─────────────────────────────────────────────────── paged cache ──
+
+def _sequences(page_table: torch.Tensor, seq_starts: torch.Tensor, seq_lens: torch.Tensor, tokens: int,
+               device: torch.device) -> Tuple[int, ...]:
+    batch = seq_lens.shape[0]
+    assert page_table.dim() == 2 and page_table.shape[0] == batch and seq_lens.dim() == 1, \
+        "page_table must be [batch, max_pages] and seq_lens [batch]"
+    assert seq_starts.shape == (batch + 1,), f"seq_starts must be [{batch + 1}], got {tuple(seq_starts.shape)}"
+    for t, name in ((page_table, "page_table"), (seq_starts, "seq_starts"), (seq_lens, "seq_lens")):
+        assert t.dtype == torch.int32, f"{name} must be int32"
+        assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs a unit inner stride"
+        assert t.device == device, f"all tensors must be on {device}, got {t.device}"
+    return (page_table.data_ptr(), seq_starts.data_ptr(), seq_lens.data_ptr(), page_table.stride(0), page_table.shape[1],
+            batch, tokens)
+
+
+def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Tensor,
+              seq_lens: torch.Tensor, table: Optional[torch.Tensor] = None, layout: str = "half",
+              Q: Optional[torch.Tensor] = None, out_q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write the new tokens' K and V, [tokens, kv_heads, D] (any strides), to their pages, K
+    rotated at its position when a ``table`` is given. With Q [tokens, q_heads, D] the queries
+    are rotated in the same launch into ``out_q`` (which may be Q) and returned. ``seq_lens``
+    count the new tokens. A 4-bit cache gets the e2m1 codes and e4m3 scales of the values times
+    ``1 / gain``. Two tokens of one call must not share a slot (sequences may share pages that
+    nobody writes to)."""
+    tokens = K.shape[0]
+    dim = cache.head_dim
+    assert K.shape == (tokens, cache.kv_heads, dim) and V.shape == K.shape, \
+        f"K and V must be [tokens, {cache.kv_heads}, {dim}], got {tuple(K.shape)} and {tuple(V.shape)}"
+    assert V.dtype == K.dtype and (cache.dtype is None or K.dtype == cache.dtype), "K, V and the cache must share a dtype"
+    _unit(K, "K")
+    _unit(V, "V")
+    rot = _table(table, dim, layout)
+    code = _dtype_code(K)
+    device = cache.device
+    q_heads, q, o = 0, (0, 0, 0, 0), (0, 0, 0, 0)
+    if Q is not None:
+        assert Q.dim() == 3 and Q.shape[0] == tokens and Q.shape[2] == dim and Q.dtype == K.dtype, \
+            f"Q must be [{tokens}, q_heads, {dim}] {K.dtype}"
+        _unit(Q, "Q")
+        q_heads = Q.shape[1]
+    else:
+        assert out_q is None, "out_q without Q"
+    _check_device(device, K, V, table, Q, out_q)
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
+    if Q is not None:
+        out_q = _output(out_q, Q, "out_q")
+        q, o = _view(Q), _view(out_q)
+    _call("lunarad_kv_append", _APPEND.pack(*_view(K), *_view(V), *q, *o, cache._address, *seqs, *rot, q_heads, code), device)
+    return out_q
+
+
+def kv_read(cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Tensor, seq_lens: torch.Tensor, tokens: int,
+            dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the last ``seq_starts[b + 1] - seq_starts[b]`` positions of each
+    sequence as dense [tokens, kv_heads, D] tensors, in the cache's dtype (``dtype``, float16 by
+    default, for a 4-bit one)."""
+    if dtype is None:
+        dtype = torch.float16 if cache.dtype is None else cache.dtype
+    assert cache.dtype is None or dtype == cache.dtype, f"a {cache.dtype} cache is read as such, not as {dtype}"
+    assert tokens >= 0, "tokens must not be negative"
+    device = cache.device
+    _check_device(device)
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
+    k, v = (torch.empty(tokens, cache.kv_heads, cache.head_dim, dtype=dtype, device=device) for _ in range(2))
+    _call("lunarad_kv_read", _READ.pack(k.data_ptr(), v.data_ptr(), cache._address, *seqs, _dtype_code(k)), device)
+    return k, v
+
+
+def paged_attention(Q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Tensor,
+                    seq_lens: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                    max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(Q K^T * scale) V over the cached keys, for Q [tokens, q_heads, D] (any strides).
+
+    A token at position p sees the keys 0..p of its sequence, with ``window`` > 0 the last
+    ``window`` of them; its own key and value must be in the cache (``kv_append`` first). Query
+    head h reads key head ``h // (q_heads // kv_heads)``. ``scale`` defaults to ``1 / sqrt(D)``.
+    fp32 softmax; a row that sees no key is zero. ``max_q_len``, the most tokens any sequence
+    has here, is a hint that steers the choice of kernels (default: any number)."""
+    assert Q.dim() == 3 and Q.shape[2] == cache.head_dim, f"Q must be [tokens, q_heads, {cache.head_dim}], got {tuple(Q.shape)}"
+    tokens, q_heads, dim = Q.shape
+    assert cache.dtype is None or Q.dtype == cache.dtype, "Q and the cache must share a dtype"
+    assert q_heads > 0 and q_heads % cache.kv_heads == 0, f"{q_heads} query heads are no multiple of {cache.kv_heads} key heads"
+    _unit(Q, "Q")
+    code = _dtype_code(Q)
+    device = cache.device
+    _check_device(device, Q, out)
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
+    out = _output(out, Q, "out")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    head = (*_view(Q), *_view(out), cache._address, *seqs, q_heads, window, max_q_len or 0, code)
+    args = _ATTENTION.pack(*head, 0, 0, scale)
+    lib = _lib.load()
+    need = lib.lunarad_paged_attention_workspace(args)
+    if need < 0:
+        _lib.check(-need)
+    if need > 0:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        args = _ATTENTION.pack(*head, workspace.data_ptr(), need, scale)
+    _call("lunarad_paged_attention", args, device)
+    return out

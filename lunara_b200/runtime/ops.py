@@ -14,6 +14,10 @@ from typing import Optional, Sequence
 import torch
 
 from lunara_b200.runtime import _lib
+from lunara_b200.runtime.decoder import (  # noqa: F401  (decoder operators, re-exported)
+    kv_append, kv_read, paged_attention, qk_norm_rotary, rotary, rotary_table,
+)
+from lunara_b200.runtime.kv_cache import PagedKVCache  # noqa: F401
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
