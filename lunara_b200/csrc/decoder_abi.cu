@@ -113,7 +113,8 @@ int check_attention(const char* fn, const lunarad_paged_attention_args* a) {
   if (a->q_heads < 1 || a->q_heads % c.kv_heads != 0)
     return fail(LUNARA_ERR_INVALID_ARG, "%s: %lld query heads are no multiple of %lld key heads", fn,
                 (long long)a->q_heads, (long long)c.kv_heads);
-  if (a->q_heads > kMaxHeads) return fail(LUNARA_ERR_UNSUPPORTED, "%s: more than 65535 heads", fn);
+  if (a->q_heads > kMaxHeads || a->seqs.tokens * a->q_heads >= kMaxSlots)
+    return fail(LUNARA_ERR_UNSUPPORTED, "%s: more than 65535 heads or 2^31 query rows", fn);
   if (c.dim > 256) return fail(LUNARA_ERR_UNSUPPORTED, "%s: head dim %lld > 256", fn, (long long)c.dim);
   if (c.page_size * a->seqs.max_pages >= kMaxSlots)
     return fail(LUNARA_ERR_UNSUPPORTED, "%s: page table covers 2^31 positions or more", fn);

@@ -3,43 +3,42 @@
 //   O[t] = sum_j softmax_j(scale q_t . k_j) v_j   over the keys j that the
 //   query's position sees: j <= p, and with a window j > p - window.
 //
-// Simple kernel (any dtype and head dimension up to 256): one warp per query
-// token and head, lanes over the head dimension, one key after the other with
-// the running maximum and sum of the softmax in fp32.
+// Streaming kernel (16-bit and 4-bit caches): the query rows of one sequence
+// and key head (its tokens times the query heads of the group) make tiles of
+// 16 rows; their keys are cut into tiles of KT, and all tiles of the batch, in
+// the order (sequence, key head, row tile, key tile), are dealt to the warps of
+// a persistent grid in equal contiguous runs. Bound by HBM: a decode step reads
+// each cached byte once for group * 4 operations per element.
+//   * Every warp works alone (no block barrier after the start): it copies its
+//     tiles with cp.async into a ring of its own in shared memory. The order of
+//     the head dimension inside Q K^T and of the columns of V inside P V is
+//     free; it is chosen so that a lane's mma fragments are contiguous in
+//     memory, and no ldmatrix or swizzle is needed. With 16 bits each lane
+//     copies exactly the 16-byte pieces that it consumes itself.
+//   * S = Q K^T and O += P V by mma.sync m16n8k16 with fp32 accumulators. At
+//     16 rows these products need a fraction of the legacy tensor rate while
+//     HBM delivers its 23 bytes per clock and SM; tcgen05 needs 64 rows or more
+//     (paged_prefill.cu takes those).
+//   * The running maximum is raised only when a row's maximum grows by more
+//     than 2^8 (a warp vote), so O is rescaled a few times per row in all.
+//   * 4-bit caches: codes become f16 pairs by one cvt per pair, times their
+//     e4m3 scale by one half2 product, exactly (6 significant bits; 2^-10 ..
+//     2688); the products run in f16 whatever the queries' type. bf16 queries
+//     are brought into f16's range row by row with a power of two, which drops
+//     bits below 2^-24 of the row's largest element only.
+// Runs that cut a (sequence, key head, row tile) leave partial O, maximum and
+// sum in the workspace, and a second kernel joins them; all others write O. The
+// split depends on the lengths only, so results repeat bit for bit.
+//
+// Simple kernel (fp32, and head dimensions or strides the streaming kernel does
+// not take): one warp per query row, one key after the other.
+#include <type_traits>
+
 #include "kernels.h"
-#include "paged.cuh"
+#include "paged_attention.cuh"
 
 namespace lunara {
 namespace {
-
-struct PagedParams {
-  const void* q;
-  void* o;
-  int64_t q_head, q_tok, o_head, o_tok;   // strides
-  const void* k;
-  const void* v;
-  const void* ks;
-  const void* vs;
-  int64_t k_page, k_head, v_page, v_head, ks_page, ks_head, vs_page, vs_head;
-  int num_pages, kv_heads, page_size, dim, q_heads, group;
-  Seqs seqs;
-  int window;
-  float scale;   // softmax scale times the keys' gain
-  float v_gain;
-  unsigned int* err;
-};
-
-// The keys that a position sees, as [lo, hi), cut to the page table.
-__device__ __forceinline__ void visible(const PagedParams& p, int64_t pos, int& lo, int& hi) {
-  const int64_t cap = static_cast<int64_t>(p.seqs.max_pages) * p.page_size;
-  int64_t e = pos + 1;
-  if (e > cap) {
-    atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCachePosition));
-    e = cap;
-  }
-  hi = static_cast<int>(e);
-  lo = p.window > 0 && pos + 1 > p.window ? static_cast<int>(min(pos + 1 - p.window, e)) : 0;
-}
 
 constexpr int kSimpleThreads = 128;
 constexpr int kPer = 8;   // elements per lane: head dimension up to 256
@@ -75,8 +74,9 @@ __global__ void __launch_bounds__(kSimpleThreads) paged_simple_kernel(const __gr
     qv[e] = d < p.dim ? Io<T>::to_f(q[d]) * p.scale : 0.f;
     ov[e] = 0.f;
   }
-  int lo = 0, hi = 0;
-  if (pos >= 0) visible(p, pos, lo, hi);
+  int lo, hi;
+  visible(p, pos, lo, hi);
+  if (hi <= pos) atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCachePosition));
   float m = -INFINITY, l = 0.f;
   for (int j = lo; j < hi; ++j) {
     int slot;
@@ -114,20 +114,783 @@ __global__ void __launch_bounds__(kSimpleThreads) paged_simple_kernel(const __gr
   }
 }
 
+// ------------------------------------------------------- streaming kernel --
+constexpr int kRowTile = 16;
+constexpr int kWarps = 4;
+constexpr int kStreamThreads = 32 * kWarps;
+constexpr int kMaxBatch = 1024;          // sequences per launch (their prefix sums stand in shared memory)
+constexpr float kRescaleLog2 = 8.0f;
+
+// Sizes of one instance; DP is the head dimension rounded up to 64 or 128.
+template <bool E2M1, int DP>
+struct Shape {
+  static constexpr int KT = E2M1 || DP == 64 ? 32 : 16;   // keys per tile
+  static constexpr int kSteps = DP / 16;                  // k-steps of Q K^T
+  static constexpr int kCols = DP / 8;                    // n-tiles of P V
+  static constexpr int kRun = E2M1 ? DP / 8 : 8;          // neighbouring columns of V that a lane holds
+  // 16 bits: 16-byte pieces per lane and row. 4 bits: rows of DP / 2 bytes of
+  // codes; V's rows are padded so that the four rows that a quarter warp reads
+  // at once lie in different banks.
+  static constexpr int kKRow = E2M1 ? DP / 2 : 2 * DP;
+  static constexpr int kVRow = E2M1 ? DP / 2 + 16 : 2 * DP;
+  static constexpr int kKBytes = KT * kKRow, kVBytes = KT * kVRow;
+  static constexpr int kScaleBytes = E2M1 ? KT * (DP / 16) : 0;   // of K, and of V
+  static constexpr int kStageBytes = kKBytes + kVBytes + 2 * kScaleBytes;
+  static constexpr int kStages = 3;
+  static constexpr int kRingBytes = kStages * kStageBytes;        // per warp
+  static constexpr int kCtasPerSm = E2M1 ? 3 : 2;
+};
+
+// 16 bytes to shared memory, or zeros (then nothing is read).
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(a) : "memory");
+  return u;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 u;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(a) : "memory");
+  return u;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t u;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(a) : "memory");
+  return u;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t u;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
+  return u;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+  uint32_t u;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(a) : "memory");
+  return u;
+}
+
+// D += A B, m16n8k16: A row-major, B column-major, 16-bit, fp32 accumulators.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// The four bytes of codes in w as f16 pairs.
+__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 t0, t1, t2, t3;\n\t"
+      "mov.b32 {t0, t1, t2, t3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, t0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, t1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, t2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, t3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// Two e4m3 bytes as an f16 pair.
+__device__ __forceinline__ uint32_t scales_to_half2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
+  return r;
+}
+
+// Row tiles of a sequence, and the key tiles of each of them.
+__device__ __forceinline__ void seq_tiles(const PagedParams& p, const SeqInfo& s, int KT, int& row_tiles, int& tiles) {
+  const int64_t rows = static_cast<int64_t>(s.n) * p.group;
+  if (rows < p.min_rows || rows >= p.max_rows || s.hi <= s.lo) {
+    row_tiles = tiles = 0;
+    return;
+  }
+  row_tiles = static_cast<int>((rows + kRowTile - 1) / kRowTile);
+  tiles = (s.hi + KT - 1) / KT - s.lo / KT;
+}
+
+// prefix[b] = tiles of the sequences before b (batch + 1 entries in shared
+// memory), by the whole block.
+__device__ __forceinline__ void prefix_tiles(const PagedParams& p, int KT, int64_t* prefix, int64_t* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int64_t carry = 0;
+  for (int b0 = 0; b0 < p.seqs.batch; b0 += blockDim.x) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    int64_t x = 0;
+    if (b < p.seqs.batch) {
+      int rt, nt;
+      seq_tiles(p, load_seq(p, b), KT, rt, nt);
+      x = static_cast<int64_t>(p.kv_heads) * rt * nt;
+    }
+    int64_t inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    int64_t before = carry, all = 0;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += warp_sums[w];
+      all += warp_sums[w];
+    }
+    if (b < p.seqs.batch) prefix[b + 1] = before + inc;
+    carry += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+}
+
+// Worker w of `workers` takes the tiles [run_start(w), run_start(w + 1)); there
+// are never more workers than tiles, so that none of them has an empty run (the
+// join reads a part of every worker between a row's first and last one).
+__device__ __forceinline__ int used_workers(const PagedParams& p, int64_t total) {
+  return static_cast<int>(min(total, static_cast<int64_t>(p.workers)));
+}
+__device__ __forceinline__ int64_t run_start(int64_t total, int workers, int w) { return total * w / workers; }
+// The worker whose run holds tile t.
+__device__ __forceinline__ int run_of(int64_t total, int workers, int64_t t) {
+  return static_cast<int>(((t + 1) * workers + total - 1) / total) - 1;
+}
+
+template <typename T, bool E2M1, int DP>
+__global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
+    paged_stream_kernel(const __grid_constant__ PagedParams p) {
+  using S = Shape<E2M1, DP>;
+  using M = typename std::conditional<E2M1, __half, T>::type;   // type of the products
+  constexpr int KT = S::KT;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int64_t warp_sums[kWarps];
+  int64_t* prefix = reinterpret_cast<int64_t*>(smem + kWarps * S::kRingBytes);
+  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * S::kRingBytes;
+  pdl_wait();
+  pdl_launch_dependents();
+  prefix_tiles(p, KT, prefix, warp_sums);
+  const int64_t total = prefix[p.seqs.batch];
+  const int workers = used_workers(p, total), worker = static_cast<int>(blockIdx.x) * kWarps + warp;
+  if (worker >= workers) return;
+  const int64_t t_first = run_start(total, workers, worker), t_end = run_start(total, workers, worker + 1);
+  const bool grouped = E2M1 || (p.page_size & 7) == 0;   // 8 neighbouring keys stand in one page
+  constexpr int kElem = E2M1 ? 1 : 2;
+  const int row_bytes = E2M1 ? p.dim / 2 : p.dim * 2;
+  const int64_t k_page = p.k_page * kElem, v_page = p.v_page * kElem;
+
+  for (int64_t t = t_first; t < t_end;) {
+    // ------------------------------------------------ where the run stands --
+    int b = 0;
+    for (int end = p.seqs.batch; b + 1 < end;) {   // last b with prefix[b] <= t
+      const int mid = (b + end) >> 1;
+      if (prefix[mid] <= t) b = mid; else end = mid;
+    }
+    const SeqInfo s = load_seq(p, b);
+    int row_tiles, seg_tiles;
+    seq_tiles(p, s, KT, row_tiles, seg_tiles);
+    const int64_t in_seq = t - prefix[b];
+    const int seg = static_cast<int>(in_seq / seg_tiles);
+    const int tile0 = static_cast<int>(in_seq - static_cast<int64_t>(seg) * seg_tiles);
+    const int kh = seg / row_tiles, rt = seg - kh * row_tiles;
+    const int n_tiles = static_cast<int>(min(static_cast<int64_t>(seg_tiles - tile0), t_end - t));
+    const int key0 = (s.lo / KT + tile0) * KT;
+    const int rows = min(kRowTile, s.n * p.group - rt * kRowTile);
+
+    // This lane's rows g and g + 8: their token, head and visible keys.
+    int tok[2], head[2], lo[2], hi[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = rt * kRowTile + min(g + 8 * r, rows - 1);
+      const int i = row / p.group;
+      tok[r] = s.first + i;
+      head[r] = kh * p.group + row - i * p.group;
+      visible(p, s.pos0 + i, lo[r], hi[r]);
+    }
+    // Keys that some row sees, and that all rows see.
+    int any_lo, any_hi, all_lo, all_hi;
+    visible(p, s.pos0 + (rt * kRowTile + rows - 1) / p.group, all_lo, any_hi);
+    visible(p, s.pos0 + rt * kRowTile / p.group, any_lo, all_hi);
+
+    // -------------------------------------------------------------- pages --
+    // Lane l holds the page of the l-th group of 8 keys of a batch of 256
+    // (grouped) or of the l-th key of a tile; the next batch is loaded ahead.
+    const int32_t* table = p.seqs.page_table + b * p.seqs.table_stride;
+    auto load_pages = [&](int first) {
+      const int key = grouped ? first + 8 * lane : first + lane;
+      if (key + (grouped ? 8 : 1) <= any_lo || key >= any_hi) return -1;   // nothing of it is read
+      const int page = table[p.seqs.page_div.div(key)];
+      if (page >= 0 && page < p.num_pages) return page;
+      atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCachePage));
+      return -1;
+    };
+    const int batch_keys = grouped ? 256 : KT;
+    int batch0 = key0;
+    int pages = load_pages(batch0), pages_next = load_pages(batch0 + batch_keys);
+
+    const char* kb = static_cast<const char*>(p.k) + kh * p.k_head * kElem;
+    const char* vb = static_cast<const char*>(p.v) + kh * p.v_head * kElem;
+
+    // Starts the copies of tile i into its stage; returns a bit for each of its
+    // keys that takes part. All others are zero-filled: neither a stale slot's
+    // NaN nor a bad page may reach a product.
+    auto issue = [&](int i, int stage) -> uint32_t {
+      const int first = key0 + i * KT;
+      if (first - batch0 >= batch_keys) {
+        batch0 += batch_keys;
+        pages = pages_next;
+        pages_next = load_pages(batch0 + batch_keys);
+      }
+      const int g0 = (first - batch0) >> 3;   // grouped: the tile's first group in the batch
+      uint32_t ok = __ballot_sync(0xffffffffu, pages >= 0);
+      if (grouped) {
+        const uint32_t x = (ok >> g0) & ((1u << (KT / 8)) - 1u);   // a bit for each group -> a byte
+        ok = ((x & 1u) | ((x & 2u) << 7) | ((x & 4u) << 14) | ((x & 8u) << 21)) * 0xFFu;
+      }
+      if (any_lo > first) ok &= any_lo - first < 32 ? ~0u << (any_lo - first) : 0u;
+      if (any_hi < first + 32) ok &= any_hi > first ? (1u << (any_hi - first)) - 1u : 0u;
+      if (KT < 32) ok &= (1u << (KT & 31)) - 1u;
+      const uint32_t at = ring + stage * S::kStageBytes;
+      // Page and slot of the group (grouped) or key at `local`.
+      auto place = [&](int local, int64_t& page, int& slot) {
+        const int pg = __shfl_sync(0xffffffffu, pages, grouped ? g0 + (local >> 3) : local);
+        const int key = first + (grouped ? local & ~7 : local);
+        slot = key - p.seqs.page_div.div(key) * p.page_size + (grouped ? local & 7 : 0);
+        page = max(pg, 0);
+      };
+      if constexpr (E2M1) {
+        constexpr int kPieces = DP / 32;   // 16-byte pieces of a row of codes
+        const uint8_t* ksb = static_cast<const uint8_t*>(p.ks) + kh * p.ks_head;
+        const uint8_t* vsb = static_cast<const uint8_t*>(p.vs) + kh * p.vs_head;
+#pragma unroll
+        for (int j = 0; j < KT * kPieces / 32; ++j) {
+          const int q = lane + 32 * j, local = q / kPieces, off = 16 * (q % kPieces);
+          int64_t page;
+          int slot;
+          place(local, page, slot);
+          const bool in = ((ok >> local) & 1u) != 0u && off < row_bytes;
+          const int at_row = slot * row_bytes + off;
+          copy_async(at + local * S::kKRow + off, in ? kb + page * k_page + at_row : kb, in);
+          copy_async(at + S::kKBytes + local * S::kVRow + off, in ? vb + page * v_page + at_row : vb, in);
+        }
+        // Scales: those of a group of 8 keys are srow / 2 pieces of 16 bytes.
+        // A group with a masked key is copied whole: scales of masked keys
+        // multiply zeroed codes, and are cleared where they are read.
+        const int srow = p.dim / 16;
+        constexpr int kScalePieces = DP / 32;   // per group
+        constexpr int kAll = 2 * (KT / 8) * kScalePieces;
+        const int kv = lane / (kAll / 2), rest = lane % (kAll / 2), grp = rest / kScalePieces, piece = rest % kScalePieces;
+        int64_t page;
+        int slot;
+        place(8 * (grp & (KT / 8 - 1)), page, slot);
+        if (lane < kAll) {
+          const bool in = ((ok >> (8 * grp)) & 0xFFu) != 0u && 16 * piece < 8 * srow;
+          const uint8_t* src = kv == 0 ? ksb + page * p.ks_page : vsb + page * p.vs_page;
+          copy_async(at + S::kKBytes + S::kVBytes + kv * S::kScaleBytes + grp * (8 * srow) + 16 * piece,
+                         in ? src + slot * srow + 16 * piece : static_cast<const uint8_t*>(p.ks), in);
+        }
+      } else {
+        // K row 8 i + g: pieces c, c + 4, ...; V rows 16 a + 8 h + 2 c + e
+        // (the lane's keys of an mma k-step): pieces g, g + 8.
+#pragma unroll
+        for (int i8 = 0; i8 < KT / 8; ++i8) {
+          int64_t page;
+          int slot;
+          place(8 * i8 + g, page, slot);
+          const bool use = ((ok >> (8 * i8 + g)) & 1u) != 0u;
+          const char* src = kb + page * k_page + slot * row_bytes + 16 * c;
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j) {
+            const bool in = use && 16 * (c + 4 * j) < row_bytes;
+            copy_async(at + ((i8 * (DP / 32) + j) * 32 + lane) * 16, in ? src + 64 * j : kb, in);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int local = 8 * i8 + 2 * c + e;
+            place(local, page, slot);
+            const bool vuse = ((ok >> local) & 1u) != 0u;
+            const char* vsrc = vb + page * v_page + slot * row_bytes + 16 * g;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+              const bool in = vuse && 16 * (g + 8 * j) < row_bytes;
+              copy_async(at + S::kKBytes + (((2 * i8 + e) * (DP / 64) + j) * 32 + lane) * 16, in ? vsrc + 128 * j : vb, in);
+            }
+          }
+        }
+      }
+      copy_commit();
+      return ok;
+    };
+
+    uint32_t ok_of[S::kStages];   // of the tiles in flight, oldest first
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      ok_of[i] = 0u;
+      if (i < n_tiles) ok_of[i] = issue(i, i);
+      else copy_commit();
+    }
+
+    // ------------------------------------------------------------ queries --
+    uint32_t qf[S::kSteps][4];
+    float sl2[2];
+    // The maximum below needs a positive factor: a negative scale turns the
+    // queries' signs instead, and a zero one becomes too small to matter.
+    sl2[0] = sl2[1] = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    {
+      const T* q0 = static_cast<const T*>(p.q) + tok[0] * p.q_tok + head[0] * p.q_head;
+      const T* q1 = static_cast<const T*>(p.q) + tok[1] * p.q_tok + head[1] * p.q_head;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        // The lane's i-th 8 elements: with 16 bits pieces c + 4 i of K's rows,
+        // with 4 bits its i-th word of DP / 32 neighbouring ones.
+        const int d = E2M1 ? (DP / 4) * c + 8 * i : 8 * (c + 4 * i);
+        uint4 u0 = make_uint4(0u, 0u, 0u, 0u), u1 = u0;
+        if (d < p.dim) {
+          u0 = *reinterpret_cast<const uint4*>(q0 + d);
+          u1 = *reinterpret_cast<const uint4*>(q1 + d);
+          u0.x ^= flip; u0.y ^= flip; u0.z ^= flip; u0.w ^= flip;
+          u1.x ^= flip; u1.y ^= flip; u1.z ^= flip; u1.w ^= flip;
+        }
+        qf[2 * i][0] = u0.x; qf[2 * i][1] = u1.x; qf[2 * i][2] = u0.y; qf[2 * i][3] = u1.y;
+        qf[2 * i + 1][0] = u0.z; qf[2 * i + 1][1] = u1.z; qf[2 * i + 1][2] = u0.w; qf[2 * i + 1][3] = u1.w;
+      }
+      if constexpr (E2M1 && std::is_same<T, __nv_bfloat16>::value) {
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < S::kSteps; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Io<T>::unpack2(qf[w][i]);
+            top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        float down[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          // 2^-e for 2^e <= top < 2^(e + 1), whose scale goes to the scores;
+          // rows of zeros and rows at fp32's ends stay as they are.
+          const uint32_t e = __float_as_uint(top[r]) >> 23;
+          const bool use = e > 64u && e < 190u;
+          down[r] = use ? __uint_as_float((254u - e) << 23) : 1.f;
+          sl2[r] *= use ? __uint_as_float(e << 23) : 1.f;
+        }
+#pragma unroll
+        for (int w = 0; w < S::kSteps; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Io<T>::unpack2(qf[w][i]);
+            qf[w][i] = Io<__half>::pack2(f.x * down[i & 1], f.y * down[i & 1]);
+          }
+      }
+    }
+
+    // ---------------------------------------------------------- key tiles --
+    float acc[S::kCols][4];
+#pragma unroll
+    for (int j = 0; j < S::kCols; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // maximum (scaled, log2) and this lane's part of the sum
+
+    int stage = 0;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int ahead = stage == 0 ? S::kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
+      if (i + S::kStages - 1 < n_tiles) ok_of[S::kStages - 1] = issue(i + S::kStages - 1, ahead);
+      else {
+        ok_of[S::kStages - 1] = 0u;
+        copy_commit();
+      }
+      copy_wait<S::kStages - 1>();
+      if constexpr (E2M1) __syncwarp();   // rows copied by other lanes
+      const uint32_t ok = ok_of[0];
+#pragma unroll
+      for (int k = 0; k + 1 < S::kStages; ++k) ok_of[k] = ok_of[k + 1];
+      const uint32_t at = ring + stage * S::kStageBytes;
+      const int first = key0 + i * KT;
+      if (ok != 0u) {
+        // S = Q K^T
+        float sc[KT / 8][4];
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+        if constexpr (E2M1) {
+          const int srow = p.dim / 16;
+          const uint32_t ks_at = at + S::kKBytes + S::kVBytes;
+#pragma unroll
+          for (int n = 0; n < KT / 8; ++n) {
+            const uint32_t row = at + (8 * n + g) * S::kKRow;
+            if constexpr (DP == 128) {
+              const uint32_t two = 2 * c < srow ? lds16(ks_at + (8 * n + g) * srow + 2 * c) : 0u;
+              const uint32_t s01 = scales_to_half2(two);
+              const uint32_t s0 = __byte_perm(s01, s01, 0x1010), s1 = __byte_perm(s01, s01, 0x3232);
+              const uint4 w = lds128(row + 16 * c);
+              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t h[4];
+                codes_to_half2(ws[q], h);
+                const uint32_t sx = q < 2 ? s0 : s1;
+                mma16816<M>(sc[n], qf[2 * q], hmul2(h[0], sx), hmul2(h[1], sx));
+                mma16816<M>(sc[n], qf[2 * q + 1], hmul2(h[2], sx), hmul2(h[3], sx));
+              }
+            } else {
+              const uint32_t one = c < srow ? lds8(ks_at + (8 * n + g) * srow + c) : 0u;
+              const uint32_t sx = scales_to_half2(one * 0x101u);
+              const uint2 w = lds64(row + 8 * c);
+              const uint32_t ws[2] = {w.x, w.y};
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t h[4];
+                codes_to_half2(ws[q], h);
+                mma16816<M>(sc[n], qf[2 * q], hmul2(h[0], sx), hmul2(h[1], sx));
+                mma16816<M>(sc[n], qf[2 * q + 1], hmul2(h[2], sx), hmul2(h[3], sx));
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+            for (int n = 0; n < KT / 8; ++n) {
+              const uint4 u = lds128(at + ((n * (DP / 32) + j) * 32 + lane) * 16);
+              mma16816<M>(sc[n], qf[2 * j], u.x, u.y);
+              mma16816<M>(sc[n], qf[2 * j + 1], u.z, u.w);
+            }
+        }
+        // Masks, where the tile has a key that not every row sees. (A key
+        // column n, 2 c + e stands at 8 n + 2 c + e.)
+        constexpr uint32_t kFull = KT == 32 ? ~0u : (1u << (KT & 31)) - 1u;
+        if (ok != kFull || first < all_lo || first + KT > all_hi) {
+#pragma unroll
+          for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int local = 8 * n + 2 * c + (e & 1), key = first + local;
+              if (((ok >> local) & 1u) == 0u || key < lo[e >> 1] || key >= hi[e >> 1]) sc[n][e] = -INFINITY;
+            }
+        }
+        // Running maximum; NaN propagates, so a NaN score makes its row NaN.
+        float top[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < KT / 8; ++n) x = fmax3_nan(x, sc[n][2 * r], sc[n][2 * r + 1]);
+          x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          top[r] = x * sl2[r];
+        }
+        const bool grown = !(top[0] <= m[0] + kRescaleLog2) || !(top[1] <= m[1] + kRescaleLog2);
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float next = fmax_nan(m[r], top[r]);
+            const float alpha = next == -INFINITY ? 1.f : ex2_approx(m[r] - next);
+            m[r] = next;
+            l[r] *= alpha;
+#pragma unroll
+            for (int j = 0; j < S::kCols; ++j) {
+              acc[j][2 * r] *= alpha;
+              acc[j][2 * r + 1] *= alpha;
+            }
+          }
+        }
+        const float off0 = m[0] == -INFINITY ? 0.f : m[0], off1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+        for (int n = 0; n < KT / 8; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] = ex2_approx(fmaf(sc[n][e], sl2[e >> 1], e < 2 ? -off0 : -off1));
+          l[0] += sc[n][0] + sc[n][1];
+          l[1] += sc[n][2] + sc[n][3];
+        }
+        // O += P V
+#pragma unroll
+        for (int a = 0; a < KT / 16; ++a) {
+          const uint32_t pf[4] = {Io<M>::pack2(sc[2 * a][0], sc[2 * a][1]), Io<M>::pack2(sc[2 * a][2], sc[2 * a][3]),
+                                  Io<M>::pack2(sc[2 * a + 1][0], sc[2 * a + 1][1]),
+                                  Io<M>::pack2(sc[2 * a + 1][2], sc[2 * a + 1][3])};
+          if constexpr (E2M1) {
+            const int srow = p.dim / 16;
+            const uint32_t vs_at = at + S::kKBytes + S::kVBytes + S::kScaleBytes;
+            const int block = DP == 128 ? g : g >> 1;   // of this lane's columns
+            uint32_t sx[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = 16 * a + 8 * h + 2 * c;
+              const uint32_t b0 = block < srow && ((ok >> key) & 1u) ? lds8(vs_at + key * srow + block) : 0u;
+              const uint32_t b1 = block < srow && ((ok >> (key + 1)) & 1u) ? lds8(vs_at + (key + 1) * srow + block) : 0u;
+              sx[h] = scales_to_half2(b0 | (b1 << 8));
+            }
+            constexpr int kW = DP / 64;   // words of codes per lane and key
+            uint32_t w[2][2][kW];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t row = at + S::kKBytes + (16 * a + 8 * h + 2 * c + e) * S::kVRow + (DP / 16) * g;
+                if constexpr (DP == 128) {
+                  const uint2 u = lds64(row);
+                  w[h][e][0] = u.x;
+                  w[h][e][1] = u.y;
+                } else {
+                  w[h][e][0] = lds32(row);
+                }
+              }
+#pragma unroll
+            for (int q = 0; q < kW; ++q) {
+              // Bytes that pair the codes of two keys: even and odd columns.
+              uint32_t ev[2][4], od[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t x = w[h][0][q], y = w[h][1][q];
+                codes_to_half2((x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u), ev[h]);
+                codes_to_half2(((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), od[h]);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                mma16816<M>(acc[8 * q + 2 * j], pf, hmul2(ev[0][j], sx[0]), hmul2(ev[1][j], sx[1]));
+                mma16816<M>(acc[8 * q + 2 * j + 1], pf, hmul2(od[0][j], sx[0]), hmul2(od[1][j], sx[1]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+              uint32_t w[4][4];   // [key][word]
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint4 u = lds128(at + S::kKBytes + (((4 * a + e) * (DP / 64) + j) * 32 + lane) * 16);
+                w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                mma16816<M>(acc[8 * j + 2 * q], pf, __byte_perm(w[0][q], w[1][q], 0x5410),
+                            __byte_perm(w[2][q], w[3][q], 0x5410));
+                mma16816<M>(acc[8 * j + 2 * q + 1], pf, __byte_perm(w[0][q], w[1][q], 0x7632),
+                            __byte_perm(w[2][q], w[3][q], 0x7632));
+              }
+            }
+          }
+        }
+      }
+      if constexpr (E2M1) __syncwarp();   // the stage may be written again
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    }
+    copy_wait<0>();
+
+    // ------------------------------------------------------------- results --
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    const bool whole = tile0 == 0 && n_tiles == seg_tiles;
+    const int64_t part = static_cast<int64_t>(worker) * 2 + (t == t_first ? 0 : 1);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (g + 8 * r < rows) {
+        const float f = whole ? (l[r] == 0.f ? 0.f : p.v_gain / l[r]) : 1.f;
+        T* out = static_cast<T*>(p.o) + tok[r] * p.o_tok + head[r] * p.o_head;
+        float* po = p.part_o + (part * kRowTile + g + 8 * r) * DP;
+        // Column n = 2 c + e of the n-tile j is element 64 i + kRun n + (j % kRun), j = kRun i + ...
+#pragma unroll
+        for (int i = 0; i < S::kCols / S::kRun; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int d8 = 0; d8 < S::kRun; d8 += 8) {
+              const int d = 64 * i + S::kRun * (2 * c + e) + d8;
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = l[r] == 0.f ? 0.f : acc[S::kRun * i + d8 + k][2 * r + e] * f;
+              if (whole) {
+                if (d < p.dim)
+                  *reinterpret_cast<uint4*>(out + d) = make_uint4(Io<T>::pack2(x[0], x[1]), Io<T>::pack2(x[2], x[3]),
+                                                                  Io<T>::pack2(x[4], x[5]), Io<T>::pack2(x[6], x[7]));
+              } else {
+                *reinterpret_cast<float4*>(po + d) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(po + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+              }
+            }
+        if (!whole && c == 0)
+          *reinterpret_cast<float2*>(p.part_ml + (part * kRowTile + g + 8 * r) * 2) = make_float2(m[r], l[r]);
+      }
+    }
+    t += n_tiles;
+  }
+}
+
+// Joins the parts of the rows whose keys several workers took, and clears the
+// rows of sequences without keys. One block per query row. The lengths are
+// read before the streaming kernel has ended (it has started, so whatever
+// came before it is complete), the parts after it.
+constexpr int kJoinThreads = 128;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int KT) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int64_t warp_sums[kJoinThreads / 32];
+  __shared__ float s_o[kJoinThreads / 32][DP];
+  __shared__ float2 s_ml[kJoinThreads / 32];
+  int64_t* prefix = reinterpret_cast<int64_t*>(smem);
+  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+  constexpr int kWarpsHere = kJoinThreads / 32, kE = DP / 32;
+  prefix_tiles(p, KT, prefix, warp_sums);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int token = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), kh = h / p.group;
+  int b;
+  int64_t pos;
+  if (!find_token(p.seqs, token, b, pos)) return;
+  const SeqInfo s = load_seq(p, b);
+  const int64_t rows = static_cast<int64_t>(s.n) * p.group;
+  if (rows < p.min_rows || rows >= p.max_rows) return;
+  int row_tiles, seg_tiles;
+  seq_tiles(p, s, KT, row_tiles, seg_tiles);
+  T* out = static_cast<T*>(p.o) + token * p.o_tok + h * p.o_head;
+  if (seg_tiles == 0) {
+    for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) out[d] = Io<T>::from_f(0.f);
+    return;
+  }
+  const int row = (token - s.first) * p.group + h - kh * p.group;
+  const int64_t total = prefix[p.seqs.batch];
+  const int64_t t0 = prefix[b] + (static_cast<int64_t>(kh) * row_tiles + row / kRowTile) * seg_tiles;
+  const int workers = used_workers(p, total);
+  const int w0 = run_of(total, workers, t0), w1 = run_of(total, workers, t0 + seg_tiles - 1);
+  if (w0 == w1) return;   // written by its worker
+  const int first_slot = run_start(total, workers, w0) == t0 ? 0 : 1;
+  // Each warp joins every fourth part; the lane holds elements 4 lane .. (or 2 lane ..).
+  float m = -INFINITY, l = 0.f, o[kE];
+#pragma unroll
+  for (int e = 0; e < kE; ++e) o[e] = 0.f;
+  for (int w = w0 + warp; w <= w1; w += kWarpsHere) {
+    const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * kRowTile + row % kRowTile;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+    float x[kE];
+    if constexpr (kE == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
+      x[0] = v.x; x[1] = v.y;
+    }
+    const float next = fmax_nan(m, ml.x);
+    const float base = next == -INFINITY ? 0.f : next;
+    const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
+    l = l * fa + ml.y * fb;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
+    m = next;
+  }
+#pragma unroll
+  for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
+  if (lane == 0) s_ml[warp] = make_float2(m, l);
+  __syncthreads();
+  float top = s_ml[0].x;
+#pragma unroll
+  for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, f[kWarpsHere];
+#pragma unroll
+  for (int w = 0; w < kWarpsHere; ++w) {
+    f[w] = ex2_approx(s_ml[w].x - base);
+    sum += s_ml[w].y * f[w];
+  }
+  const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
+  for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
+    out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
+  }
+}
+
+// ------------------------------------------------------------------- host --
 template <typename T, bool E2M1>
 cudaError_t run_simple(const PagedParams& p, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(ceil_div64(p.seqs.tokens, kSimpleThreads / 32)), p.q_heads);
   return launch_pdl(paged_simple_kernel<T, E2M1>, grid, dim3(kSimpleThreads), 0, s, p);
 }
 
+int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
+int stream_workers(bool e2m1) { return device_num_sms() * kWarps * (e2m1 ? 3 : 2); }
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// 16-byte copies of whole rows: aligned bases and strides, rows of 16-byte
+// pieces; for 4 bits also pages of whole groups of 8 keys.
+bool stream_ok(const lunarad_paged_attention_args& a) {
+  const lunarad_cache& c = *a.cache;
+  const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
+  if (a.dtype == LUNARA_F32 || c.dim > 128) return false;
+  if (!al16(a.q.data) || a.q.head_stride % 8 || a.q.seq_stride % 8) return false;
+  if (!al16(a.o.data) || a.o.head_stride % 8 || a.o.seq_stride % 8) return false;
+  if (!al16(c.k) || !al16(c.v)) return false;
+  const int64_t vec = e2m1 ? 16 : 8;
+  if (c.k_page_stride % vec || c.k_head_stride % vec || c.v_page_stride % vec || c.v_head_stride % vec) return false;
+  if (!e2m1) return c.dim % 8 == 0;
+  return c.dim % 32 == 0 && c.page_size % 8 == 0 && al16(c.k_scales) && al16(c.v_scales) && c.ks_page_stride % 16 == 0 &&
+         c.ks_head_stride % 16 == 0 && c.vs_page_stride % 16 == 0 && c.vs_head_stride % 16 == 0;
+}
+
+template <typename T, bool E2M1, int DP>
+cudaError_t run_stream(PagedParams p, cudaStream_t s) {
+  using S = Shape<E2M1, DP>;
+  const size_t prefix = sizeof(int64_t) * (static_cast<size_t>(p.seqs.batch < kMaxBatch ? p.seqs.batch : kMaxBatch) + 2);
+  const size_t smem = static_cast<size_t>(kWarps) * S::kRingBytes + prefix;
+  static_assert(kWarps * S::kRingBytes + 8 * (kMaxBatch + 2) + 1280 <= 228 * 1024 / S::kCtasPerSm, "shared memory per SM");
+  auto kern = paged_stream_kernel<T, E2M1, DP>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kWarps * S::kRingBytes + 8 * (kMaxBatch + 2));
+  if (e != cudaSuccess) return e;
+  const int batch = p.seqs.batch;
+  const Seqs all = p.seqs;
+  for (int b0 = 0; b0 < batch; b0 += kMaxBatch) {   // more sequences than the prefix sums hold: one after the other
+    p.seqs.batch = batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch;
+    p.seqs.page_table = all.page_table + b0 * all.table_stride;
+    p.seqs.starts = all.starts + b0;
+    p.seqs.lens = all.lens + b0;
+    e = launch_pdl(kern, dim3(p.workers / kWarps), dim3(kStreamThreads), smem, s, p);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(paged_join_kernel<T, DP>, dim3(p.seqs.tokens, p.q_heads), dim3(kJoinThreads), prefix, s, p, S::KT);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
 template <typename T>
-cudaError_t run(const PagedParams& p, bool e2m1, cudaStream_t s) {
+cudaError_t run(const PagedParams& p, bool stream_kernel, bool e2m1, cudaStream_t s) {
+  if constexpr (!std::is_same<T, float>::value) {
+    if (stream_kernel) {
+      if (e2m1) return p.dim <= 64 ? run_stream<T, true, 64>(p, s) : run_stream<T, true, 128>(p, s);
+      return p.dim <= 64 ? run_stream<T, false, 64>(p, s) : run_stream<T, false, 128>(p, s);
+    }
+  }
   return e2m1 ? run_simple<T, true>(p, s) : run_simple<T, false>(p, s);
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace(const lunarad_paged_attention_args&) { return 0; }
+int64_t paged_attention_workspace(const lunarad_paged_attention_args& a) {
+  if (!stream_ok(a)) return 0;
+  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1) * kRowTile;
+  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
+}
 
 cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, cudaStream_t stream) {
   const lunarad_cache& c = *a.cache;
@@ -161,11 +924,19 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, cudaSt
   const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
   p.scale = static_cast<float>(a.scale * (e2m1 ? c.k_gain : 1.0));
   p.v_gain = e2m1 ? static_cast<float>(c.v_gain) : 1.f;
+  p.min_rows = 0;
+  p.max_rows = INT64_MAX;
+  const bool stream_kernel = stream_ok(a);
+  if (stream_kernel) {
+    p.workers = stream_workers(e2m1);
+    p.part_o = static_cast<float*>(a.workspace);
+    p.part_ml = p.part_o + int64_t{2} * p.workers * kRowTile * padded_dim(c.dim);
+  }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;
-  if (a.dtype == LUNARA_F16) return run<__half>(p, e2m1, stream);
-  if (a.dtype == LUNARA_BF16) return run<__nv_bfloat16>(p, e2m1, stream);
-  return run<float>(p, e2m1, stream);
+  if (a.dtype == LUNARA_F16) return run<__half>(p, stream_kernel, e2m1, stream);
+  if (a.dtype == LUNARA_BF16) return run<__nv_bfloat16>(p, stream_kernel, e2m1, stream);
+  return run<float>(p, stream_kernel, e2m1, stream);
 }
 
 }  // namespace lunara

@@ -102,7 +102,7 @@ def attention(c=None, seqs=SEQS, q_heads=4, window=0, max_q=0, dtype=0, scale=0.
     (lambda: append(q_heads=4, q=(0, 1, 1, 1)), "Q is NULL"), (lambda: append(k=(0, 1, 1, 1)), "K is NULL"),
     (lambda: read(dtype=1), "differ"), (lambda: read(out=0), "NULL"), (lambda: read(out=17), "aligned"),
     (lambda: attention(q_heads=3), "multiple"), (lambda: attention(q_heads=0), "multiple"), (lambda: attention(dtype=1), "differ"),
-    (lambda: attention(c=cache(dim=512)), "256"), (lambda: attention(window=-1), "window"),
+    (lambda: attention(seqs=(16, 16, 16, 8, 8, 2, 1 << 30)), "2^31"), (lambda: attention(c=cache(dim=512)), "256"), (lambda: attention(window=-1), "window"),
     (lambda: attention(max_q=-1), "max_q_len"), (lambda: attention(scale=math.inf), "finite"),
     (lambda: attention(seqs=(16, 16, 16, 1 << 29, 1 << 29, 2, 5)), "2^31"), (lambda: attention(q=(0, 1, 1, 1)), "Q is NULL"),
 ])

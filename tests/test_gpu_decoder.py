@@ -13,7 +13,13 @@ of the output's type, relative to the value.
             error (dim + 2) 2^-24 scale sum |q||k| (which enters p and the sum), n the
             number of keys summed, 2^-13 the exponential (cubic: 7.5e-5; 2^-18 in fp32,
             which has no cubic).
-fp16 results below its normal range are off by half its smallest step, 2^-25.
+fp16 results below its normal range are off by half its smallest step, 2^-25. So are fp16
+probabilities (fp16 queries, and every product with a 4-bit cache): one below 2^-14 of its
+row's largest is off by up to 2^-25 of that, whatever its own size, and the largest is at
+least 1 in the sum that divides it; that moves the output by up to 2^-25 sum |v| over the
+keys. It shows where the values of the keys that matter are zeros, as 4-bit codes can be.
+The rounding of the output is half a step of the computed value, which is off by the other
+terms already: they count (1 + h) times.
 """
 import pytest
 import torch
@@ -357,7 +363,10 @@ def check_attention(p, q_heads, window=0, scale=None, max_q_len=None, q=None, wh
         o, spread, reach = ref.attend(q[at:at + n], k, v, whole - n, scale, window)
         want[at:at + n] = o
         d = (p.dim + 2) * 2.0 ** -24 * reach[..., None]
-        tol[at:at + n] = half_step(p.dtype) * o.abs() + (hp + 2 * d + (whole + 8) * 2.0 ** -24 + ex) * spread + TINY
+        inner = (hp + 2 * d + (whole + 8) * 2.0 ** -24 + ex) * spread
+        if p.bits == 4 or p.dtype == F16:
+            inner = inner + TINY * v.abs().sum(0).repeat_interleave(q_heads // p.heads, 0)
+        tol[at:at + n] = half_step(p.dtype) * o.abs() + (1 + half_step(p.dtype)) * inner + TINY
         at += n
     within(out, want, tol, what or "paged attention")
     assert ops.device_error() == 0
@@ -498,6 +507,23 @@ def test_paged_attention_extreme_scores():
         check_attention(p, 4, q=q, what="extreme scores")
 
 
+@pytest.mark.parametrize("bits,dim", [(16, 64), (16, 128), (4, 128), (16, 20)])
+@pytest.mark.parametrize("lens", ["mixed", "chunks"])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_paged_attention_scales(scale, lens, bits, dim):
+    p = ref.Paged(SEQS[lens], 2, dim, 16, BF16, seed=15, bits=bits)
+    check_attention(p, 4, scale=scale)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_attention_many_sequences(bits):
+    """More sequences than one launch plans for."""
+    g = torch.Generator().manual_seed(16)
+    lens = [(n, n + w) for n, w in zip(torch.randint(0, 3, (2100,), generator=g).tolist(), torch.randint(0, 40, (2100,), generator=g).tolist())]
+    p = ref.Paged(lens, 1, 64, 8, F16, seed=16, bits=bits, extra_tokens=2)
+    check_attention(p, 2)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("lens", ["decode", "chunks", "long"])
 def test_paged_attention_deterministic_and_captured(lens, bits):
@@ -582,7 +608,10 @@ def test_decoding_step_by_step(dtype, bits):
                 hp = 0.0 if dtype == F32 else half_step(dtype)
                 d = (dim + 2) * 2.0 ** -24 * reach[..., None]
                 ex = 2.0 ** -18 if dtype == F32 else 2.0 ** -13
-                tol = half_step(dtype) * o.abs() + (hp + 2 * d + (have[b] + 8) * 2.0 ** -24 + ex) * spread + TINY
+                inner = (hp + 2 * d + (have[b] + 8) * 2.0 ** -24 + ex) * spread
+                if bits == 4 or dtype == F16:
+                    inner = inner + TINY * pv.double().abs().sum(0).repeat_interleave(group, 0)
+                tol = half_step(dtype) * o.abs() + (1 + half_step(dtype)) * inner + TINY
                 within(out[at:at + s], o, tol, f"sequence {b} at {have[b]}")
             at += s
     assert ops.device_error() == 0
