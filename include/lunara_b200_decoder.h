@@ -161,9 +161,10 @@ int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream);
  * (0x502) are left out, and a length outside the page table (0x503) is cut.
  * max_q_len: the longest sequence's number of tokens if known (0 = unknown);
  * it only steers the choice of kernels.
- * workspace: device memory of lunarad_paged_attention_workspace() bytes,
- * 16-byte aligned, in use until the call's work is done; calls that may run at
- * the same time need one each. Its contents need no preparation. */
+ * workspace: device memory of lunarad_paged_attention_workspace() bytes or
+ * more (NULL when that is 0), 16-byte aligned, in use until the call's work is
+ * done; calls that may run at the same time need one each. Its contents need
+ * no preparation. */
 typedef struct lunarad_paged_attention_args {
   lunarad_view q, o;
   const lunarad_cache* cache;
@@ -172,15 +173,14 @@ typedef struct lunarad_paged_attention_args {
   int64_t window;
   int64_t max_q_len;
   int64_t dtype;
-  void* workspace;
-  int64_t workspace_bytes;
   double scale;
 } lunarad_paged_attention_args;
-int lunarad_paged_attention(const lunarad_paged_attention_args* args, void* stream);
+int lunarad_paged_attention(const lunarad_paged_attention_args* args, void* workspace, int64_t workspace_bytes,
+                            void* stream);
 
-/* Workspace bytes that lunarad_paged_attention needs for these arguments
- * (workspace and workspace_bytes ignored), or -lunara_status. */
-int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* args);
+/* Workspace bytes that lunarad_paged_attention needs for these arguments on
+ * `device`, or -lunara_status. */
+int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* args, int device);
 
 #ifdef __cplusplus
 }

@@ -61,8 +61,9 @@ int current_device() {
 
 }  // namespace
 
-int device_num_sms() {
-  const int dev = current_device();
+int device_num_sms() { return device_num_sms_of(current_device()); }
+
+int device_num_sms_of(int dev) {
   if (dev < 0 || dev >= kMaxDevices) return 148;
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_sms[dev] == 0) {

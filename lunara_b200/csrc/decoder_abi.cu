@@ -207,15 +207,16 @@ int lunarad_kv_read(const lunarad_kv_read_args* a, void* stream) {
   return from_cuda(launch_kv_read(*a, as_stream(stream)), fn);
 }
 
-int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* a) {
+int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* a, int device) {
   const int rc = check_attention("lunarad_paged_attention_workspace", a);
   if (rc != LUNARA_OK) return -rc;
   ok();
   if (a->seqs.batch == 0 || a->seqs.tokens == 0) return 0;
-  return paged_attention_workspace(*a);
+  return paged_attention_workspace(*a, device_num_sms_of(device));
 }
 
-int lunarad_paged_attention(const lunarad_paged_attention_args* a, void* stream) {
+int lunarad_paged_attention(const lunarad_paged_attention_args* a, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
   static const char* fn = "lunarad_paged_attention";
   int rc = check_attention(fn, a);
   if (rc != LUNARA_OK) return rc;
@@ -223,10 +224,10 @@ int lunarad_paged_attention(const lunarad_paged_attention_args* a, void* stream)
   rc = check_view(fn, "Q", a->q, a->dtype);
   if (rc == LUNARA_OK) rc = check_view(fn, "O", a->o, a->dtype);
   if (rc != LUNARA_OK) return rc;
-  const int64_t need = paged_attention_workspace(*a);
-  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 16)))
+  const int64_t need = paged_attention_workspace(*a, device_num_sms());
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(LUNARA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
-  return from_cuda(launch_paged_attention(*a, as_stream(stream)), fn);
+  return from_cuda(launch_paged_attention(*a, workspace, as_stream(stream)), fn);
 }
 
 }  // extern "C"

@@ -10,7 +10,8 @@
 
 namespace lunara {
 
-int device_num_sms();
+int device_num_sms();             // of the current device
+int device_num_sms_of(int dev);
 
 // Status of an entry point: keeps a message for lunara_last_error_string()
 // and returns the code (fail), clears it (ok), or does either by a CUDA result.

@@ -828,7 +828,7 @@ cudaError_t run_simple(const PagedParams& p, cudaStream_t s) {
 }
 
 int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
-int stream_workers(bool e2m1) { return device_num_sms() * kWarps * (e2m1 ? 3 : 2); }
+int stream_workers(bool e2m1, int sms) { return sms * kWarps * (e2m1 ? 3 : 2); }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -886,13 +886,13 @@ cudaError_t run(const PagedParams& p, bool stream_kernel, bool e2m1, cudaStream_
 
 }  // namespace
 
-int64_t paged_attention_workspace(const lunarad_paged_attention_args& a) {
+int64_t paged_attention_workspace(const lunarad_paged_attention_args& a, int sms) {
   if (!stream_ok(a)) return 0;
-  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1) * kRowTile;
+  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, sms) * kRowTile;
   return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, cudaStream_t stream) {
+cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* workspace, cudaStream_t stream) {
   const lunarad_cache& c = *a.cache;
   PagedParams p{};
   p.q = a.q.data;
@@ -928,8 +928,8 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, cudaSt
   p.max_rows = INT64_MAX;
   const bool stream_kernel = stream_ok(a);
   if (stream_kernel) {
-    p.workers = stream_workers(e2m1);
-    p.part_o = static_cast<float*>(a.workspace);
+    p.workers = stream_workers(e2m1, device_num_sms());
+    p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + int64_t{2} * p.workers * kRowTile * padded_dim(c.dim);
   }
   p.err = device_error_word();

@@ -69,8 +69,8 @@ DECODER_SIGNATURES = {
     "lunarad_qk_norm_rotary": ([_args, _p], _i),
     "lunarad_kv_append": ([_args, _p], _i),
     "lunarad_kv_read": ([_args, _p], _i),
-    "lunarad_paged_attention": ([_args, _p], _i),
-    "lunarad_paged_attention_workspace": ([_args], _i64),
+    "lunarad_paged_attention": ([_args, _p, _i64, _p], _i),
+    "lunarad_paged_attention_workspace": ([_args, _i], _i64),
 }
 
 # Internal self-test entry points, declared in include/lunara_b200_selftest.h

@@ -39,7 +39,7 @@ _ROTARY = struct.Struct("21q")
 _QK_NORM = struct.Struct("31qd")
 _APPEND = struct.Struct("30q")
 _READ = struct.Struct("11q")
-_ATTENTION = struct.Struct("22qd")
+_ATTENTION = struct.Struct("20qd")
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -56,19 +56,21 @@ def _layout_code(layout: str) -> int:
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}") from None
 
 
-def _check_device(device: torch.device, *ts: Optional[torch.Tensor]) -> None:
-    assert device.type == "cuda", "lunara kernels take CUDA tensors"
+def _check_device(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
+    """Index of the device that all the tensors are on."""
+    assert like.is_cuda, "lunara kernels take CUDA tensors"
+    index = like.get_device()
     for t in ts:
-        if t is not None:
-            assert t.device == device, f"all tensors must be on {device}, got {t.device}"
+        assert t is None or t.get_device() == index, f"all tensors must be on {like.device}, got {t.device}"
+    return index
 
 
-def _call(name: str, args: bytes, device: torch.device) -> None:
-    lib = _lib.load()
-    if torch._C._cuda_getDevice() != device.index:
-        with torch.cuda.device(device):
-            return _call(name, args, device)
-    rc = getattr(lib, name)(args, torch._C._cuda_getCurrentRawStream(device.index))
+def _call(name: str, args: bytes, index: int, *more) -> None:
+    """Run an entry point on the current stream of device `index`."""
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _call(name, args, index, *more)
+    rc = getattr(_lib.load(), name)(args, *more, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
 
@@ -181,7 +183,8 @@ def _dense(x: torch.Tensor, name: str) -> Tuple[int, int, int, int]:
 
 def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        out = torch.empty_like(like)   # dense, in the order of like's strides
+        return out if out.stride(-1) == 1 else torch.empty_like(like, memory_format=torch.contiguous_format)
     assert out.shape == like.shape and out.dtype == like.dtype, f"{name} must be {tuple(like.shape)} {like.dtype}"
     _unit(out, name)
     _writable(out, name)
@@ -203,10 +206,10 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, layout
     assert table is not None, "rotary needs a table"
     pos = _positions(positions, batch, seq, X.dim())
     code = _dtype_code(X)
-    _check_device(X.device, positions, table, out)
+    device = _check_device(X, positions, table, out)
     out = _output(out, X, "out")
     _call("lunarad_rotary", _ROTARY.pack(*_view(X), *_view(out), *pos, *rot, batch, heads, seq, dim, 1 if inverse else 0,
-                                         code), X.device)
+                                         code), device)
     return out
 
 
@@ -232,28 +235,26 @@ def qk_norm_rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, ta
     rot = _table(table, dim, layout)
     pos = _positions(positions, batch, seq, Q.dim())
     code = _dtype_code(Q)
-    _check_device(Q.device, K, positions, table, q_weight, k_weight, out_q, out_k)
+    device = _check_device(Q, K, positions, table, q_weight, k_weight, out_q, out_k)
     wq, wk = _weight(q_weight, Q, dim, "q_weight"), _weight(k_weight, Q, dim, "k_weight")
     out_q, out_k = _output(out_q, Q, "out_q"), _output(out_k, K, "out_k")
     _call("lunarad_qk_norm_rotary", _QK_NORM.pack(*_view(Q), *_view(K), *_view(out_q), *_view(out_k), wq, wk, *pos, *rot, batch,
-                                                  q_heads, k_heads, seq, dim, code, eps), Q.device)
+                                                  q_heads, k_heads, seq, dim, code, eps), device)
     return out_q, out_k
 
 
 # ─────────────────────────────────────────────────── paged cache ──
 
-def _sequences(page_table: torch.Tensor, seq_starts: torch.Tensor, seq_lens: torch.Tensor, tokens: int,
-               device: torch.device) -> Tuple[int, ...]:
+def _sequences(page_table: torch.Tensor, seq_starts: torch.Tensor, seq_lens: torch.Tensor, tokens: int) -> Tuple[int, ...]:
+    shape, stride = page_table.shape, page_table.stride()
     batch = seq_lens.shape[0]
-    assert page_table.dim() == 2 and page_table.shape[0] == batch and seq_lens.dim() == 1, \
-        "page_table must be [batch, max_pages] and seq_lens [batch]"
+    assert len(shape) == 2 and shape[0] == batch and seq_lens.dim() == 1, "page_table must be [batch, max_pages] and seq_lens [batch]"
     assert seq_starts.shape == (batch + 1,), f"seq_starts must be [{batch + 1}], got {tuple(seq_starts.shape)}"
-    for t, name in ((page_table, "page_table"), (seq_starts, "seq_starts"), (seq_lens, "seq_lens")):
-        assert t.dtype == torch.int32, f"{name} must be int32"
-        assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs a unit inner stride"
-        assert t.device == device, f"all tensors must be on {device}, got {t.device}"
-    return (page_table.data_ptr(), seq_starts.data_ptr(), seq_lens.data_ptr(), page_table.stride(0), page_table.shape[1],
-            batch, tokens)
+    i32 = torch.int32
+    assert page_table.dtype is i32 and seq_starts.dtype is i32 and seq_lens.dtype is i32, "page_table, seq_starts and seq_lens must be int32"
+    assert (stride[1] == 1 or shape[1] <= 1) and (seq_lens.stride(0) == 1 or batch <= 1) and (seq_starts.stride(0) == 1 or batch < 1), \
+        "page_table, seq_starts and seq_lens need a unit inner stride"
+    return page_table.data_ptr(), seq_starts.data_ptr(), seq_lens.data_ptr(), stride[0], shape[1], batch, tokens
 
 
 def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Tensor,
@@ -274,7 +275,6 @@ def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table:
     _unit(V, "V")
     rot = _table(table, dim, layout)
     code = _dtype_code(K)
-    device = cache.device
     q_heads, q, o = 0, (0, 0, 0, 0), (0, 0, 0, 0)
     if Q is not None:
         assert Q.dim() == 3 and Q.shape[0] == tokens and Q.shape[2] == dim and Q.dtype == K.dtype, \
@@ -283,8 +283,8 @@ def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table:
         q_heads = Q.shape[1]
     else:
         assert out_q is None, "out_q without Q"
-    _check_device(device, K, V, table, Q, out_q)
-    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
+    device = _check_device(cache.k_pages, K, V, table, Q, out_q, page_table, seq_starts, seq_lens)
     if Q is not None:
         out_q = _output(out_q, Q, "out_q")
         q, o = _view(Q), _view(out_q)
@@ -301,10 +301,10 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Ten
         dtype = torch.float16 if cache.dtype is None else cache.dtype
     assert cache.dtype is None or dtype == cache.dtype, f"a {cache.dtype} cache is read as such, not as {dtype}"
     assert tokens >= 0, "tokens must not be negative"
-    device = cache.device
-    _check_device(device)
-    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
-    k, v = (torch.empty(tokens, cache.kv_heads, cache.head_dim, dtype=dtype, device=device) for _ in range(2))
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
+    device = _check_device(cache.k_pages, page_table, seq_starts, seq_lens)
+    k = torch.empty((tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
     _call("lunarad_kv_read", _READ.pack(k.data_ptr(), v.data_ptr(), cache._address, *seqs, _dtype_code(k)), device)
     return k, v
 
@@ -325,20 +325,15 @@ def paged_attention(Q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     assert q_heads > 0 and q_heads % cache.kv_heads == 0, f"{q_heads} query heads are no multiple of {cache.kv_heads} key heads"
     _unit(Q, "Q")
     code = _dtype_code(Q)
-    device = cache.device
-    _check_device(device, Q, out)
-    seqs = _sequences(page_table, seq_starts, seq_lens, tokens, device)
+    seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
+    device = _check_device(cache.k_pages, Q, out, page_table, seq_starts, seq_lens)
     out = _output(out, Q, "out")
     if scale is None:
-        scale = 1.0 / math.sqrt(dim)
-    head = (*_view(Q), *_view(out), cache._address, *seqs, q_heads, window, max_q_len or 0, code)
-    args = _ATTENTION.pack(*head, 0, 0, scale)
-    lib = _lib.load()
-    need = lib.lunarad_paged_attention_workspace(args)
+        scale = dim ** -0.5
+    args = _ATTENTION.pack(*_view(Q), *_view(out), cache._address, *seqs, q_heads, window, max_q_len or 0, code, scale)
+    need = _lib.load().lunarad_paged_attention_workspace(args, device)
     if need < 0:
         _lib.check(-need)
-    if need > 0:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        args = _ATTENTION.pack(*head, workspace.data_ptr(), need, scale)
-    _call("lunarad_paged_attention", args, device)
+    workspace = Q.new_empty((need + 1) // 2 if code != _lib.F32 else (need + 3) // 4) if need else None
+    _call("lunarad_paged_attention", args, device, workspace.data_ptr() if need else None, need)
     return out

@@ -75,7 +75,7 @@ def read(c=None, seqs=SEQS, dtype=0, out=16):
 
 def attention(c=None, seqs=SEQS, q_heads=4, window=0, max_q=0, dtype=0, scale=0.1, q=VIEW):
     return _lib.load().lunarad_paged_attention(
-        decoder._ATTENTION.pack(*q, *VIEW, cache() if c is None else c, *seqs, q_heads, window, max_q, dtype, 0, 0, scale), None)
+        decoder._ATTENTION.pack(*q, *VIEW, cache() if c is None else c, *seqs, q_heads, window, max_q, dtype, scale), None, 0, None)
 
 
 @pytest.mark.parametrize("call,needle", [
@@ -121,10 +121,11 @@ def test_empty_work_is_ok_without_device():
 
 def test_workspace_refuses_like_the_call():
     lib = _lib.load()
-    bad = decoder._ATTENTION.pack(*VIEW, *VIEW, cache(), *SEQS, 3, 0, 0, 0, 0, 0, 0.1)
-    assert lib.lunarad_paged_attention_workspace(bad) == -_lib.ERR_INVALID_ARG
-    good = decoder._ATTENTION.pack(*VIEW, *VIEW, cache(), *SEQS, 4, 0, 0, 0, 0, 0, 0.1)
-    assert lib.lunarad_paged_attention_workspace(good) >= 0
+    bad = decoder._ATTENTION.pack(*VIEW, *VIEW, cache(), *SEQS, 3, 0, 0, 0, 0.1)
+    assert lib.lunarad_paged_attention_workspace(bad, 0) == -_lib.ERR_INVALID_ARG
+    good = decoder._ATTENTION.pack(*VIEW, *VIEW, cache(), *SEQS, 4, 0, 0, 0, 0.1)
+    assert lib.lunarad_paged_attention_workspace(good, 0) > 0
+    assert lib.lunarad_paged_attention(good, None, 0, None) == _lib.ERR_INVALID_ARG and "workspace" in err()
 
 
 # ── the torch layer ──────────────────────────────────────────────────────────
@@ -211,9 +212,9 @@ def test_page_tables_refused(change, needle):
     tab, starts, lens = seqs()
     q = torch.zeros(3, 4, 64, dtype=torch.float16)
     with pytest.raises(AssertionError, match=needle):
-        decoder._sequences(change((tab,)), starts, lens, 3, torch.device("cpu"))
+        decoder._sequences(change((tab,)), starts, lens, 3)
     with pytest.raises(AssertionError, match="seq_starts"):
-        decoder._sequences(tab, starts[:-1], lens, 3, torch.device("cpu"))
+        decoder._sequences(tab, starts[:-1], lens, 3)
     with pytest.raises(AssertionError, match="multiple"):
         ops.paged_attention(q[:, :3], pages(), tab, starts, lens)
     with pytest.raises(AssertionError, match="must be"):
