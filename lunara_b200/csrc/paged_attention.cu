@@ -736,10 +736,12 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
 }
 
 // Joins the parts of the rows whose keys several workers took, and clears the
-// rows of sequences without keys. One block per query row. The lengths are
-// read before the streaming kernel has ended (it has started, so whatever
-// came before it is complete), the parts after it.
-constexpr int kJoinThreads = 128;
+// rows of sequences without keys. Block x takes the row tile that run x begins
+// inside, if no earlier run begins inside it too; blockIdx.y takes every
+// kJoinShares-th row, its warps every fourth part. The lengths are read before
+// the streaming kernel has ended (it has started, so whatever came before it is
+// complete), the parts after it.
+constexpr int kJoinThreads = 128, kJoinShares = 4;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int KT) {
@@ -751,72 +753,92 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
   constexpr int kWarpsHere = kJoinThreads / 32, kE = DP / 32;
   prefix_tiles(p, KT, prefix, warp_sums);
+  const int64_t total = prefix[p.seqs.batch];
+  const int workers = used_workers(p, total), w1 = static_cast<int>(blockIdx.x);
+  SeqInfo s{};
+  int row_tiles = 0, seg_tiles = 1, kh = 0, rt = 0;
+  int64_t start = 0;
+  bool mine = w1 > 0 && w1 < workers;
+  if (mine) {
+    const int64_t t = run_start(total, workers, w1);
+    int b = 0;
+    for (int end = p.seqs.batch; b + 1 < end;) {   // last b with prefix[b] <= t
+      const int mid = (b + end) >> 1;
+      if (prefix[mid] <= t) b = mid; else end = mid;
+    }
+    s = load_seq(p, b);
+    seq_tiles(p, s, KT, row_tiles, seg_tiles);
+    const int seg = static_cast<int>((t - prefix[b]) / seg_tiles);
+    kh = seg / row_tiles;
+    rt = seg - kh * row_tiles;
+    start = prefix[b] + static_cast<int64_t>(seg) * seg_tiles;
+    mine = t > start && run_start(total, workers, w1 - 1) <= start;
+  }
   pdl_wait();
   pdl_launch_dependents();
-  const int token = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), kh = h / p.group;
-  int b;
-  int64_t pos;
-  if (!find_token(p.seqs, token, b, pos)) return;
-  const SeqInfo s = load_seq(p, b);
-  const int64_t rows = static_cast<int64_t>(s.n) * p.group;
-  if (rows < p.min_rows || rows >= p.max_rows) return;
-  int row_tiles, seg_tiles;
-  seq_tiles(p, s, KT, row_tiles, seg_tiles);
-  T* out = static_cast<T*>(p.o) + token * p.o_tok + h * p.o_head;
-  if (seg_tiles == 0) {
-    for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) out[d] = Io<T>::from_f(0.f);
-    return;
-  }
-  const int row = (token - s.first) * p.group + h - kh * p.group;
-  const int64_t total = prefix[p.seqs.batch];
-  const int64_t t0 = prefix[b] + (static_cast<int64_t>(kh) * row_tiles + row / kRowTile) * seg_tiles;
-  const int workers = used_workers(p, total);
-  const int w0 = run_of(total, workers, t0), w1 = run_of(total, workers, t0 + seg_tiles - 1);
-  if (w0 == w1) return;   // written by its worker
-  const int first_slot = run_start(total, workers, w0) == t0 ? 0 : 1;
-  // Each warp joins every fourth part; the lane holds elements 4 lane .. (or 2 lane ..).
-  float m = -INFINITY, l = 0.f, o[kE];
-#pragma unroll
-  for (int e = 0; e < kE; ++e) o[e] = 0.f;
-  for (int w = w0 + warp; w <= w1; w += kWarpsHere) {
-    const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * kRowTile + row % kRowTile;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-    float x[kE];
-    if constexpr (kE == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
-      x[0] = v.x; x[1] = v.y;
+  if (blockIdx.y == 0) {
+    for (int b = w1; b < p.seqs.batch; b += gridDim.x) {
+      const SeqInfo z = load_seq(p, b);
+      const int64_t rows = static_cast<int64_t>(z.n) * p.group;
+      if (rows < p.min_rows || rows >= p.max_rows || z.hi > z.lo) continue;
+      const int width = p.q_heads * p.dim;
+      for (int token = z.first; token < z.first + z.n; ++token)
+        for (int e = threadIdx.x; e < width; e += kJoinThreads)
+          static_cast<T*>(p.o)[token * p.o_tok + e / p.dim * p.o_head + e % p.dim] = Io<T>::from_f(0.f);
     }
-    const float next = fmax_nan(m, ml.x);
-    const float base = next == -INFINITY ? 0.f : next;
-    const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
-    l = l * fa + ml.y * fb;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
-    m = next;
   }
+  if (!mine) return;
+  const int w0 = w1 - 1, last = run_of(total, workers, start + seg_tiles - 1);
+  const int first_slot = run_start(total, workers, w0) == start ? 0 : 1;
+  const int rows = min(kRowTile, s.n * p.group - rt * kRowTile);
+  for (int r = static_cast<int>(blockIdx.y); r < rows; r += kJoinShares) {
+    float m = -INFINITY, l = 0.f, o[kE];
 #pragma unroll
-  for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
-  if (lane == 0) s_ml[warp] = make_float2(m, l);
-  __syncthreads();
-  float top = s_ml[0].x;
+    for (int e = 0; e < kE; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int w = w0 + warp; w <= last; w += kWarpsHere) {
+      const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * kRowTile + r;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+      float x[kE];
+      if constexpr (kE == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
+        x[0] = v.x; x[1] = v.y;
+      }
+      const float next = fmax_nan(m, ml.x);
+      const float base = next == -INFINITY ? 0.f : next;
+      const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
+      l = l * fa + ml.y * fb;
 #pragma unroll
-  for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, f[kWarpsHere];
+      for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
+      m = next;
+    }
+    __syncthreads();   // the row before has been read
 #pragma unroll
-  for (int w = 0; w < kWarpsHere; ++w) {
-    f[w] = ex2_approx(s_ml[w].x - base);
-    sum += s_ml[w].y * f[w];
-  }
-  const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
-  for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
-    float x = 0.f;
+    for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    float top = s_ml[0].x;
 #pragma unroll
-    for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
-    out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
+    for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, f[kWarpsHere];
+#pragma unroll
+    for (int w = 0; w < kWarpsHere; ++w) {
+      f[w] = ex2_approx(s_ml[w].x - base);
+      sum += s_ml[w].y * f[w];
+    }
+    const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
+    const int row = rt * kRowTile + r, i = row / p.group;
+    T* out = static_cast<T*>(p.o) + (s.first + i) * p.o_tok + (kh * p.group + row - i * p.group) * p.o_head;
+    for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
+      out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
+    }
   }
 }
 
@@ -848,6 +870,22 @@ bool stream_ok(const lunarad_paged_attention_args& a) {
          c.ks_head_stride % 16 == 0 && c.vs_page_stride % 16 == 0 && c.vs_head_stride % 16 == 0;
 }
 
+// Sequences with this many query rows go to the tcgen05 kernel where it takes
+// the cache.
+constexpr int64_t kPrefillRows = 64;
+
+bool prefill_ok(const lunarad_paged_attention_args& a) {
+  const lunarad_cache& c = *a.cache;
+  const int64_t group = a.q_heads / c.kv_heads;
+  const int64_t most = a.max_q_len > 0 && a.max_q_len < a.seqs.tokens ? a.max_q_len : a.seqs.tokens;   // tokens of a sequence
+  return stream_ok(a) && c.kind != LUNARAD_KIND_E2M1 && (c.dim == 64 || c.dim == 128) && most * group >= kPrefillRows;
+}
+
+int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {
+  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, sms) * kRowTile;
+  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
+}
+
 template <typename T, bool E2M1, int DP>
 cudaError_t run_stream(PagedParams p, cudaStream_t s) {
   using S = Shape<E2M1, DP>;
@@ -867,7 +905,7 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
     p.seqs.lens = all.lens + b0;
     e = launch_pdl(kern, dim3(p.workers / kWarps), dim3(kStreamThreads), smem, s, p);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(paged_join_kernel<T, DP>, dim3(p.seqs.tokens, p.q_heads), dim3(kJoinThreads), prefix, s, p, S::KT);
+    e = launch_pdl(paged_join_kernel<T, DP>, dim3(p.workers, kJoinShares), dim3(kJoinThreads), prefix, s, p, S::KT);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -888,8 +926,7 @@ cudaError_t run(const PagedParams& p, bool stream_kernel, bool e2m1, cudaStream_
 
 int64_t paged_attention_workspace(const lunarad_paged_attention_args& a, int sms) {
   if (!stream_ok(a)) return 0;
-  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, sms) * kRowTile;
-  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
+  return stream_workspace(a, sms) + (prefill_ok(a) ? paged_prefill_workspace(static_cast<int>(a.cache->dim), sms) : 0);
 }
 
 cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* workspace, cudaStream_t stream) {
@@ -934,6 +971,13 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
   }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;
+  if (prefill_ok(a)) {
+    PagedParams q = p;
+    q.min_rows = p.max_rows = kPrefillRows;
+    const cudaError_t e = launch_paged_prefill(q, static_cast<int>(a.dtype),
+                                               static_cast<char*>(workspace) + stream_workspace(a, device_num_sms()), stream);
+    if (e != cudaSuccess) return e;
+  }
   if (a.dtype == LUNARA_F16) return run<__half>(p, stream_kernel, e2m1, stream);
   if (a.dtype == LUNARA_BF16) return run<__nv_bfloat16>(p, stream_kernel, e2m1, stream);
   return run<float>(p, stream_kernel, e2m1, stream);

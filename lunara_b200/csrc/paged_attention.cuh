@@ -63,4 +63,9 @@ __device__ __forceinline__ void visible(const PagedParams& p, int64_t pos, int& 
   lo = p.window > 0 && pos + 1 > p.window ? static_cast<int>(min(pos + 1 - p.window, e)) : 0;
 }
 
+// Many query rows per sequence (paged_prefill.cu): 16-bit caches with head
+// dimension 64 or 128.
+int64_t paged_prefill_workspace(int dim, int sms);
+cudaError_t launch_paged_prefill(PagedParams p, int dtype, void* workspace, cudaStream_t stream);
+
 }  // namespace lunara
