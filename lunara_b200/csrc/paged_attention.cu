@@ -175,6 +175,10 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   return u;
 }
 
+__device__ __forceinline__ void sts8(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
 // D += A B, m16n8k16: A row-major, B column-major, 16-bit, fp32 accumulators.
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -268,7 +272,8 @@ __device__ __forceinline__ int run_of(int64_t total, int workers, int64_t t) {
   return static_cast<int>(((t + 1) * workers + total - 1) / total) - 1;
 }
 
-template <typename T, bool E2M1, int DP>
+// EXACT: the head dimension is DP, a constant.
+template <typename T, bool E2M1, int DP, bool EXACT>
 __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
     paged_stream_kernel(const __grid_constant__ PagedParams p) {
   using S = Shape<E2M1, DP>;
@@ -289,8 +294,8 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
   const int64_t t_first = run_start(total, workers, worker), t_end = run_start(total, workers, worker + 1);
   const bool grouped = E2M1 || (p.page_size & 7) == 0;   // 8 neighbouring keys stand in one page
   constexpr int kElem = E2M1 ? 1 : 2;
-  const int row_bytes = E2M1 ? p.dim / 2 : p.dim * 2;
-  const int64_t k_page = p.k_page * kElem, v_page = p.v_page * kElem;
+  const int dim = EXACT ? DP : p.dim;
+  const int row_bytes = E2M1 ? dim / 2 : dim * 2, srow = dim / 16;
 
   for (int64_t t = t_first; t < t_end;) {
     // ------------------------------------------------ where the run stands --
@@ -326,36 +331,49 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
     visible(p, s.pos0 + rt * kRowTile / p.group, any_lo, all_hi);
 
     // -------------------------------------------------------------- pages --
-    // Lane l holds the page of the l-th group of 8 keys of a batch of 256
-    // (grouped) or of the l-th key of a tile; the next batch is loaded ahead.
+    // Lane l looks up the l-th group of 8 keys of a batch of 256 (grouped) or
+    // the l-th key of a tile, a batch ahead of its use, and keeps where it
+    // stands in K, V and the scales, in units of p.unit bytes (32 bits reach
+    // 64 or 256 GiB).
     const int32_t* table = p.seqs.page_table + b * p.seqs.table_stride;
-    auto load_pages = [&](int first) {
-      const int key = grouped ? first + 8 * lane : first + lane;
-      if (key + (grouped ? 8 : 1) <= any_lo || key >= any_hi) return -1;   // nothing of it is read
+    const int per_lane = grouped ? 8 : 1, batch_keys = grouped ? 256 : KT;
+    auto load_page = [&](int first) {
+      const int key = first + per_lane * lane;
+      if (key + per_lane <= any_lo || key >= any_hi) return -1;   // nothing of it is read
       const int page = table[p.seqs.page_div.div(key)];
       if (page >= 0 && page < p.num_pages) return page;
       atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCachePage));
       return -1;
     };
-    const int batch_keys = grouped ? 256 : KT;
-    int batch0 = key0;
-    int pages = load_pages(batch0), pages_next = load_pages(batch0 + batch_keys);
-
+    uint32_t k_at = 0, v_at = 0, ks_at = 0, vs_at = 0, have = 0;   // have: a bit per lane whose lookup found a page
+    int batch0 = key0 - batch_keys, page_next = load_page(key0);
+    auto next_batch = [&] {
+      const int page = page_next;
+      batch0 += batch_keys;
+      page_next = load_page(batch0 + batch_keys);
+      have = __ballot_sync(0xffffffffu, page >= 0);
+      const int key = batch0 + per_lane * lane;
+      const uint32_t slot = static_cast<uint32_t>(key - p.seqs.page_div.div(key) * p.page_size);
+      const uint32_t pg = static_cast<uint32_t>(max(page, 0)), use = page >= 0 ? 1u : 0u;
+      k_at = (pg * p.k_page_u + slot * p.row_u) * use;
+      v_at = (pg * p.v_page_u + slot * p.row_u) * use;
+      if constexpr (E2M1) {   // groups of 8 scale rows: pieces of 16 bytes
+        ks_at = (pg * p.ks_page_u + (slot >> 3) * static_cast<uint32_t>(srow >> 1)) * use;
+        vs_at = (pg * p.vs_page_u + (slot >> 3) * static_cast<uint32_t>(srow >> 1)) * use;
+      }
+    };
     const char* kb = static_cast<const char*>(p.k) + kh * p.k_head * kElem;
     const char* vb = static_cast<const char*>(p.v) + kh * p.v_head * kElem;
+    auto place = [&](const char* base, uint32_t at) { return base + static_cast<uint64_t>(at) * p.unit; };
 
     // Starts the copies of tile i into its stage; returns a bit for each of its
     // keys that takes part. All others are zero-filled: neither a stale slot's
     // NaN nor a bad page may reach a product.
     auto issue = [&](int i, int stage) -> uint32_t {
       const int first = key0 + i * KT;
-      if (first - batch0 >= batch_keys) {
-        batch0 += batch_keys;
-        pages = pages_next;
-        pages_next = load_pages(batch0 + batch_keys);
-      }
+      if (first - batch0 >= batch_keys) next_batch();
       const int g0 = (first - batch0) >> 3;   // grouped: the tile's first group in the batch
-      uint32_t ok = __ballot_sync(0xffffffffu, pages >= 0);
+      uint32_t ok = have;
       if (grouped) {
         const uint32_t x = (ok >> g0) & ((1u << (KT / 8)) - 1u);   // a bit for each group -> a byte
         ok = ((x & 1u) | ((x & 2u) << 7) | ((x & 4u) << 14) | ((x & 8u) << 21)) * 0xFFu;
@@ -364,70 +382,52 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
       if (any_hi < first + 32) ok &= any_hi > first ? (1u << (any_hi - first)) - 1u : 0u;
       if (KT < 32) ok &= (1u << (KT & 31)) - 1u;
       const uint32_t at = ring + stage * S::kStageBytes;
-      // Page and slot of the group (grouped) or key at `local`.
-      auto place = [&](int local, int64_t& page, int& slot) {
-        const int pg = __shfl_sync(0xffffffffu, pages, grouped ? g0 + (local >> 3) : local);
-        const int key = first + (grouped ? local & ~7 : local);
-        slot = key - p.seqs.page_div.div(key) * p.page_size + (grouped ? local & 7 : 0);
-        page = max(pg, 0);
-      };
       if constexpr (E2M1) {
         constexpr int kPieces = DP / 32;   // 16-byte pieces of a row of codes
-        const uint8_t* ksb = static_cast<const uint8_t*>(p.ks) + kh * p.ks_head;
-        const uint8_t* vsb = static_cast<const uint8_t*>(p.vs) + kh * p.vs_head;
+        const int piece = lane % kPieces, in_group = (lane / kPieces) & 7;
+        const bool lane_in = EXACT || 16 * piece < row_bytes;
+        const char* kl = kb + in_group * row_bytes + 16 * piece;
+        const char* vl = vb + in_group * row_bytes + 16 * piece;
 #pragma unroll
         for (int j = 0; j < KT * kPieces / 32; ++j) {
-          const int q = lane + 32 * j, local = q / kPieces, off = 16 * (q % kPieces);
-          int64_t page;
-          int slot;
-          place(local, page, slot);
-          const bool in = ((ok >> local) & 1u) != 0u && off < row_bytes;
-          const int at_row = slot * row_bytes + off;
-          copy_async(at + local * S::kKRow + off, in ? kb + page * k_page + at_row : kb, in);
-          copy_async(at + S::kKBytes + local * S::kVRow + off, in ? vb + page * v_page + at_row : vb, in);
+          const int local = (lane + 32 * j) / kPieces, src = g0 + (local >> 3);
+          const uint32_t ka = __shfl_sync(0xffffffffu, k_at, src), va = __shfl_sync(0xffffffffu, v_at, src);
+          const bool in = ((ok >> local) & 1u) != 0u && lane_in;
+          copy_async(at + local * S::kKRow + 16 * piece, place(kl, ka), in);
+          copy_async(at + S::kKBytes + local * S::kVRow + 16 * piece, place(vl, va), in);
         }
-        // Scales: those of a group of 8 keys are srow / 2 pieces of 16 bytes.
-        // A group with a masked key is copied whole: scales of masked keys
-        // multiply zeroed codes, and are cleared where they are read.
-        const int srow = p.dim / 16;
-        constexpr int kScalePieces = DP / 32;   // per group
-        constexpr int kAll = 2 * (KT / 8) * kScalePieces;
-        const int kv = lane / (kAll / 2), rest = lane % (kAll / 2), grp = rest / kScalePieces, piece = rest % kScalePieces;
-        int64_t page;
-        int slot;
-        place(8 * (grp & (KT / 8 - 1)), page, slot);
+        // The scales of a group of 8 keys are srow / 2 pieces of 16 bytes. A
+        // group with a masked key is copied whole; see clear_scales below.
+        constexpr int kScalePieces = DP / 32, kAll = 2 * (KT / 8) * kScalePieces;
+        const int kv = lane / (kAll / 2), rest = lane % (kAll / 2), grp = rest / kScalePieces, sp = rest % kScalePieces;
+        const uint32_t ka = __shfl_sync(0xffffffffu, ks_at, g0 + grp), va = __shfl_sync(0xffffffffu, vs_at, g0 + grp);
         if (lane < kAll) {
-          const bool in = ((ok >> (8 * grp)) & 0xFFu) != 0u && 16 * piece < 8 * srow;
-          const uint8_t* src = kv == 0 ? ksb + page * p.ks_page : vsb + page * p.vs_page;
-          copy_async(at + S::kKBytes + S::kVBytes + kv * S::kScaleBytes + grp * (8 * srow) + 16 * piece,
-                         in ? src + slot * srow + 16 * piece : static_cast<const uint8_t*>(p.ks), in);
+          const bool in = ((ok >> (8 * grp)) & 0xFFu) != 0u && (EXACT || 2 * sp < srow);
+          const uint8_t* src = kv == 0 ? static_cast<const uint8_t*>(p.ks) + kh * p.ks_head + static_cast<uint64_t>(ka) * 16
+                                       : static_cast<const uint8_t*>(p.vs) + kh * p.vs_head + static_cast<uint64_t>(va) * 16;
+          copy_async(at + S::kKBytes + S::kVBytes + kv * S::kScaleBytes + grp * (8 * srow) + 16 * sp, src + 16 * sp, in);
         }
       } else {
-        // K row 8 i + g: pieces c, c + 4, ...; V rows 16 a + 8 h + 2 c + e
-        // (the lane's keys of an mma k-step): pieces g, g + 8.
+        // K row 8 i + g: pieces c, c + 4, ...; V rows 8 i + 2 c + e (the lane's
+        // keys of an mma k-step): pieces g, g + 8.
+        const char* kl = kb + (grouped ? g * row_bytes : 0) + 16 * c;
+        const char* vl = vb + (grouped ? 2 * c * row_bytes : 0) + 16 * g;
 #pragma unroll
         for (int i8 = 0; i8 < KT / 8; ++i8) {
-          int64_t page;
-          int slot;
-          place(8 * i8 + g, page, slot);
+          const char* src = place(kl, __shfl_sync(0xffffffffu, k_at, grouped ? g0 + i8 : 8 * i8 + g));
           const bool use = ((ok >> (8 * i8 + g)) & 1u) != 0u;
-          const char* src = kb + page * k_page + slot * row_bytes + 16 * c;
 #pragma unroll
-          for (int j = 0; j < DP / 32; ++j) {
-            const bool in = use && 16 * (c + 4 * j) < row_bytes;
-            copy_async(at + ((i8 * (DP / 32) + j) * 32 + lane) * 16, in ? src + 64 * j : kb, in);
-          }
+          for (int j = 0; j < DP / 32; ++j)
+            copy_async(at + ((i8 * (DP / 32) + j) * 32 + lane) * 16, src + 64 * j, use && (EXACT || 16 * (c + 4 * j) < row_bytes));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int local = 8 * i8 + 2 * c + e;
-            place(local, page, slot);
+            const char* vsrc = place(vl, __shfl_sync(0xffffffffu, v_at, grouped ? g0 + i8 : local)) + (grouped ? e * row_bytes : 0);
             const bool vuse = ((ok >> local) & 1u) != 0u;
-            const char* vsrc = vb + page * v_page + slot * row_bytes + 16 * g;
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-              const bool in = vuse && 16 * (g + 8 * j) < row_bytes;
-              copy_async(at + S::kKBytes + (((2 * i8 + e) * (DP / 64) + j) * 32 + lane) * 16, in ? vsrc + 128 * j : vb, in);
-            }
+            for (int j = 0; j < DP / 64; ++j)
+              copy_async(at + S::kKBytes + (((2 * i8 + e) * (DP / 64) + j) * 32 + lane) * 16, vsrc + 128 * j,
+                         vuse && (EXACT || 16 * (g + 8 * j) < row_bytes));
           }
         }
       }
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
         // with 4 bits its i-th word of DP / 32 neighbouring ones.
         const int d = E2M1 ? (DP / 4) * c + 8 * i : 8 * (c + 4 * i);
         uint4 u0 = make_uint4(0u, 0u, 0u, 0u), u1 = u0;
-        if (d < p.dim) {
+        if (d < dim) {
           u0 = *reinterpret_cast<const uint4*>(q0 + d);
           u1 = *reinterpret_cast<const uint4*>(q1 + d);
           u0.x ^= flip; u0.y ^= flip; u0.z ^= flip; u0.w ^= flip;
@@ -522,7 +522,17 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
       for (int k = 0; k + 1 < S::kStages; ++k) ok_of[k] = ok_of[k + 1];
       const uint32_t at = ring + stage * S::kStageBytes;
       const int first = key0 + i * KT;
+      constexpr uint32_t kFull = KT == 32 ? ~0u : (1u << (KT & 31)) - 1u;
       if (ok != 0u) {
+        if constexpr (E2M1) {
+          // A masked key's scales may be anything, NaN too: V's must not meet
+          // the zero probability of that key. (K's only touch its own scores.)
+          if (ok != kFull) {
+            if (((ok >> lane) & 1u) == 0u)
+              for (int k = 0; k < srow; ++k) sts8(at + S::kKBytes + S::kVBytes + S::kScaleBytes + lane * srow + k, 0u);
+            __syncwarp();
+          }
+        }
         // S = Q K^T
         float sc[KT / 8][4];
 #pragma unroll
@@ -530,13 +540,12 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
         if constexpr (E2M1) {
-          const int srow = p.dim / 16;
-          const uint32_t ks_at = at + S::kKBytes + S::kVBytes;
+          const uint32_t k_scales = at + S::kKBytes + S::kVBytes;
 #pragma unroll
           for (int n = 0; n < KT / 8; ++n) {
             const uint32_t row = at + (8 * n + g) * S::kKRow;
             if constexpr (DP == 128) {
-              const uint32_t two = 2 * c < srow ? lds16(ks_at + (8 * n + g) * srow + 2 * c) : 0u;
+              const uint32_t two = EXACT || 2 * c < srow ? lds16(k_scales + (8 * n + g) * srow + 2 * c) : 0u;
               const uint32_t s01 = scales_to_half2(two);
               const uint32_t s0 = __byte_perm(s01, s01, 0x1010), s1 = __byte_perm(s01, s01, 0x3232);
               const uint4 w = lds128(row + 16 * c);
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
                 mma16816<M>(sc[n], qf[2 * q + 1], hmul2(h[2], sx), hmul2(h[3], sx));
               }
             } else {
-              const uint32_t one = c < srow ? lds8(ks_at + (8 * n + g) * srow + c) : 0u;
+              const uint32_t one = EXACT || c < srow ? lds8(k_scales + (8 * n + g) * srow + c) : 0u;
               const uint32_t sx = scales_to_half2(one * 0x101u);
               const uint2 w = lds64(row + 8 * c);
               const uint32_t ws[2] = {w.x, w.y};
@@ -575,7 +584,6 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
         }
         // Masks, where the tile has a key that not every row sees. (A key
         // column n, 2 c + e stands at 8 n + 2 c + e.)
-        constexpr uint32_t kFull = KT == 32 ? ~0u : (1u << (KT & 31)) - 1u;
         if (ok != kFull || first < all_lo || first + KT > all_hi) {
 #pragma unroll
           for (int n = 0; n < KT / 8; ++n)
@@ -626,16 +634,15 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
                                   Io<M>::pack2(sc[2 * a + 1][0], sc[2 * a + 1][1]),
                                   Io<M>::pack2(sc[2 * a + 1][2], sc[2 * a + 1][3])};
           if constexpr (E2M1) {
-            const int srow = p.dim / 16;
-            const uint32_t vs_at = at + S::kKBytes + S::kVBytes + S::kScaleBytes;
-            const int block = DP == 128 ? g : g >> 1;   // of this lane's columns
+            // This lane's columns lie in one scale block. (Where it is behind
+            // the head dimension another key's scale is read; those columns
+            // are not stored.)
+            const uint32_t v_scales = at + S::kKBytes + S::kVBytes + S::kScaleBytes + (DP == 128 ? g : g >> 1);
             uint32_t sx[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int key = 16 * a + 8 * h + 2 * c;
-              const uint32_t b0 = block < srow && ((ok >> key) & 1u) ? lds8(vs_at + key * srow + block) : 0u;
-              const uint32_t b1 = block < srow && ((ok >> (key + 1)) & 1u) ? lds8(vs_at + (key + 1) * srow + block) : 0u;
-              sx[h] = scales_to_half2(b0 | (b1 << 8));
+              sx[h] = scales_to_half2(lds8(v_scales + key * srow) | (lds8(v_scales + (key + 1) * srow) << 8));
             }
             constexpr int kW = DP / 64;   // words of codes per lane and key
             uint32_t w[2][2][kW];
@@ -719,7 +726,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] = l[r] == 0.f ? 0.f : acc[S::kRun * i + d8 + k][2 * r + e] * f;
               if (whole) {
-                if (d < p.dim)
+                if (d < dim)
                   *reinterpret_cast<uint4*>(out + d) = make_uint4(Io<T>::pack2(x[0], x[1]), Io<T>::pack2(x[2], x[3]),
                                                                   Io<T>::pack2(x[4], x[5]), Io<T>::pack2(x[6], x[7]));
               } else {
@@ -854,6 +861,25 @@ int stream_workers(bool e2m1, int sms) { return sms * kWarps * (e2m1 ? 3 : 2); }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Bytes of the unit in which the streaming kernel keeps where a page and row
+// stands, in 32 bits: 64 where all strides allow it (so that 256 GiB are
+// reached), else 16. 0 when a page stands beyond that.
+int place_unit(const lunarad_cache& c) {
+  const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
+  const int64_t elem = e2m1 ? 1 : 2, row = e2m1 ? c.dim / 2 : c.dim * 2;
+  const int64_t step = c.page_size % 8 == 0 ? 8 * row : row;   // rows are looked up by groups of 8, or one by one
+  const int64_t kp = c.k_page_stride * elem, vp = c.v_page_stride * elem;
+  const int64_t unit = step % 64 == 0 && row % 64 == 0 && kp % 64 == 0 && vp % 64 == 0 ? 64 : 16;
+  const int64_t most = int64_t{1} << 31, pages = c.num_pages;
+  if (kp < 0 || vp < 0 || c.ks_page_stride < 0 || c.vs_page_stride < 0) return 0;
+  const int64_t used = c.page_size * row / unit + 1;
+  if (kp / unit * pages + used >= 2 * most || vp / unit * pages + used >= 2 * most) return 0;
+  if (e2m1 && (c.ks_page_stride / 16 * pages + c.page_size * c.dim / 256 + 1 >= 2 * most ||
+               c.vs_page_stride / 16 * pages + c.page_size * c.dim / 256 + 1 >= 2 * most))
+    return 0;
+  return static_cast<int>(unit);
+}
+
 // 16-byte copies of whole rows: aligned bases and strides, rows of 16-byte
 // pieces; for 4 bits also pages of whole groups of 8 keys.
 bool stream_ok(const lunarad_paged_attention_args& a) {
@@ -862,7 +888,7 @@ bool stream_ok(const lunarad_paged_attention_args& a) {
   if (a.dtype == LUNARA_F32 || c.dim > 128) return false;
   if (!al16(a.q.data) || a.q.head_stride % 8 || a.q.seq_stride % 8) return false;
   if (!al16(a.o.data) || a.o.head_stride % 8 || a.o.seq_stride % 8) return false;
-  if (!al16(c.k) || !al16(c.v)) return false;
+  if (!al16(c.k) || !al16(c.v) || place_unit(c) == 0) return false;
   const int64_t vec = e2m1 ? 16 : 8;
   if (c.k_page_stride % vec || c.k_head_stride % vec || c.v_page_stride % vec || c.v_head_stride % vec) return false;
   if (!e2m1) return c.dim % 8 == 0;
@@ -886,13 +912,13 @@ int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {
   return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-template <typename T, bool E2M1, int DP>
+template <typename T, bool E2M1, int DP, bool EXACT>
 cudaError_t run_stream(PagedParams p, cudaStream_t s) {
   using S = Shape<E2M1, DP>;
   const size_t prefix = sizeof(int64_t) * (static_cast<size_t>(p.seqs.batch < kMaxBatch ? p.seqs.batch : kMaxBatch) + 2);
   const size_t smem = static_cast<size_t>(kWarps) * S::kRingBytes + prefix;
   static_assert(kWarps * S::kRingBytes + 8 * (kMaxBatch + 2) + 1280 <= 228 * 1024 / S::kCtasPerSm, "shared memory per SM");
-  auto kern = paged_stream_kernel<T, E2M1, DP>;
+  auto kern = paged_stream_kernel<T, E2M1, DP, EXACT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kWarps * S::kRingBytes + 8 * (kMaxBatch + 2));
   if (e != cudaSuccess) return e;
@@ -911,12 +937,18 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
   return cudaSuccess;
 }
 
+template <typename T, bool E2M1>
+cudaError_t run_stream_dim(const PagedParams& p, cudaStream_t s) {
+  if (p.dim == 64) return run_stream<T, E2M1, 64, true>(p, s);
+  if (p.dim < 64) return run_stream<T, E2M1, 64, false>(p, s);
+  return p.dim == 128 ? run_stream<T, E2M1, 128, true>(p, s) : run_stream<T, E2M1, 128, false>(p, s);
+}
+
 template <typename T>
 cudaError_t run(const PagedParams& p, bool stream_kernel, bool e2m1, cudaStream_t s) {
   if constexpr (!std::is_same<T, float>::value) {
     if (stream_kernel) {
-      if (e2m1) return p.dim <= 64 ? run_stream<T, true, 64>(p, s) : run_stream<T, true, 128>(p, s);
-      return p.dim <= 64 ? run_stream<T, false, 64>(p, s) : run_stream<T, false, 128>(p, s);
+      return e2m1 ? run_stream_dim<T, true>(p, s) : run_stream_dim<T, false>(p, s);
     }
   }
   return e2m1 ? run_simple<T, true>(p, s) : run_simple<T, false>(p, s);
@@ -965,6 +997,13 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
   p.max_rows = INT64_MAX;
   const bool stream_kernel = stream_ok(a);
   if (stream_kernel) {
+    p.unit = static_cast<uint32_t>(place_unit(c));
+    const int64_t elem = e2m1 ? 1 : 2;
+    p.k_page_u = static_cast<uint32_t>(c.k_page_stride * elem / p.unit);
+    p.v_page_u = static_cast<uint32_t>(c.v_page_stride * elem / p.unit);
+    p.row_u = static_cast<uint32_t>((e2m1 ? c.dim / 2 : c.dim * 2) / p.unit);
+    p.ks_page_u = static_cast<uint32_t>(c.ks_page_stride / 16);
+    p.vs_page_u = static_cast<uint32_t>(c.vs_page_stride / 16);
     p.workers = stream_workers(e2m1, device_num_sms());
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + int64_t{2} * p.workers * kRowTile * padded_dim(c.dim);

@@ -14,6 +14,9 @@ struct PagedParams {
   const void* ks;
   const void* vs;
   int64_t k_page, k_head, v_page, v_head, ks_page, ks_head, vs_page, vs_head;
+  // The same for the streaming kernel: strides in units of `unit` bytes, of the
+  // scales in 16 bytes.
+  uint32_t unit, k_page_u, v_page_u, row_u, ks_page_u, vs_page_u;
   int num_pages, kv_heads, page_size, dim, q_heads, group;
   Seqs seqs;
   int window;
