@@ -115,18 +115,18 @@ __global__ void __launch_bounds__(kSimpleThreads) paged_simple_kernel(const __gr
 }
 
 // ------------------------------------------------------- streaming kernel --
-constexpr int kRowTile = 16;
 constexpr int kWarps = 4;
 constexpr int kStreamThreads = 32 * kWarps;
 constexpr int kMaxBatch = 1024;          // sequences per launch (their prefix sums stand in shared memory)
 constexpr float kRescaleLog2 = 8.0f;
 
-// Sizes of one instance; DP is the head dimension rounded up to 64 or 128.
-template <bool E2M1, int DP>
+// Sizes of one instance; DP is the head dimension rounded up to 64 or 128, NT
+// the 8-row tiles of queries that share the keys.
+template <bool E2M1, int DP, int NT>
 struct Shape {
+  static constexpr int kRows = 8 * NT;
   static constexpr int KT = E2M1 || DP == 64 ? 32 : 16;   // keys per tile
-  static constexpr int kSteps = DP / 16;                  // k-steps of Q K^T
-  static constexpr int kCols = DP / 8;                    // n-tiles of P V
+  static constexpr int kSteps = DP / 16;                  // k-steps of K Q^T
   static constexpr int kRun = E2M1 ? DP / 8 : 8;          // neighbouring columns of V that a lane holds
   // 16 bits: 16-byte pieces per lane and row. 4 bits: rows of DP / 2 bytes of
   // codes; V's rows are padded so that the four rows that a quarter warp reads
@@ -136,9 +136,9 @@ struct Shape {
   static constexpr int kKBytes = KT * kKRow, kVBytes = KT * kVRow;
   static constexpr int kScaleBytes = E2M1 ? KT * (DP / 16) : 0;   // of K, and of V
   static constexpr int kStageBytes = kKBytes + kVBytes + 2 * kScaleBytes;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = E2M1 ? (NT == 1 ? 2 : 3) : 3;
   static constexpr int kRingBytes = kStages * kStageBytes;        // per warp
-  static constexpr int kCtasPerSm = E2M1 ? 3 : 2;
+  static constexpr int kCtasPerSm = E2M1 ? (NT == 1 ? 4 : 3) : 2;
 };
 
 // 16 bytes to shared memory, or zeros (then nothing is read).
@@ -179,17 +179,25 @@ __device__ __forceinline__ void sts8(uint32_t a, uint32_t v) {
   asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 
+// The 8 x 8 matrix of 16-bit elements whose rows the lanes 4 r .. 4 r + 3 hold, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
 // D += A B, m16n8k16: A row-major, B column-major, 16-bit, fp32 accumulators.
 template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
@@ -216,47 +224,72 @@ __device__ __forceinline__ uint32_t scales_to_half2(uint32_t two) {
 }
 
 // Row tiles of a sequence, and the key tiles of each of them.
-__device__ __forceinline__ void seq_tiles(const PagedParams& p, const SeqInfo& s, int KT, int& row_tiles, int& tiles) {
+struct Tiling {
+  int KT, rows;   // keys and rows of a tile
+};
+__device__ __forceinline__ void seq_tiles(const PagedParams& p, const SeqInfo& s, Tiling tl, int& row_tiles, int& tiles) {
   const int64_t rows = static_cast<int64_t>(s.n) * p.group;
   if (rows < p.min_rows || rows >= p.max_rows || s.hi <= s.lo) {
     row_tiles = tiles = 0;
     return;
   }
-  row_tiles = static_cast<int>((rows + kRowTile - 1) / kRowTile);
-  tiles = (s.hi + KT - 1) / KT - s.lo / KT;
+  row_tiles = static_cast<int>((rows + tl.rows - 1) / tl.rows);
+  tiles = (s.hi + tl.KT - 1) / tl.KT - s.lo / tl.KT;
 }
 
 // prefix[b] = tiles of the sequences before b (batch + 1 entries in shared
-// memory), by the whole block.
-__device__ __forceinline__ void prefix_tiles(const PagedParams& p, int KT, int64_t* prefix, int64_t* warp_sums) {
+// memory), by the whole block. SEGMENTS: segments[b] = their (key head, row
+// tile) pairs that have tiles, likewise.
+template <bool SEGMENTS>
+__device__ __forceinline__ void prefix_tiles(const PagedParams& p, Tiling tl, int64_t* prefix, int64_t* warp_sums,
+                                             int* segments = nullptr, int* warp_segments = nullptr) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int64_t carry = 0;
+  int carry_segments = 0;
   for (int b0 = 0; b0 < p.seqs.batch; b0 += blockDim.x) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    int64_t x = 0;
+    int64_t inc = 0;
+    int inc_segments = 0;
     if (b < p.seqs.batch) {
       int rt, nt;
-      seq_tiles(p, load_seq(p, b), KT, rt, nt);
-      x = static_cast<int64_t>(p.kv_heads) * rt * nt;
+      seq_tiles(p, load_seq(p, b), tl, rt, nt);
+      inc_segments = p.kv_heads * rt;
+      inc = static_cast<int64_t>(inc_segments) * nt;
     }
-    int64_t inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
+      if constexpr (SEGMENTS) {
+        const int z = __shfl_up_sync(0xffffffffu, inc_segments, o);
+        if (lane >= o) inc_segments += z;
+      }
     }
-    if (lane == 31) warp_sums[warp] = inc;
+    if (lane == 31) {
+      warp_sums[warp] = inc;
+      if constexpr (SEGMENTS) warp_segments[warp] = inc_segments;
+    }
     __syncthreads();
-    int64_t before = carry, all = 0;
+    int64_t before = carry;
+    int before_segments = carry_segments;
     for (int w = 0; w < warps; ++w) {
       if (w < warp) before += warp_sums[w];
-      all += warp_sums[w];
+      carry += warp_sums[w];
+      if constexpr (SEGMENTS) {
+        if (w < warp) before_segments += warp_segments[w];
+        carry_segments += warp_segments[w];
+      }
     }
-    if (b < p.seqs.batch) prefix[b + 1] = before + inc;
-    carry += all;
+    if (b < p.seqs.batch) {
+      prefix[b + 1] = before + inc;
+      if constexpr (SEGMENTS) segments[b + 1] = before_segments + inc_segments;
+    }
     __syncthreads();
   }
-  if (threadIdx.x == 0) prefix[0] = 0;
+  if (threadIdx.x == 0) {
+    prefix[0] = 0;
+    if constexpr (SEGMENTS) segments[0] = 0;
+  }
   __syncthreads();
 }
 
@@ -273,12 +306,13 @@ __device__ __forceinline__ int run_of(int64_t total, int workers, int64_t t) {
 }
 
 // EXACT: the head dimension is DP, a constant.
-template <typename T, bool E2M1, int DP, bool EXACT>
-__global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
+template <typename T, bool E2M1, int DP, int NT, bool EXACT>
+__global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerSm)
     paged_stream_kernel(const __grid_constant__ PagedParams p) {
-  using S = Shape<E2M1, DP>;
+  using S = Shape<E2M1, DP, NT>;
   using M = typename std::conditional<E2M1, __half, T>::type;   // type of the products
   constexpr int KT = S::KT;
+  constexpr Tiling kTiling{S::KT, S::kRows};
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t warp_sums[kWarps];
   int64_t* prefix = reinterpret_cast<int64_t*>(smem + kWarps * S::kRingBytes);
@@ -287,7 +321,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
   const uint32_t ring = smem_u32(smem) + warp * S::kRingBytes;
   pdl_wait();
   pdl_launch_dependents();
-  prefix_tiles(p, KT, prefix, warp_sums);
+  prefix_tiles<false>(p, kTiling, prefix, warp_sums);
   const int64_t total = prefix[p.seqs.batch];
   const int workers = used_workers(p, total), worker = static_cast<int>(blockIdx.x) * kWarps + warp;
   if (worker >= workers) return;
@@ -306,29 +340,25 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
     }
     const SeqInfo s = load_seq(p, b);
     int row_tiles, seg_tiles;
-    seq_tiles(p, s, KT, row_tiles, seg_tiles);
+    seq_tiles(p, s, kTiling, row_tiles, seg_tiles);
     const int64_t in_seq = t - prefix[b];
     const int seg = static_cast<int>(in_seq / seg_tiles);
     const int tile0 = static_cast<int>(in_seq - static_cast<int64_t>(seg) * seg_tiles);
     const int kh = seg / row_tiles, rt = seg - kh * row_tiles;
     const int n_tiles = static_cast<int>(min(static_cast<int64_t>(seg_tiles - tile0), t_end - t));
     const int key0 = (s.lo / KT + tile0) * KT;
-    const int rows = min(kRowTile, s.n * p.group - rt * kRowTile);
+    const int row0 = rt * S::kRows, rows = min(S::kRows, s.n * p.group - row0);
 
-    // This lane's rows g and g + 8: their token, head and visible keys.
-    int tok[2], head[2], lo[2], hi[2];
+    // Keys that the lane's query columns 2 c and 2 c + 1 (of each 8-row tile) see.
+    int lo[NT][2], hi[NT][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = rt * kRowTile + min(g + 8 * r, rows - 1);
-      const int i = row / p.group;
-      tok[r] = s.first + i;
-      head[r] = kh * p.group + row - i * p.group;
-      visible(p, s.pos0 + i, lo[r], hi[r]);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) visible(p, s.pos0 + (row0 + min(8 * n + 2 * c + r, rows - 1)) / p.group, lo[n][r], hi[n][r]);
     // Keys that some row sees, and that all rows see.
     int any_lo, any_hi, all_lo, all_hi;
-    visible(p, s.pos0 + (rt * kRowTile + rows - 1) / p.group, all_lo, any_hi);
-    visible(p, s.pos0 + rt * kRowTile / p.group, any_lo, all_hi);
+    visible(p, s.pos0 + (row0 + rows - 1) / p.group, all_lo, any_hi);
+    visible(p, s.pos0 + row0 / p.group, any_lo, all_hi);
 
     // -------------------------------------------------------------- pages --
     // Lane l looks up the l-th group of 8 keys of a batch of 256 (grouped) or
@@ -444,68 +474,74 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
     }
 
     // ------------------------------------------------------------ queries --
-    uint32_t qf[S::kSteps][4];
-    float sl2[2];
+    // Q^T as the B operand: the lane holds query row g of each 8-row tile.
+    uint32_t qf[NT][S::kSteps][2];
     // The maximum below needs a positive factor: a negative scale turns the
     // queries' signs instead, and a zero one becomes too small to matter.
-    sl2[0] = sl2[1] = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);
+    float sl2[NT][2];   // of the columns 2 c, 2 c + 1
+    const float scale_log2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    {
-      const T* q0 = static_cast<const T*>(p.q) + tok[0] * p.q_tok + head[0] * p.q_head;
-      const T* q1 = static_cast<const T*>(p.q) + tok[1] * p.q_tok + head[1] * p.q_head;
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        // The lane's i-th 8 elements: with 16 bits pieces c + 4 i of K's rows,
-        // with 4 bits its i-th word of DP / 32 neighbouring ones.
-        const int d = E2M1 ? (DP / 4) * c + 8 * i : 8 * (c + 4 * i);
-        uint4 u0 = make_uint4(0u, 0u, 0u, 0u), u1 = u0;
-        if (d < dim) {
-          u0 = *reinterpret_cast<const uint4*>(q0 + d);
-          u1 = *reinterpret_cast<const uint4*>(q1 + d);
-          u0.x ^= flip; u0.y ^= flip; u0.z ^= flip; u0.w ^= flip;
-          u1.x ^= flip; u1.y ^= flip; u1.z ^= flip; u1.w ^= flip;
-        }
-        qf[2 * i][0] = u0.x; qf[2 * i][1] = u1.x; qf[2 * i][2] = u0.y; qf[2 * i][3] = u1.y;
-        qf[2 * i + 1][0] = u0.z; qf[2 * i + 1][1] = u1.z; qf[2 * i + 1][2] = u0.w; qf[2 * i + 1][3] = u1.w;
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + min(8 * n + g, rows - 1), i = row / p.group;
+      const T* q = static_cast<const T*>(p.q) + (s.first + i) * p.q_tok + (kh * p.group + row - i * p.group) * p.q_head;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        // The lane's j-th 8 elements: with 16 bits piece c + 4 j of the row,
+        // with 4 bits the j-th 8 of DP / 4 neighbouring ones.
+        const int d = E2M1 ? (DP / 4) * c + 8 * j : 8 * (c + 4 * j);
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (d < dim) u = *reinterpret_cast<const uint4*>(q + d);
+        qf[n][2 * j][0] = u.x ^ flip; qf[n][2 * j][1] = u.y ^ flip;
+        qf[n][2 * j + 1][0] = u.z ^ flip; qf[n][2 * j + 1][1] = u.w ^ flip;
       }
+      float up = 1.f;
       if constexpr (E2M1 && std::is_same<T, __nv_bfloat16>::value) {
-        float top[2] = {0.f, 0.f};
+        float top = 0.f;
 #pragma unroll
         for (int w = 0; w < S::kSteps; ++w)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = Io<T>::unpack2(qf[w][i]);
-            top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(f.x), fabsf(f.y)));
+          for (int k = 0; k < 2; ++k) {
+            const float2 f = Io<T>::unpack2(qf[n][w][k]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
-        float down[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-          // 2^-e for 2^e <= top < 2^(e + 1), whose scale goes to the scores;
-          // rows of zeros and rows at fp32's ends stay as they are.
-          const uint32_t e = __float_as_uint(top[r]) >> 23;
-          const bool use = e > 64u && e < 190u;
-          down[r] = use ? __uint_as_float((254u - e) << 23) : 1.f;
-          sl2[r] *= use ? __uint_as_float(e << 23) : 1.f;
-        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // Times 2^-e for 2^e <= top < 2^(e + 1), and the scores times 2^e;
+        // rows of zeros and rows at fp32's ends stay as they are.
+        const uint32_t e = __float_as_uint(top) >> 23;
+        const bool use = e > 64u && e < 190u;
+        const float down = use ? __uint_as_float((254u - e) << 23) : 1.f;
+        up = use ? __uint_as_float(e << 23) : 1.f;
 #pragma unroll
         for (int w = 0; w < S::kSteps; ++w)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = Io<T>::unpack2(qf[w][i]);
-            qf[w][i] = Io<__half>::pack2(f.x * down[i & 1], f.y * down[i & 1]);
+          for (int k = 0; k < 2; ++k) {
+            const float2 f = Io<T>::unpack2(qf[n][w][k]);
+            qf[n][w][k] = Io<__half>::pack2(f.x * down, f.y * down);
           }
       }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) sl2[n][r] = scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * c + r));
     }
 
     // ---------------------------------------------------------- key tiles --
-    float acc[S::kCols][4];
+    // O^T: m-tile j holds, in rows g and g + 8, the lane's elements 2 j and
+    // 2 j + 1 of V's row, for the query columns 2 c and 2 c + 1.
+    constexpr int kMTiles = DP / 16;
+    float acc[NT][kMTiles][4];
 #pragma unroll
-    for (int j = 0; j < S::kCols; ++j)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // maximum (scaled, log2) and this lane's part of the sum
+      for (int j = 0; j < kMTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
+    float m[NT][2], l[NT][2];   // per column: maximum (scaled, log2), and this lane's part of the sum
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
 
     int stage = 0;
     for (int i = 0; i < n_tiles; ++i) {
@@ -533,42 +569,50 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
             __syncwarp();
           }
         }
-        // S = Q K^T
-        float sc[KT / 8][4];
+        // S^T = K Q^T: m-tiles of 16 keys (rows g and g + 8 of each).
+        float sc[NT][KT / 16][4];
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+          for (int a = 0; a < KT / 16; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][a][e] = 0.f;
         if constexpr (E2M1) {
           const uint32_t k_scales = at + S::kKBytes + S::kVBytes;
+          constexpr int kWords = DP / 32;   // words of 8 codes per lane and key
 #pragma unroll
-          for (int n = 0; n < KT / 8; ++n) {
-            const uint32_t row = at + (8 * n + g) * S::kKRow;
-            if constexpr (DP == 128) {
-              const uint32_t two = EXACT || 2 * c < srow ? lds16(k_scales + (8 * n + g) * srow + 2 * c) : 0u;
-              const uint32_t s01 = scales_to_half2(two);
-              const uint32_t s0 = __byte_perm(s01, s01, 0x1010), s1 = __byte_perm(s01, s01, 0x3232);
-              const uint4 w = lds128(row + 16 * c);
-              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+          for (int a = 0; a < KT / 16; ++a) {
+            uint32_t w[2][kWords], sx[2][2];   // of keys g and g + 8
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t h[4];
-                codes_to_half2(ws[q], h);
-                const uint32_t sx = q < 2 ? s0 : s1;
-                mma16816<M>(sc[n], qf[2 * q], hmul2(h[0], sx), hmul2(h[1], sx));
-                mma16816<M>(sc[n], qf[2 * q + 1], hmul2(h[2], sx), hmul2(h[3], sx));
+            for (int h = 0; h < 2; ++h) {
+              const int key = 16 * a + 8 * h + g;
+              if constexpr (DP == 128) {
+                const uint4 u = lds128(at + key * S::kKRow + 16 * c);
+                w[h][0] = u.x; w[h][1] = u.y; w[h][2] = u.z; w[h][3] = u.w;
+                const uint32_t s01 = scales_to_half2(EXACT || 2 * c < srow ? lds16(k_scales + key * srow + 2 * c) : 0u);
+                sx[h][0] = __byte_perm(s01, s01, 0x1010);
+                sx[h][1] = __byte_perm(s01, s01, 0x3232);
+              } else {
+                const uint2 u = lds64(at + key * S::kKRow + 8 * c);
+                w[h][0] = u.x; w[h][1] = u.y;
+                sx[h][0] = sx[h][1] = scales_to_half2((EXACT || c < srow ? lds8(k_scales + key * srow + c) : 0u) * 0x101u);
               }
-            } else {
-              const uint32_t one = EXACT || c < srow ? lds8(k_scales + (8 * n + g) * srow + c) : 0u;
-              const uint32_t sx = scales_to_half2(one * 0x101u);
-              const uint2 w = lds64(row + 8 * c);
-              const uint32_t ws[2] = {w.x, w.y};
+            }
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                uint32_t h[4];
-                codes_to_half2(ws[q], h);
-                mma16816<M>(sc[n], qf[2 * q], hmul2(h[0], sx), hmul2(h[1], sx));
-                mma16816<M>(sc[n], qf[2 * q + 1], hmul2(h[2], sx), hmul2(h[3], sx));
+            for (int q = 0; q < kWords; ++q) {
+              uint32_t x[4], y[4];
+              codes_to_half2(w[0][q], x);
+              codes_to_half2(w[1][q], y);
+              const uint32_t s0 = sx[0][2 * q / kWords], s1 = sx[1][2 * q / kWords];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                x[k] = hmul2(x[k], s0);
+                y[k] = hmul2(y[k], s1);
+              }
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma16816<M>(sc[n][a], x[0], y[0], x[1], y[1], qf[n][2 * q][0], qf[n][2 * q][1]);
+                mma16816<M>(sc[n][a], x[2], y[2], x[3], y[3], qf[n][2 * q + 1][0], qf[n][2 * q + 1][1]);
               }
             }
           }
@@ -576,63 +620,80 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
 #pragma unroll
           for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
-            for (int n = 0; n < KT / 8; ++n) {
-              const uint4 u = lds128(at + ((n * (DP / 32) + j) * 32 + lane) * 16);
-              mma16816<M>(sc[n], qf[2 * j], u.x, u.y);
-              mma16816<M>(sc[n], qf[2 * j + 1], u.z, u.w);
+            for (int a = 0; a < KT / 16; ++a) {
+              const uint4 u = lds128(at + ((2 * a * (DP / 32) + j) * 32 + lane) * 16);
+              const uint4 v = lds128(at + (((2 * a + 1) * (DP / 32) + j) * 32 + lane) * 16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma16816<M>(sc[n][a], u.x, v.x, u.y, v.y, qf[n][2 * j][0], qf[n][2 * j][1]);
+                mma16816<M>(sc[n][a], u.z, v.z, u.w, v.w, qf[n][2 * j + 1][0], qf[n][2 * j + 1][1]);
+              }
             }
         }
-        // Masks, where the tile has a key that not every row sees. (A key
-        // column n, 2 c + e stands at 8 n + 2 c + e.)
+        // Masks, where the tile has a key that not every row sees. Element e of
+        // m-tile a: key 16 a + 8 (e / 2) + g, column 2 c + e % 2.
         if (ok != kFull || first < all_lo || first + KT > all_hi) {
 #pragma unroll
-          for (int n = 0; n < KT / 8; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int local = 8 * n + 2 * c + (e & 1), key = first + local;
-              if (((ok >> local) & 1u) == 0u || key < lo[e >> 1] || key >= hi[e >> 1]) sc[n][e] = -INFINITY;
-            }
+            for (int a = 0; a < KT / 16; ++a)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int local = 16 * a + 8 * (e >> 1) + g, key = first + local;
+                if (((ok >> local) & 1u) == 0u || key < lo[n][e & 1] || key >= hi[n][e & 1]) sc[n][a][e] = -INFINITY;
+              }
         }
-        // Running maximum; NaN propagates, so a NaN score makes its row NaN.
-        float top[2];
+        // Running maxima; NaN propagates, so a NaN score makes its row NaN.
+        float top[NT][2];
+        bool grown = false;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float x = -INFINITY;
-#pragma unroll
-          for (int n = 0; n < KT / 8; ++n) x = fmax3_nan(x, sc[n][2 * r], sc[n][2 * r + 1]);
-          x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          top[r] = x * sl2[r];
-        }
-        const bool grown = !(top[0] <= m[0] + kRescaleLog2) || !(top[1] <= m[1] + kRescaleLog2);
-        if (__any_sync(0xffffffffu, grown)) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float next = fmax_nan(m[r], top[r]);
-            const float alpha = next == -INFINITY ? 1.f : ex2_approx(m[r] - next);
-            m[r] = next;
-            l[r] *= alpha;
+            float x = fmax_nan(sc[n][0][r], sc[n][0][2 + r]);
 #pragma unroll
-            for (int j = 0; j < S::kCols; ++j) {
-              acc[j][2 * r] *= alpha;
-              acc[j][2 * r + 1] *= alpha;
+            for (int a = 1; a < KT / 16; ++a) x = fmax3_nan(x, sc[n][a][r], sc[n][a][2 + r]);
+            x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            top[n][r] = x * sl2[n][r];
+            grown |= !(top[n][r] <= m[n][r] + kRescaleLog2);
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float next = fmax_nan(m[n][r], top[n][r]);
+              const float alpha = next == -INFINITY ? 1.f : ex2_approx(m[n][r] - next);
+              m[n][r] = next;
+              l[n][r] *= alpha;
+#pragma unroll
+              for (int j = 0; j < kMTiles; ++j) {
+                acc[n][j][r] *= alpha;
+                acc[n][j][2 + r] *= alpha;
+              }
             }
+        }
+        // P^T as the B operand of V^T P^T: 8 x 8 blocks transposed.
+        uint32_t pf[NT][KT / 16][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float off0 = m[n][0] == -INFINITY ? 0.f : m[n][0], off1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+          for (int a = 0; a < KT / 16; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sc[n][a][e] = ex2_approx(fmaf(sc[n][a][e], sl2[n][e & 1], (e & 1) == 0 ? -off0 : -off1));
+            l[n][0] += sc[n][a][0] + sc[n][a][2];
+            l[n][1] += sc[n][a][1] + sc[n][a][3];
+            pf[n][a][0] = transpose8x8(Io<M>::pack2(sc[n][a][0], sc[n][a][1]));
+            pf[n][a][1] = transpose8x8(Io<M>::pack2(sc[n][a][2], sc[n][a][3]));
           }
         }
-        const float off0 = m[0] == -INFINITY ? 0.f : m[0], off1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll
-        for (int n = 0; n < KT / 8; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] = ex2_approx(fmaf(sc[n][e], sl2[e >> 1], e < 2 ? -off0 : -off1));
-          l[0] += sc[n][0] + sc[n][1];
-          l[1] += sc[n][2] + sc[n][3];
-        }
-        // O += P V
+        // O^T += V^T P^T
 #pragma unroll
         for (int a = 0; a < KT / 16; ++a) {
-          const uint32_t pf[4] = {Io<M>::pack2(sc[2 * a][0], sc[2 * a][1]), Io<M>::pack2(sc[2 * a][2], sc[2 * a][3]),
-                                  Io<M>::pack2(sc[2 * a + 1][0], sc[2 * a + 1][1]),
-                                  Io<M>::pack2(sc[2 * a + 1][2], sc[2 * a + 1][3])};
           if constexpr (E2M1) {
             // This lane's columns lie in one scale block. (Where it is behind
             // the head dimension another key's scale is read; those columns
@@ -661,19 +722,24 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
               }
 #pragma unroll
             for (int q = 0; q < kW; ++q) {
-              // Bytes that pair the codes of two keys: even and odd columns.
+              // Bytes that pair the codes of two keys: even and odd elements.
               uint32_t ev[2][4], od[2][4];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const uint32_t x = w[h][0][q], y = w[h][1][q];
                 codes_to_half2((x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u), ev[h]);
                 codes_to_half2(((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), od[h]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  ev[h][j] = hmul2(ev[h][j], sx[h]);
+                  od[h][j] = hmul2(od[h][j], sx[h]);
+                }
               }
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                mma16816<M>(acc[8 * q + 2 * j], pf, hmul2(ev[0][j], sx[0]), hmul2(ev[1][j], sx[1]));
-                mma16816<M>(acc[8 * q + 2 * j + 1], pf, hmul2(od[0][j], sx[0]), hmul2(od[1][j], sx[1]));
-              }
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma16816<M>(acc[n][4 * q + j], ev[0][j], od[0][j], ev[1][j], od[1][j], pf[n][a][0], pf[n][a][1]);
             }
           } else {
 #pragma unroll
@@ -686,10 +752,10 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
               }
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                mma16816<M>(acc[8 * j + 2 * q], pf, __byte_perm(w[0][q], w[1][q], 0x5410),
-                            __byte_perm(w[2][q], w[3][q], 0x5410));
-                mma16816<M>(acc[8 * j + 2 * q + 1], pf, __byte_perm(w[0][q], w[1][q], 0x7632),
-                            __byte_perm(w[2][q], w[3][q], 0x7632));
+                const uint32_t a0 = __byte_perm(w[0][q], w[1][q], 0x5410), a1 = __byte_perm(w[0][q], w[1][q], 0x7632);
+                const uint32_t a2 = __byte_perm(w[2][q], w[3][q], 0x5410), a3 = __byte_perm(w[2][q], w[3][q], 0x7632);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<M>(acc[n][4 * j + q], a0, a1, a2, a3, pf[n][a][0], pf[n][a][1]);
               }
             }
           }
@@ -702,29 +768,33 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
 
     // ------------------------------------------------------------- results --
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
     const bool whole = tile0 == 0 && n_tiles == seg_tiles;
     const int64_t part = static_cast<int64_t>(worker) * 2 + (t == t_first ? 0 : 1);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (g + 8 * r < rows) {
-        const float f = whole ? (l[r] == 0.f ? 0.f : p.v_gain / l[r]) : 1.f;
-        T* out = static_cast<T*>(p.o) + tok[r] * p.o_tok + head[r] * p.o_head;
-        float* po = p.part_o + (part * kRowTile + g + 8 * r) * DP;
-        // Column n = 2 c + e of the n-tile j is element 64 i + kRun n + (j % kRun), j = kRun i + ...
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < S::kCols / S::kRun; ++i)
+      for (int r = 0; r < 2; ++r) {
+        const int in_tile = 8 * n + 2 * c + r, row = row0 + in_tile;
+        if (in_tile < rows) {
+          const bool none = l[n][r] == 0.f;
+          const float f = whole ? p.v_gain / l[n][r] : 1.f;
+          const int i = row / p.group;
+          T* out = static_cast<T*>(p.o) + (s.first + i) * p.o_tok + (kh * p.group + row - i * p.group) * p.o_head;
+          float* po = p.part_o + (part * S::kRows + in_tile) * DP;
+          // The lane's kRun neighbouring elements kRun g + 64 k ..
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int k = 0; k < DP / (8 * S::kRun); ++k)
 #pragma unroll
             for (int d8 = 0; d8 < S::kRun; d8 += 8) {
-              const int d = 64 * i + S::kRun * (2 * c + e) + d8;
+              const int d = 64 * k + S::kRun * g + d8, j0 = (S::kRun * k + d8) / 2;
               float x[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) x[k] = l[r] == 0.f ? 0.f : acc[S::kRun * i + d8 + k][2 * r + e] * f;
+              for (int e = 0; e < 8; ++e) x[e] = none ? 0.f : acc[n][j0 + (e >> 1)][2 * (e & 1) + r] * f;
               if (whole) {
                 if (d < dim)
                   *reinterpret_cast<uint4*>(out + d) = make_uint4(Io<T>::pack2(x[0], x[1]), Io<T>::pack2(x[2], x[3]),
@@ -734,57 +804,40 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP>::kCtasPerSm)
                 *reinterpret_cast<float4*>(po + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
               }
             }
-        if (!whole && c == 0)
-          *reinterpret_cast<float2*>(p.part_ml + (part * kRowTile + g + 8 * r) * 2) = make_float2(m[r], l[r]);
+          if (!whole && g == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (part * S::kRows + in_tile) * 2) = make_float2(m[n][r], l[n][r]);
+        }
       }
-    }
     t += n_tiles;
   }
 }
 
-// Joins the parts of the rows whose keys several workers took, and clears the
-// rows of sequences without keys. Block x takes the row tile that run x begins
-// inside, if no earlier run begins inside it too; blockIdx.y takes every
-// kJoinShares-th row, its warps every fourth part. The lengths are read before
-// the streaming kernel has ended (it has started, so whatever came before it is
-// complete), the parts after it.
+// Joins the parts of the segments (key head, row tile) that several workers
+// took, and clears the rows of sequences without keys. A block per segment (and
+// more, where there are more than blocks); blockIdx.y takes every kJoinShares-th
+// row, its warps every fourth part. The lengths are read before the streaming
+// kernel has ended (it has started, so whatever came before it is complete),
+// the parts after it.
 constexpr int kJoinThreads = 128, kJoinShares = 4;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int KT) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, Tiling tl) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t warp_sums[kJoinThreads / 32];
+  __shared__ int warp_segments[kJoinThreads / 32];
   __shared__ float s_o[kJoinThreads / 32][DP];
   __shared__ float2 s_ml[kJoinThreads / 32];
   int64_t* prefix = reinterpret_cast<int64_t*>(smem);
+  int* segments = reinterpret_cast<int*>(prefix + p.seqs.batch + 1);
   const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
   constexpr int kWarpsHere = kJoinThreads / 32, kE = DP / 32;
-  prefix_tiles(p, KT, prefix, warp_sums);
+  prefix_tiles<true>(p, tl, prefix, warp_sums, segments, warp_segments);
   const int64_t total = prefix[p.seqs.batch];
-  const int workers = used_workers(p, total), w1 = static_cast<int>(blockIdx.x);
-  SeqInfo s{};
-  int row_tiles = 0, seg_tiles = 1, kh = 0, rt = 0;
-  int64_t start = 0;
-  bool mine = w1 > 0 && w1 < workers;
-  if (mine) {
-    const int64_t t = run_start(total, workers, w1);
-    int b = 0;
-    for (int end = p.seqs.batch; b + 1 < end;) {   // last b with prefix[b] <= t
-      const int mid = (b + end) >> 1;
-      if (prefix[mid] <= t) b = mid; else end = mid;
-    }
-    s = load_seq(p, b);
-    seq_tiles(p, s, KT, row_tiles, seg_tiles);
-    const int seg = static_cast<int>((t - prefix[b]) / seg_tiles);
-    kh = seg / row_tiles;
-    rt = seg - kh * row_tiles;
-    start = prefix[b] + static_cast<int64_t>(seg) * seg_tiles;
-    mine = t > start && run_start(total, workers, w1 - 1) <= start;
-  }
+  const int workers = used_workers(p, total);
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.y == 0) {
-    for (int b = w1; b < p.seqs.batch; b += gridDim.x) {
+    for (int b = blockIdx.x; b < p.seqs.batch; b += gridDim.x) {
       const SeqInfo z = load_seq(p, b);
       const int64_t rows = static_cast<int64_t>(z.n) * p.group;
       if (rows < p.min_rows || rows >= p.max_rows || z.hi > z.lo) continue;
@@ -794,57 +847,69 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
           static_cast<T*>(p.o)[token * p.o_tok + e / p.dim * p.o_head + e % p.dim] = Io<T>::from_f(0.f);
     }
   }
-  if (!mine) return;
-  const int w0 = w1 - 1, last = run_of(total, workers, start + seg_tiles - 1);
-  const int first_slot = run_start(total, workers, w0) == start ? 0 : 1;
-  const int rows = min(kRowTile, s.n * p.group - rt * kRowTile);
-  for (int r = static_cast<int>(blockIdx.y); r < rows; r += kJoinShares) {
-    float m = -INFINITY, l = 0.f, o[kE];
+  for (int x = blockIdx.x; x < segments[p.seqs.batch]; x += gridDim.x) {
+    int b = 0;
+    for (int end = p.seqs.batch; b + 1 < end;) {   // last b with segments[b] <= x
+      const int mid = (b + end) >> 1;
+      if (segments[mid] <= x) b = mid; else end = mid;
+    }
+    const SeqInfo s = load_seq(p, b);
+    int row_tiles, seg_tiles;
+    seq_tiles(p, s, tl, row_tiles, seg_tiles);
+    const int seg = x - segments[b], kh = seg / row_tiles, rt = seg - kh * row_tiles;
+    const int64_t start = prefix[b] + static_cast<int64_t>(seg) * seg_tiles;
+    const int w0 = run_of(total, workers, start), last = run_of(total, workers, start + seg_tiles - 1);
+    if (w0 == last) continue;   // its worker has written it
+    const int first_slot = run_start(total, workers, w0) == start ? 0 : 1;
+    const int rows = min(tl.rows, s.n * p.group - rt * tl.rows);
+    for (int r = static_cast<int>(blockIdx.y); r < rows; r += kJoinShares) {
+      float m = -INFINITY, l = 0.f, o[kE];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = 0.f;
+      for (int e = 0; e < kE; ++e) o[e] = 0.f;
 #pragma unroll 4
-    for (int w = w0 + warp; w <= last; w += kWarpsHere) {
-      const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * kRowTile + r;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      float x[kE];
-      if constexpr (kE == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
-        x[0] = v.x; x[1] = v.y;
+      for (int w = w0 + warp; w <= last; w += kWarpsHere) {
+        const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * tl.rows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+        float x[kE];
+        if constexpr (kE == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
+          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
+          x[0] = v.x; x[1] = v.y;
+        }
+        const float next = fmax_nan(m, ml.x);
+        const float base = next == -INFINITY ? 0.f : next;
+        const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
+        l = l * fa + ml.y * fb;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
+        m = next;
       }
-      const float next = fmax_nan(m, ml.x);
-      const float base = next == -INFINITY ? 0.f : next;
-      const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
-      l = l * fa + ml.y * fb;
+      __syncthreads();   // the row before has been read
 #pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
-      m = next;
-    }
-    __syncthreads();   // the row before has been read
+      for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
+      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      __syncthreads();
+      float top = s_ml[0].x;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
-    if (lane == 0) s_ml[warp] = make_float2(m, l);
-    __syncthreads();
-    float top = s_ml[0].x;
+      for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, f[kWarpsHere];
 #pragma unroll
-    for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, f[kWarpsHere];
+      for (int w = 0; w < kWarpsHere; ++w) {
+        f[w] = ex2_approx(s_ml[w].x - base);
+        sum += s_ml[w].y * f[w];
+      }
+      const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
+      const int row = rt * tl.rows + r, i = row / p.group;
+      T* out = static_cast<T*>(p.o) + (s.first + i) * p.o_tok + (kh * p.group + row - i * p.group) * p.o_head;
+      for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
+        float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarpsHere; ++w) {
-      f[w] = ex2_approx(s_ml[w].x - base);
-      sum += s_ml[w].y * f[w];
-    }
-    const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
-    const int row = rt * kRowTile + r, i = row / p.group;
-    T* out = static_cast<T*>(p.o) + (s.first + i) * p.o_tok + (kh * p.group + row - i * p.group) * p.o_head;
-    for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
-      float x = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
-      out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
+        for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
+        out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
+      }
     }
   }
 }
@@ -857,7 +922,16 @@ cudaError_t run_simple(const PagedParams& p, cudaStream_t s) {
 }
 
 int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
-int stream_workers(bool e2m1, int sms) { return sms * kWarps * (e2m1 ? 3 : 2); }
+
+// 8-row tiles that share the keys: one where a sequence is likely to have no
+// more than 8 query rows (by the caller's hint, else by the mean), two else. With
+// one the products, exponentials and accumulators are half as many (four
+// 131072-key 4-bit contexts of 4 rows: @NT1@ us, with two @NT2@).
+int row_tiles_of(const lunarad_paged_attention_args& a) {
+  const int64_t mean = (a.seqs.tokens + a.seqs.batch - 1) / a.seqs.batch;
+  return (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / a.cache->kv_heads) <= 8 ? 1 : 2;
+}
+int stream_workers(bool e2m1, int nt, int sms) { return sms * kWarps * (e2m1 ? (nt == 1 ? 4 : 3) : 2); }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -908,17 +982,25 @@ bool prefill_ok(const lunarad_paged_attention_args& a) {
 }
 
 int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {
-  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, sms) * kRowTile;
+  const int nt = row_tiles_of(a);
+  const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, nt, sms) * 8 * nt;
   return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-template <typename T, bool E2M1, int DP, bool EXACT>
+// No more segments than this, and few enough blocks to run at once.
+unsigned join_blocks(const PagedParams& p, int rows) {
+  const int64_t most = p.kv_heads * (p.seqs.batch + static_cast<int64_t>(p.seqs.tokens) * p.group / rows);
+  const int64_t cap = int64_t{device_num_sms()} * 4;
+  return static_cast<unsigned>(most < cap ? most : cap);
+}
+
+template <typename T, bool E2M1, int DP, int NT, bool EXACT>
 cudaError_t run_stream(PagedParams p, cudaStream_t s) {
-  using S = Shape<E2M1, DP>;
+  using S = Shape<E2M1, DP, NT>;
   const size_t prefix = sizeof(int64_t) * (static_cast<size_t>(p.seqs.batch < kMaxBatch ? p.seqs.batch : kMaxBatch) + 2);
   const size_t smem = static_cast<size_t>(kWarps) * S::kRingBytes + prefix;
   static_assert(kWarps * S::kRingBytes + 8 * (kMaxBatch + 2) + 1280 <= 228 * 1024 / S::kCtasPerSm, "shared memory per SM");
-  auto kern = paged_stream_kernel<T, E2M1, DP, EXACT>;
+  auto kern = paged_stream_kernel<T, E2M1, DP, NT, EXACT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kWarps * S::kRingBytes + 8 * (kMaxBatch + 2));
   if (e != cudaSuccess) return e;
@@ -931,24 +1013,26 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
     p.seqs.lens = all.lens + b0;
     e = launch_pdl(kern, dim3(p.workers / kWarps), dim3(kStreamThreads), smem, s, p);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(paged_join_kernel<T, DP>, dim3(p.workers, kJoinShares), dim3(kJoinThreads), prefix, s, p, S::KT);
+    e = launch_pdl(paged_join_kernel<T, DP>, dim3(join_blocks(p, S::kRows), kJoinShares), dim3(kJoinThreads),
+                   prefix + 4 * static_cast<size_t>(p.seqs.batch + 1), s, p, Tiling{S::KT, S::kRows});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
-template <typename T, bool E2M1>
+template <typename T, bool E2M1, int NT>
 cudaError_t run_stream_dim(const PagedParams& p, cudaStream_t s) {
-  if (p.dim == 64) return run_stream<T, E2M1, 64, true>(p, s);
-  if (p.dim < 64) return run_stream<T, E2M1, 64, false>(p, s);
-  return p.dim == 128 ? run_stream<T, E2M1, 128, true>(p, s) : run_stream<T, E2M1, 128, false>(p, s);
+  if (p.dim == 64) return run_stream<T, E2M1, 64, NT, true>(p, s);
+  if (p.dim < 64) return run_stream<T, E2M1, 64, NT, false>(p, s);
+  return p.dim == 128 ? run_stream<T, E2M1, 128, NT, true>(p, s) : run_stream<T, E2M1, 128, NT, false>(p, s);
 }
 
 template <typename T>
 cudaError_t run(const PagedParams& p, bool stream_kernel, bool e2m1, cudaStream_t s) {
   if constexpr (!std::is_same<T, float>::value) {
     if (stream_kernel) {
-      return e2m1 ? run_stream_dim<T, true>(p, s) : run_stream_dim<T, false>(p, s);
+      if (e2m1) return p.nt == 1 ? run_stream_dim<T, true, 1>(p, s) : run_stream_dim<T, true, 2>(p, s);
+      return p.nt == 1 ? run_stream_dim<T, false, 1>(p, s) : run_stream_dim<T, false, 2>(p, s);
     }
   }
   return e2m1 ? run_simple<T, true>(p, s) : run_simple<T, false>(p, s);
@@ -1004,9 +1088,10 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
     p.row_u = static_cast<uint32_t>((e2m1 ? c.dim / 2 : c.dim * 2) / p.unit);
     p.ks_page_u = static_cast<uint32_t>(c.ks_page_stride / 16);
     p.vs_page_u = static_cast<uint32_t>(c.vs_page_stride / 16);
-    p.workers = stream_workers(e2m1, device_num_sms());
+    p.nt = row_tiles_of(a);
+    p.workers = stream_workers(e2m1, p.nt, device_num_sms());
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = p.part_o + int64_t{2} * p.workers * kRowTile * padded_dim(c.dim);
+    p.part_ml = p.part_o + int64_t{2} * p.workers * 8 * p.nt * padded_dim(c.dim);
   }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;

@@ -24,7 +24,8 @@ struct PagedParams {
   float v_gain;
   // Sequences with min_rows <= (their tokens * group) < max_rows are this kernel's.
   int64_t min_rows, max_rows;
-  // Split work: partial results of each worker (two slots of kRowTile rows).
+  int nt;   // 8-row tiles per row tile of the streaming kernel
+  // Split work: partial results of each worker (two slots of a row tile).
   float* part_o;
   float* part_ml;
   int workers;
