@@ -13,8 +13,7 @@
 //     tiles with cp.async into a ring of its own in shared memory. The order of
 //     the head dimension inside Q K^T and of the columns of V inside P V is
 //     free; it is chosen so that a lane's mma fragments are contiguous in
-//     memory, and no ldmatrix or swizzle is needed. With 16 bits each lane
-//     copies exactly the 16-byte pieces that it consumes itself.
+//     memory, and no ldmatrix is needed.
 //   * S = Q K^T and O += P V by mma.sync m16n8k16 with fp32 accumulators. At
 //     16 rows these products need a fraction of the legacy tensor rate while
 //     HBM delivers its 23 bytes per clock and SM; tcgen05 needs 64 rows or more
@@ -128,17 +127,13 @@ struct Shape {
   static constexpr int KT = E2M1 || DP == 64 ? 32 : 16;   // keys per tile
   static constexpr int kSteps = DP / 16;                  // k-steps of K Q^T
   static constexpr int kRun = E2M1 ? DP / 8 : 8;          // neighbouring columns of V that a lane holds
-  // 16 bits: 16-byte pieces per lane and row. 4 bits: rows of DP / 2 bytes of
-  // codes; V's rows are padded so that the four rows that a quarter warp reads
-  // at once lie in different banks.
-  static constexpr int kKRow = E2M1 ? DP / 2 : 2 * DP;
-  static constexpr int kVRow = E2M1 ? DP / 2 + 16 : 2 * DP;
-  static constexpr int kKBytes = KT * kKRow, kVBytes = KT * kVRow;
+  static constexpr int kRow = E2M1 ? DP / 2 : 2 * DP;             // bytes of a row, codes or elements
+  static constexpr int kKBytes = KT * kRow, kVBytes = KT * kRow;
   static constexpr int kScaleBytes = E2M1 ? KT * (DP / 16) : 0;   // of K, and of V
   static constexpr int kStageBytes = kKBytes + kVBytes + 2 * kScaleBytes;
-  static constexpr int kStages = E2M1 ? (NT == 1 ? 2 : 3) : 3;
+  static constexpr int kStages = NT == 1 ? 2 : 3;
   static constexpr int kRingBytes = kStages * kStageBytes;        // per warp
-  static constexpr int kCtasPerSm = E2M1 ? (NT == 1 ? 4 : 3) : 2;
+  static constexpr int kCtasPerSm = (E2M1 ? 3 : 2) + (NT == 1 ? 1 : 0);
 };
 
 // 16 bytes to shared memory, or zeros (then nothing is read).
@@ -173,6 +168,25 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   uint32_t u;
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(a) : "memory");
   return u;
+}
+
+// Places in a stage of the 16-byte piece `piece` of K's and V's row r. The rows
+// stand one behind the other, so that 8 neighbouring lanes copy one 128-byte
+// line of memory to one 128-byte line here: a copy whose two sides do not match
+// line by line is cut into a request per sector (measured: 1.5 times the
+// sectors, 4.8 instead of 6 TB/s). Within a line the pieces are permuted so that
+// the lanes of a product read from different banks.
+template <typename S, bool E2M1>
+__device__ __forceinline__ uint32_t k_place(int r, int piece) {
+  if constexpr (E2M1) return r * S::kRow + 16 * piece;
+  else return r * S::kRow + (piece >> 3) * 128 + (((piece & 7) ^ (4 * (r & 1))) << 4);
+}
+template <typename S, bool E2M1>
+__device__ __forceinline__ uint32_t v_place(int r, int piece) {
+  constexpr int kPerLine = S::kRow >= 128 ? 1 : 128 / S::kRow;   // rows per line
+  if constexpr (kPerLine == 1) return r * S::kRow + (piece >> 3) * 128 + (((piece & 7) ^ (r & 6)) << 4);
+  else if constexpr (kPerLine == 2) return (r >> 1) * 128 + ((((r & 1) * 4 + piece) ^ (r & 6)) << 4);
+  else return (r >> 2) * 128 + ((((r & 3) * 2 + piece) ^ (2 * ((r >> 2) & 1))) << 4);
 }
 
 __device__ __forceinline__ void sts8(uint32_t a, uint32_t v) {
@@ -423,8 +437,8 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           const int local = (lane + 32 * j) / kPieces, src = g0 + (local >> 3);
           const uint32_t ka = __shfl_sync(0xffffffffu, k_at, src), va = __shfl_sync(0xffffffffu, v_at, src);
           const bool in = ((ok >> local) & 1u) != 0u && lane_in;
-          copy_async(at + local * S::kKRow + 16 * piece, place(kl, ka), in);
-          copy_async(at + S::kKBytes + local * S::kVRow + 16 * piece, place(vl, va), in);
+          copy_async(at + k_place<S, true>(local, piece), place(kl, ka), in);
+          copy_async(at + S::kKBytes + v_place<S, true>(local, piece), place(vl, va), in);
         }
         // The scales of a group of 8 keys are srow / 2 pieces of 16 bytes. A
         // group with a masked key is copied whole; see clear_scales below.
@@ -438,26 +452,26 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           copy_async(at + S::kKBytes + S::kVBytes + kv * S::kScaleBytes + grp * (8 * srow) + 16 * sp, src + 16 * sp, in);
         }
       } else {
-        // K row 8 i + g: pieces c, c + 4, ...; V rows 8 i + 2 c + e (the lane's
-        // keys of an mma k-step): pieces g, g + 8.
-        const char* kl = kb + (grouped ? g * row_bytes : 0) + 16 * c;
-        const char* vl = vb + (grouped ? 2 * c * row_bytes : 0) + 16 * g;
+        constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
+        const int piece = lane % kPieces, sub = lane / kPieces;
+        const bool lane_in = EXACT || 16 * piece < row_bytes;
 #pragma unroll
         for (int i8 = 0; i8 < KT / 8; ++i8) {
-          const char* src = place(kl, __shfl_sync(0xffffffffu, k_at, grouped ? g0 + i8 : 8 * i8 + g));
-          const bool use = ((ok >> (8 * i8 + g)) & 1u) != 0u;
+          const uint32_t ka = __shfl_sync(0xffffffffu, k_at, (g0 + i8) & 31), va = __shfl_sync(0xffffffffu, v_at, (g0 + i8) & 31);
+          const char* kg = place(kb + sub * row_bytes + 16 * piece, ka);
+          const char* vg = place(vb + sub * row_bytes + 16 * piece, va);
 #pragma unroll
-          for (int j = 0; j < DP / 32; ++j)
-            copy_async(at + ((i8 * (DP / 32) + j) * 32 + lane) * 16, src + 64 * j, use && (EXACT || 16 * (c + 4 * j) < row_bytes));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int local = 8 * i8 + 2 * c + e;
-            const char* vsrc = place(vl, __shfl_sync(0xffffffffu, v_at, grouped ? g0 + i8 : local)) + (grouped ? e * row_bytes : 0);
-            const bool vuse = ((ok >> local) & 1u) != 0u;
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j)
-              copy_async(at + S::kKBytes + (((2 * i8 + e) * (DP / 64) + j) * 32 + lane) * 16, vsrc + 128 * j,
-                         vuse && (EXACT || 16 * (g + 8 * j) < row_bytes));
+          for (int it = 0; it < 8 / kAtOnce; ++it) {
+            const int r = it * kAtOnce + sub, local = 8 * i8 + r;
+            const bool in = ((ok >> local) & 1u) != 0u && lane_in;
+            const char* ksrc = kg + it * kAtOnce * row_bytes;
+            const char* vsrc = vg + it * kAtOnce * row_bytes;
+            if (!grouped) {   // every row by its own page
+              ksrc = place(kb + 16 * piece, __shfl_sync(0xffffffffu, k_at, local));
+              vsrc = place(vb + 16 * piece, __shfl_sync(0xffffffffu, v_at, local));
+            }
+            copy_async(at + k_place<S, false>(local, piece), ksrc, in);
+            copy_async(at + S::kKBytes + v_place<S, false>(local, piece), vsrc, in);
           }
         }
       }
@@ -552,7 +566,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         copy_commit();
       }
       copy_wait<S::kStages - 1>();
-      if constexpr (E2M1) __syncwarp();   // rows copied by other lanes
+      __syncwarp();   // rows copied by other lanes
       const uint32_t ok = ok_of[0];
 #pragma unroll
       for (int k = 0; k + 1 < S::kStages; ++k) ok_of[k] = ok_of[k + 1];
@@ -587,13 +601,13 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
             for (int h = 0; h < 2; ++h) {
               const int key = 16 * a + 8 * h + g;
               if constexpr (DP == 128) {
-                const uint4 u = lds128(at + key * S::kKRow + 16 * c);
+                const uint4 u = lds128(at + k_place<S, true>(key, c));
                 w[h][0] = u.x; w[h][1] = u.y; w[h][2] = u.z; w[h][3] = u.w;
                 const uint32_t s01 = scales_to_half2(EXACT || 2 * c < srow ? lds16(k_scales + key * srow + 2 * c) : 0u);
                 sx[h][0] = __byte_perm(s01, s01, 0x1010);
                 sx[h][1] = __byte_perm(s01, s01, 0x3232);
               } else {
-                const uint2 u = lds64(at + key * S::kKRow + 8 * c);
+                const uint2 u = lds64(at + k_place<S, true>(key, c >> 1) + 8 * (c & 1));
                 w[h][0] = u.x; w[h][1] = u.y;
                 sx[h][0] = sx[h][1] = scales_to_half2((EXACT || c < srow ? lds8(k_scales + key * srow + c) : 0u) * 0x101u);
               }
@@ -621,8 +635,8 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
             for (int a = 0; a < KT / 16; ++a) {
-              const uint4 u = lds128(at + ((2 * a * (DP / 32) + j) * 32 + lane) * 16);
-              const uint4 v = lds128(at + (((2 * a + 1) * (DP / 32) + j) * 32 + lane) * 16);
+              const uint4 u = lds128(at + k_place<S, false>(16 * a + g, c + 4 * j));
+              const uint4 v = lds128(at + k_place<S, false>(16 * a + 8 + g, c + 4 * j));
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<M>(sc[n][a], u.x, v.x, u.y, v.y, qf[n][2 * j][0], qf[n][2 * j][1]);
@@ -711,13 +725,13 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const uint32_t row = at + S::kKBytes + (16 * a + 8 * h + 2 * c + e) * S::kVRow + (DP / 16) * g;
+                const int key = 16 * a + 8 * h + 2 * c + e;
                 if constexpr (DP == 128) {
-                  const uint2 u = lds64(row);
+                  const uint2 u = lds64(at + S::kKBytes + v_place<S, true>(key, g >> 1) + 8 * (g & 1));
                   w[h][e][0] = u.x;
                   w[h][e][1] = u.y;
                 } else {
-                  w[h][e][0] = lds32(row);
+                  w[h][e][0] = lds32(at + S::kKBytes + v_place<S, true>(key, g >> 2) + 4 * (g & 3));
                 }
               }
 #pragma unroll
@@ -747,7 +761,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
               uint32_t w[4][4];   // [key][word]
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const uint4 u = lds128(at + S::kKBytes + (((4 * a + e) * (DP / 64) + j) * 32 + lane) * 16);
+                const uint4 u = lds128(at + S::kKBytes + v_place<S, false>(16 * a + 8 * (e >> 1) + 2 * c + (e & 1), g + 8 * j));
                 w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
               }
 #pragma unroll
@@ -761,7 +775,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           }
         }
       }
-      if constexpr (E2M1) __syncwarp();   // the stage may be written again
+      __syncwarp();   // the stage may be written again
       stage = stage + 1 == S::kStages ? 0 : stage + 1;
     }
     copy_wait<0>();
@@ -931,7 +945,7 @@ int row_tiles_of(const lunarad_paged_attention_args& a) {
   const int64_t mean = (a.seqs.tokens + a.seqs.batch - 1) / a.seqs.batch;
   return (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / a.cache->kv_heads) <= 8 ? 1 : 2;
 }
-int stream_workers(bool e2m1, int nt, int sms) { return sms * kWarps * (e2m1 ? (nt == 1 ? 4 : 3) : 2); }
+int stream_workers(bool e2m1, int nt, int sms) { return sms * kWarps * ((e2m1 ? 3 : 2) + (nt == 1 ? 1 : 0)); }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
