@@ -252,58 +252,34 @@ __device__ __forceinline__ void seq_tiles(const PagedParams& p, const SeqInfo& s
 }
 
 // prefix[b] = tiles of the sequences before b (batch + 1 entries in shared
-// memory), by the whole block. SEGMENTS: segments[b] = their (key head, row
-// tile) pairs that have tiles, likewise.
-template <bool SEGMENTS>
-__device__ __forceinline__ void prefix_tiles(const PagedParams& p, Tiling tl, int64_t* prefix, int64_t* warp_sums,
-                                             int* segments = nullptr, int* warp_segments = nullptr) {
+// memory), by the whole block.
+__device__ __forceinline__ void prefix_tiles(const PagedParams& p, Tiling tl, int64_t* prefix, int64_t* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int64_t carry = 0;
-  int carry_segments = 0;
   for (int b0 = 0; b0 < p.seqs.batch; b0 += blockDim.x) {
     const int b = b0 + static_cast<int>(threadIdx.x);
     int64_t inc = 0;
-    int inc_segments = 0;
     if (b < p.seqs.batch) {
       int rt, nt;
       seq_tiles(p, load_seq(p, b), tl, rt, nt);
-      inc_segments = p.kv_heads * rt;
-      inc = static_cast<int64_t>(inc_segments) * nt;
+      inc = static_cast<int64_t>(p.kv_heads) * rt * nt;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
-      if constexpr (SEGMENTS) {
-        const int z = __shfl_up_sync(0xffffffffu, inc_segments, o);
-        if (lane >= o) inc_segments += z;
-      }
     }
-    if (lane == 31) {
-      warp_sums[warp] = inc;
-      if constexpr (SEGMENTS) warp_segments[warp] = inc_segments;
-    }
+    if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
     int64_t before = carry;
-    int before_segments = carry_segments;
     for (int w = 0; w < warps; ++w) {
       if (w < warp) before += warp_sums[w];
       carry += warp_sums[w];
-      if constexpr (SEGMENTS) {
-        if (w < warp) before_segments += warp_segments[w];
-        carry_segments += warp_segments[w];
-      }
     }
-    if (b < p.seqs.batch) {
-      prefix[b + 1] = before + inc;
-      if constexpr (SEGMENTS) segments[b + 1] = before_segments + inc_segments;
-    }
+    if (b < p.seqs.batch) prefix[b + 1] = before + inc;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    prefix[0] = 0;
-    if constexpr (SEGMENTS) segments[0] = 0;
-  }
+  if (threadIdx.x == 0) prefix[0] = 0;
   __syncthreads();
 }
 
@@ -335,10 +311,14 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
   const uint32_t ring = smem_u32(smem) + warp * S::kRingBytes;
   pdl_wait();
   pdl_launch_dependents();
-  prefix_tiles<false>(p, kTiling, prefix, warp_sums);
+  prefix_tiles(p, kTiling, prefix, warp_sums);
   const int64_t total = prefix[p.seqs.batch];
   const int workers = used_workers(p, total), worker = static_cast<int>(blockIdx.x) * kWarps + warp;
-  if (worker >= workers) return;
+  clear_empty<T>(p);
+  if (worker >= workers) {
+    if (lane == 0) p.cuts[worker].parts = 0;
+    return;
+  }
   const int64_t t_first = run_start(total, workers, worker), t_end = run_start(total, workers, worker + 1);
   const bool grouped = E2M1 || (p.page_size & 7) == 0;   // 8 neighbouring keys stand in one page
   constexpr int kElem = E2M1 ? 1 : 2;
@@ -823,107 +803,17 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         }
       }
     t += n_tiles;
-  }
-}
-
-// Joins the parts of the segments (key head, row tile) that several workers
-// took, and clears the rows of sequences without keys. A block per segment (and
-// more, where there are more than blocks); blockIdx.y takes every kJoinShares-th
-// row, its warps every fourth part. The lengths are read before the streaming
-// kernel has ended (it has started, so whatever came before it is complete),
-// the parts after it.
-constexpr int kJoinThreads = 128, kJoinShares = 4;
-
-template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, Tiling tl) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t warp_sums[kJoinThreads / 32];
-  __shared__ int warp_segments[kJoinThreads / 32];
-  __shared__ float s_o[kJoinThreads / 32][DP];
-  __shared__ float2 s_ml[kJoinThreads / 32];
-  int64_t* prefix = reinterpret_cast<int64_t*>(smem);
-  int* segments = reinterpret_cast<int*>(prefix + p.seqs.batch + 1);
-  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
-  constexpr int kWarpsHere = kJoinThreads / 32, kE = DP / 32;
-  prefix_tiles<true>(p, tl, prefix, warp_sums, segments, warp_segments);
-  const int64_t total = prefix[p.seqs.batch];
-  const int workers = used_workers(p, total);
-  pdl_wait();
-  pdl_launch_dependents();
-  if (blockIdx.y == 0) {
-    for (int b = blockIdx.x; b < p.seqs.batch; b += gridDim.x) {
-      const SeqInfo z = load_seq(p, b);
-      const int64_t rows = static_cast<int64_t>(z.n) * p.group;
-      if (rows < p.min_rows || rows >= p.max_rows || z.hi > z.lo) continue;
-      const int width = p.q_heads * p.dim;
-      for (int token = z.first; token < z.first + z.n; ++token)
-        for (int e = threadIdx.x; e < width; e += kJoinThreads)
-          static_cast<T*>(p.o)[token * p.o_tok + e / p.dim * p.o_head + e % p.dim] = Io<T>::from_f(0.f);
-    }
-  }
-  for (int x = blockIdx.x; x < segments[p.seqs.batch]; x += gridDim.x) {
-    int b = 0;
-    for (int end = p.seqs.batch; b + 1 < end;) {   // last b with segments[b] <= x
-      const int mid = (b + end) >> 1;
-      if (segments[mid] <= x) b = mid; else end = mid;
-    }
-    const SeqInfo s = load_seq(p, b);
-    int row_tiles, seg_tiles;
-    seq_tiles(p, s, tl, row_tiles, seg_tiles);
-    const int seg = x - segments[b], kh = seg / row_tiles, rt = seg - kh * row_tiles;
-    const int64_t start = prefix[b] + static_cast<int64_t>(seg) * seg_tiles;
-    const int w0 = run_of(total, workers, start), last = run_of(total, workers, start + seg_tiles - 1);
-    if (w0 == last) continue;   // its worker has written it
-    const int first_slot = run_start(total, workers, w0) == start ? 0 : 1;
-    const int rows = min(tl.rows, s.n * p.group - rt * tl.rows);
-    for (int r = static_cast<int>(blockIdx.y); r < rows; r += kJoinShares) {
-      float m = -INFINITY, l = 0.f, o[kE];
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] = 0.f;
-#pragma unroll 4
-      for (int w = w0 + warp; w <= last; w += kWarpsHere) {
-        const int64_t at = (static_cast<int64_t>(w) * 2 + (w == w0 ? first_slot : 0)) * tl.rows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-        float x[kE];
-        if constexpr (kE == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
-          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
-          x[0] = v.x; x[1] = v.y;
-        }
-        const float next = fmax_nan(m, ml.x);
-        const float base = next == -INFINITY ? 0.f : next;
-        const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
-        l = l * fa + ml.y * fb;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + x[e] * fb;
-        m = next;
+    if (t >= t_end && lane == 0) {
+      Cut cut{};
+      if (tile0 == 0 && n_tiles < seg_tiles) {
+        cut.parts = run_of(total, workers, t - n_tiles + seg_tiles - 1) - worker + 1;
+        cut.slot = t - n_tiles == t_first ? 0 : 1;
+        cut.rows = rows;
+        cut.first_token = s.first;
+        cut.row0 = row0;
+        cut.kv_head = kh;
       }
-      __syncthreads();   // the row before has been read
-#pragma unroll
-      for (int e = 0; e < kE; ++e) s_o[warp][kE * lane + e] = o[e];
-      if (lane == 0) s_ml[warp] = make_float2(m, l);
-      __syncthreads();
-      float top = s_ml[0].x;
-#pragma unroll
-      for (int w = 1; w < kWarpsHere; ++w) top = fmax_nan(top, s_ml[w].x);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, f[kWarpsHere];
-#pragma unroll
-      for (int w = 0; w < kWarpsHere; ++w) {
-        f[w] = ex2_approx(s_ml[w].x - base);
-        sum += s_ml[w].y * f[w];
-      }
-      const float inv = sum == 0.f ? 0.f : p.v_gain / sum;
-      const int row = rt * tl.rows + r, i = row / p.group;
-      T* out = static_cast<T*>(p.o) + (s.first + i) * p.o_tok + (kh * p.group + row - i * p.group) * p.o_head;
-      for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
-        float x = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarpsHere; ++w) x += s_o[w][d] * f[w];
-        out[d] = Io<T>::from_f(sum == 0.f ? 0.f : x * inv);
-      }
+      p.cuts[worker] = cut;
     }
   }
 }
@@ -998,14 +888,7 @@ bool prefill_ok(const lunarad_paged_attention_args& a) {
 int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {
   const int nt = row_tiles_of(a);
   const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, nt, sms) * 8 * nt;
-  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float));
-}
-
-// No more segments than this, and few enough blocks to run at once.
-unsigned join_blocks(const PagedParams& p, int rows) {
-  const int64_t most = p.kv_heads * (p.seqs.batch + static_cast<int64_t>(p.seqs.tokens) * p.group / rows);
-  const int64_t cap = int64_t{device_num_sms()} * 4;
-  return static_cast<unsigned>(most < cap ? most : cap);
+  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float)) + rows / (16 * nt) * static_cast<int64_t>(sizeof(Cut));
 }
 
 template <typename T, bool E2M1, int DP, int NT, bool EXACT>
@@ -1027,8 +910,7 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
     p.seqs.lens = all.lens + b0;
     e = launch_pdl(kern, dim3(p.workers / kWarps), dim3(kStreamThreads), smem, s, p);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(paged_join_kernel<T, DP>, dim3(join_blocks(p, S::kRows), kJoinShares), dim3(kJoinThreads),
-                   prefix + 4 * static_cast<size_t>(p.seqs.batch + 1), s, p, Tiling{S::KT, S::kRows});
+    e = launch_pdl(paged_join_kernel<T, DP>, dim3(join_blocks(p.workers), 4), dim3(kJoinThreads), 0, s, p, int{S::kRows});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -1106,6 +988,7 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
     p.workers = stream_workers(e2m1, p.nt, device_num_sms());
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + int64_t{2} * p.workers * 8 * p.nt * padded_dim(c.dim);
+    p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * 8 * p.nt * 2);
   }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;

@@ -156,7 +156,11 @@ __device__ __forceinline__ void prefix_blocks(const PagedParams& p, int64_t* pre
   __syncthreads();
 }
 
+// Worker w takes the blocks [run_start(w), run_start(w + 1)); run_of(t) takes block t.
 __device__ __forceinline__ int64_t run_start(int64_t total, int workers, int w) { return total * w / workers; }
+__device__ __forceinline__ int run_of(int64_t total, int workers, int64_t t) {
+  return static_cast<int>(((t + 1) * workers + total - 1) / total) - 1;
+}
 
 // An item, or the part of it that a run holds.
 struct Item {
@@ -293,7 +297,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
   const int workers = static_cast<int>(min(total, static_cast<int64_t>(p.workers)));
   const int worker = static_cast<int>(blockIdx.x);
   int64_t t_first = 0, t_end = 0;
-  if (worker < workers) {
+  clear_empty<T>(p);
+  if (worker >= workers) {
+    if (threadIdx.x == 0) p.cuts[worker].parts = 0;
+  } else {
     t_first = run_start(total, workers, worker);
     t_end = run_start(total, workers, worker + 1);
     if (threadIdx.x == 0) s_cursor.seek(p, prefix, t_first);
@@ -656,6 +663,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
       if (real && !whole) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
       tc_fence_before();
       mbar_arrive(&o_free[w]);
+      if (t + n >= t_end && threadIdx.x == 0) {
+        Cut cut{};
+        if (x.first == 0 && !whole) {
+          cut.parts = run_of(total, workers, t + x.item_blocks - 1) - worker + 1;
+          cut.slot = t == t_first ? 0 : 1;
+          cut.rows = static_cast<int>(min(rows - static_cast<int64_t>(x.rt) * kItemRows, static_cast<int64_t>(kItemRows)));
+          cut.first_token = x.s.first;
+          cut.row0 = x.rt * kItemRows;
+          cut.kv_head = x.kh;
+        }
+        p.cuts[worker] = cut;
+      }
       t += n;
       if (t < t_end) cur.next(p);
     }
@@ -667,85 +686,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
-  }
-}
-
-// Joins the items that runs cut: block w (of `workers`) takes the item that
-// run w begins inside, if no earlier run begins inside it too; blockIdx.y takes
-// a share of its rows. Rows of sequences without keys are cleared here.
-constexpr int kJoinThreads = 256, kJoinShares = 8;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_prefill_join_kernel(const __grid_constant__ PagedParams p) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t warp_sums[kJoinThreads / 32];
-  __shared__ Cursor s_cursor;
-  int64_t* prefix = reinterpret_cast<int64_t*>(smem);
-  prefix_blocks(p, prefix, warp_sums);
-  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
-  const int64_t total = prefix[p.seqs.batch];
-  const int workers = static_cast<int>(min(total, static_cast<int64_t>(p.workers)));
-  const int w1 = static_cast<int>(blockIdx.x);
-  bool mine = w1 > 0 && w1 < workers;
-  int64_t start = 0;
-  if (mine) {
-    const int64_t t = run_start(total, workers, w1);
-    if (threadIdx.x == 0) s_cursor.seek(p, prefix, t);
-    __syncthreads();
-    start = t - s_cursor.x.first;
-    mine = s_cursor.x.first > 0 && run_start(total, workers, w1 - 1) <= start;
-  }
-  pdl_wait();
-  pdl_launch_dependents();
-  if (blockIdx.y == 0) {
-    for (int b = w1; b < p.seqs.batch; b += gridDim.x) {
-      const SeqInfo s = load_seq(p, b);
-      const int64_t rows = static_cast<int64_t>(s.n) * p.group;
-      if (rows < p.min_rows || rows >= p.max_rows || s.hi > s.lo) continue;
-      for (int64_t e = threadIdx.x; e < static_cast<int64_t>(s.n) * p.q_heads * D; e += kJoinThreads) {
-        const int64_t token = e / (p.q_heads * D);
-        const int in_token = static_cast<int>(e - token * (p.q_heads * D));
-        static_cast<T*>(p.o)[(s.first + token) * p.o_tok + in_token / D * p.o_head + in_token % D] = Io<T>::from_f(0.f);
-      }
-    }
-  }
-  if (!mine) return;
-  const Item& x = s_cursor.x;
-  const int64_t end = start + x.item_blocks;
-  const int64_t rows = static_cast<int64_t>(x.s.n) * p.group;
-  constexpr int kE = D / 32;
-  for (int r = static_cast<int>(blockIdx.y) * (kItemRows / kJoinShares) + warp; r < (static_cast<int>(blockIdx.y) + 1) * (kItemRows / kJoinShares);
-       r += kJoinThreads / 32) {
-    const int64_t row = static_cast<int64_t>(x.rt) * kItemRows + r;
-    if (row >= rows) break;
-    float m = -INFINITY, l = 0.f, o[kE];
-#pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = 0.f;
-    for (int w = w1 - 1; w < workers && run_start(total, workers, w) < end; ++w) {
-      const int slot = w == w1 - 1 && run_start(total, workers, w) < start ? 1 : 0;
-      const int64_t at = (static_cast<int64_t>(w) * 2 + slot) * kItemRows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      float v[kE];
-      if constexpr (kE == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(p.part_o + at * D + 4 * lane);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane);
-        v[0] = u.x; v[1] = u.y;
-      }
-      const float next = fmax_nan(m, ml.x);
-      const float base = next == -INFINITY ? 0.f : next;
-      const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
-      l = l * fa + ml.y * fb;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] = o[e] * fa + v[e] * fb;
-      m = next;
-    }
-    const int64_t i = row / p.group;
-    T* out = static_cast<T*>(p.o) + (x.s.first + i) * p.o_tok + (x.kh * p.group + (row - i * p.group)) * p.o_head + kE * lane;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) out[e] = Io<T>::from_f(l == 0.f ? 0.f : o[e] * inv);
   }
 }
 
@@ -769,8 +709,7 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
     p.seqs.lens = all.lens + b0;
     e = launch_pdl(kern, dim3(p.workers), dim3(kThreads), static_cast<size_t>(L::kSmem), s, p);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(paged_prefill_join_kernel<T, D>, dim3(p.workers, kJoinShares), dim3(kJoinThreads),
-                   sizeof(int64_t) * static_cast<size_t>(p.seqs.batch + 1), s, p);
+    e = launch_pdl(paged_join_kernel<T, D>, dim3(join_blocks(p.workers), 16), dim3(kJoinThreads), 0, s, p, int{kItemRows});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -779,13 +718,14 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
 }  // namespace
 
 int64_t paged_prefill_workspace(int dim, int sms) {
-  return int64_t{2} * sms * kItemRows * (dim + 2) * static_cast<int64_t>(sizeof(float));
+  return int64_t{2} * sms * kItemRows * (dim + 2) * static_cast<int64_t>(sizeof(float)) + sms * static_cast<int64_t>(sizeof(Cut));
 }
 
 cudaError_t launch_paged_prefill(PagedParams p, int dtype, void* workspace, cudaStream_t stream) {
   p.workers = device_num_sms();
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + int64_t{2} * p.workers * kItemRows * p.dim;
+  p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * kItemRows * 2);
   if (dtype == LUNARA_BF16)
     return p.dim == 64 ? run_prefill<__nv_bfloat16, 64>(p, stream) : run_prefill<__nv_bfloat16, 128>(p, stream);
   return p.dim == 64 ? run_prefill<__half, 64>(p, stream) : run_prefill<__half, 128>(p, stream);
