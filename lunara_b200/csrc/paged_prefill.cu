@@ -13,16 +13,23 @@
 //     partial O, maximum and sum in the workspace, and a second kernel joins
 //     them.
 //   * warps 0-3, 4-7   softmax of tile 0 and 1 (thread = row)
-//     warps 8, 9       tcgen05.mma issuers of tile 0 and 1
+//     warp 8           tcgen05.mma issuer
 //                        S_w = Q_w K^T  (128 x 128 x D, operands in shared memory)
 //                        O_w += P_w V   (128 x D x 128, P_w from TMEM)
-//     warps 12-15      copy Q, K and V with cp.async, any page size, into
-//                        128-byte-swizzled tiles; rows that no query of the item
-//                        sees, and rows of bad pages, become zeros there
+//                        in the order P_0 V, next S_0, P_1 V, next S_1: one tile's
+//                        products run whole while the other's softmax has the
+//                        issue slots (an issuer per tile interleaved them: 4030
+//                        instead of 3200 cycles a block)
+//     warps 10, 11     copy K and V (and Q between them) into 128-byte-swizzled
+//                        tiles: a block whose keys all take part by TMA, a box
+//                        per page; one at the ends of what the item sees, with
+//                        bad pages, or of pages that do not tile a block, row by
+//                        row with cp.async, with zeros for the keys left out
 //   * TMEM: S_w 128 columns each, O_w D columns each; P_w (16-bit pairs) takes
 //     the first half of S_w's columns once the row is in registers. The next
-//     S_w is issued when P_w V has completed; meanwhile the other tile's
-//     products run.
+//     S_w is issued right behind P_w V; meanwhile the other tile's products run.
+#include <cudaTypedefs.h>
+
 #include <type_traits>
 
 #include "kernels.h"
@@ -34,15 +41,17 @@ namespace {
 constexpr int kItemRows = 256;
 constexpr int kTileRows = 128;
 constexpr int kBlock = 128;              // keys per block
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
+constexpr int kCopyWarps = 2;
 constexpr int kMaxBatch = 1024;          // sequences per launch
 constexpr float kRescaleLog2 = 8.0f;
-// setmaxnreg split of the launch's 512 x 128 registers.
-constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 200, kIssueRegs = 40, kCopyRegs = 72;
-static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs + 128 * kCopyRegs <= kThreads * kLaunchRegs, "register split");
+// setmaxnreg split of the launch's 384 x 168 registers.
+constexpr int kLaunchRegs = 168;
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
 constexpr int kPolyPairs = 4;            // of 16 exponential pairs on the FMA pipe, as in attention.cu
 constexpr int kMaskRing = 16;            // blocks whose key masks are kept; more than the ring can run ahead
+constexpr int kItemRing = 4;             // items whose block counts are kept; the copies run one item ahead at most
 
 template <int D>
 struct Layout {
@@ -51,7 +60,6 @@ struct Layout {
   static constexpr uint32_t kSlotBytes = kHalves * kHalfBytes; // one K or V block
   static constexpr uint32_t kQBytes = 2 * kSlotBytes;          // two row tiles
   static constexpr int kSlots = D == 128 ? 5 : 8;              // ring of K and V blocks: K0, V0, K1, V1, ...
-  static constexpr int kLag = 2;                               // slots whose copies stay in flight
   static constexpr uint32_t kSmem = kQBytes + kSlots * kSlotBytes + kMaskRing * 16 + 512 + 1024;
   static constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemCols = 512;
 };
@@ -235,7 +243,9 @@ __device__ __forceinline__ void item_keys(const PagedParams& p, const Item& x, i
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap tk,
+                         const __grid_constant__ CUtensorMap tv, int box_rows) {
   using L = Layout<D>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t IDESC_S = idesc_f16(128, kBlock, kBF16, false, false);
@@ -248,16 +258,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
   uint32_t* s_mask = reinterpret_cast<uint32_t*>(sRing + L::kSlots * L::kSlotBytes);   // [kMaskRing][4]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_mask + kMaskRing * 4);
   uint64_t* q_full = bars;
-  uint64_t* q_free = q_full + 1;            // both issuers done with Q
+  uint64_t* q_free = q_full + 1;            // the item's last S is done
   uint64_t* full = q_free + 1;              // [kSlots]
-  uint64_t* empty = full + L::kSlots;       // [kSlots] both issuers done with the slot
+  uint64_t* empty = full + L::kSlots;       // [kSlots] the products are done with the slot
   uint64_t* s_full = empty + L::kSlots;     // [2]
   uint64_t* p_ready = s_full + 2;           // [2]
   uint64_t* o_full = p_ready + 2;           // [2]
   uint64_t* o_free = o_full + 2;            // [2] the item's O_w is read
-  uint64_t* drain_bar = o_free + 2;         // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
+  uint64_t* drain_bar = o_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_blocks = reinterpret_cast<int*>(tmem_slot + 2);   // [kItemRing] blocks of an item's part
   // The prefix sums stand in the ring until the roles begin.
   int64_t* prefix = reinterpret_cast<int64_t*>(sRing);
   __shared__ int64_t warp_sums[kThreads / 32];
@@ -266,19 +277,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 128);
-    mbar_init(q_free, 2);
+    mbar_init(q_full, kCopyWarps);
+    mbar_init(q_free, 1);
     for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(&full[i], 128);
-      mbar_init(&empty[i], 2);
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&s_full[w], 1);
       mbar_init(&p_ready[w], kTileRows);
       mbar_init(&o_full[w], 1);
       mbar_init(&o_free[w], kTileRows);
-      mbar_init(&drain_bar[w], 1);
     }
+    mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -307,175 +318,209 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
   }
   __syncthreads();   // the prefix sums are used up: the ring may be written
 
-  if (warp >= 12) {
-    reg_dealloc<kCopyRegs>();
+  if (warp >= 10) {
+    reg_dealloc<kOtherRegs>();
     // -------------------------------------------------------------- copies --
-    // A warp copies 32 rows of every block; lane l looks up the place of row
-    // 32 warp + l, and D / 8 neighbouring lanes copy one row.
-    const int cw = warp - 12;
-    constexpr int kPer = D / 8, kRowsAtOnce = 32 / kPer;
+    // Warp 10 fills the ring's K slots, warp 11 its V slots.
+    const int kv = warp - 10;
+    constexpr int kPer = D / 8, kRowsAtOnce = 32 / kPer;   // lanes to a row, rows at once
     const int chunk = lane % kPer, sub = lane / kPer;
-    const uint32_t ring = smem_u32(sRing);
-    int slot = 0;
-    uint32_t phase = 0;        // of empty[slot]
-    int issued = 0, arrived = 0;   // slots
-    auto arrive_oldest = [&] {     // its copies have landed
-      fence_proxy_async_smem();
-      mbar_arrive(&full[arrived % L::kSlots]);
-      ++arrived;
-    };
+    const uint32_t lane_dst = (chunk >> 3) * L::kHalfBytes;
+    const int boxes = box_rows > 0 ? kBlock / box_rows : 0;
+    const CUtensorMap* map = kv == 0 ? &tk : &tv;
+    if (lane == 0) tma_prefetch_desc(map);
+    const uint32_t page_u = kv == 0 ? p.k_page_u : p.v_page_u;
     bool ok = true;
     Cursor cur = s_cursor;
-    int block_count = 0;
-    uint32_t items = 0;
+    int slot = kv;             // ring slot of this warp's next block, and the phase of its empty barrier
+    uint32_t phase = 0, block_count = 0, items = 0;
+    uint32_t filled = 0, filled_phase = 0;   // bits of the slots that TMA was started on, and of their phases
     for (int64_t t = t_first; ok && t < t_end; ++items) {
       cur.clip(t_end - t);
       const Item& x = cur.x;
       int lo, hi;
       item_keys(p, x, lo, hi);
-      // Q: row r of the item is token r / group, head r % group of the pair.
+      // Q: row r of the item is token r / group, head r % group; a warp copies a tile.
       if (!mbar_wait_warp(q_free, (items & 1u) ^ 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
       {
-        const int64_t rows = static_cast<int64_t>(x.s.n) * p.group - static_cast<int64_t>(x.rt) * kItemRows;
-        for (int it = 0; it < kItemRows / 4 / kRowsAtOnce; ++it) {
-          const int r = (kItemRows / 4) * cw + it * kRowsAtOnce + sub;
-          const bool in = r < rows;
-          const int64_t row = static_cast<int64_t>(x.rt) * kItemRows + (in ? r : 0);
-          const int i = static_cast<int>(row / p.group);
-          const int head = x.kh * p.group + static_cast<int>(row - static_cast<int64_t>(i) * p.group);
-          const T* src = static_cast<const T*>(p.q) + (x.s.first + i) * p.q_tok + head * p.q_head + 8 * chunk;
-          copy16(smem_u32(sQ) + (r >> 7) * L::kSlotBytes + (chunk >> 3) * L::kHalfBytes + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
-                 src, in);
+        // Lane l finds the places of rows 32 h + l (32-bit: tokens * heads is below 2^31).
+        const int row0 = x.rt * kItemRows + kTileRows * kv, rows = x.s.n * p.group;
+        const uint32_t dst = smem_u32(sQ) + kv * L::kSlotBytes + lane_dst;
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          const int row = row0 + 32 * h + lane;
+          const uint32_t use = __ballot_sync(0xffffffffu, row < rows);
+          const int i = (row < rows ? row : 0) / p.group, head = x.kh * p.group + (row < rows ? row : 0) - i * p.group;
+          const char* src = static_cast<const char*>(p.q) + ((x.s.first + i) * p.q_tok + head * p.q_head) * 2;
+          const uint32_t src_lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src)), src_hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src) >> 32);
+#pragma unroll 4
+          for (int it = 0; it < 32 / kRowsAtOnce; ++it) {
+            const int r = it * kRowsAtOnce + sub;
+            const uint64_t at = (static_cast<uint64_t>(__shfl_sync(0xffffffffu, src_hi, r)) << 32) | __shfl_sync(0xffffffffu, src_lo, r);
+            copy16(dst + (32 * h + r) * 128 + (((chunk & 7) ^ (r & 7)) << 4), reinterpret_cast<const char*>(at) + 16 * chunk, ((use >> r) & 1u) != 0u);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      while (arrived < issued) arrive_oldest();
       fence_proxy_async_smem();
-      mbar_arrive(q_full);
+      __syncwarp();
+      if (lane == 0) {
+        if (kv == 0) s_blocks[items % kItemRing] = x.n;
+        mbar_arrive(q_full);
+      }
       const int32_t* table = p.seqs.page_table + x.b * p.seqs.table_stride;
-      const char* bases[2] = {static_cast<const char*>(p.k) + x.kh * p.k_head * 2, static_cast<const char*>(p.v) + x.kh * p.v_head * 2};
-      const int row_bytes = D * 2;
-      auto find = [&](int block, int& row_slot) {   // page of this lane's row, or -1
-        const int key = block * kBlock + 32 * cw + lane;
-        if (key < lo || key >= hi) return -1;
-        const int pi = p.seqs.page_div.div(key);
-        row_slot = key - pi * p.page_size;
-        const int page = table[pi];
+      auto page_of = [&](int key) {   // -1: no page, or one outside the cache
+        const int page = table[p.seqs.page_div.div(key)];
         if (page >= 0 && page < p.num_pages) return page;
         atomicCAS(p.err, 0u, static_cast<unsigned>(kErrCachePage));
         return -1;
       };
-      int next_slot = 0, next_page = find(x.block0, next_slot);
-      for (int j = 0; j < x.n && ok; ++j, ++block_count) {
-        const int page = next_page, row_slot = next_slot;
-        if (j + 1 < x.n) next_page = find(x.block0 + j + 1, next_slot);
-        const uint32_t use = __ballot_sync(0xffffffffu, page >= 0);
-        if (lane == 0) s_mask[(block_count % kMaskRing) * 4 + cw] = use;
+      // The lane's box of a block, looked up a block ahead.
+      auto box_page = [&](int block) {
+        const int key = block * kBlock + lane * box_rows;
+        return lane < boxes && block * kBlock >= lo && block * kBlock + kBlock <= hi ? page_of(key) : -1;
+      };
+      int next = box_page(x.block0);
+      for (int j = 0; j < x.n; ++j, ++block_count) {
+        const int key0 = (x.block0 + j) * kBlock, page = next;
+        if (j + 1 < x.n) next = box_page(x.block0 + j + 1);
+        if (!mbar_wait_warp(&empty[slot], phase ^ 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
+        uint8_t* tile = sRing + slot * L::kSlotBytes;
+        const bool whole = boxes > 0 && __popc(__ballot_sync(0xffffffffu, page >= 0)) == boxes;
+        if (whole) {
+          if (lane == 0) {
+            if (kv == 0) *reinterpret_cast<uint4*>(&s_mask[(block_count % kMaskRing) * 4]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+            mbar_arrive_expect_tx(&full[slot], L::kSlotBytes);
+          }
+          __syncwarp();
+          if (lane < boxes) {
+            const int key = key0 + lane * box_rows, in_page = key - p.seqs.page_div.div(key) * p.page_size;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!mbar_wait_warp(&empty[slot], phase ^ 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
-          const int64_t stride = (kv == 0 ? p.k_page : p.v_page) * 2;
-          const uint32_t dst = ring + slot * L::kSlotBytes + (chunk >> 3) * L::kHalfBytes;
+            for (int h = 0; h < L::kHalves; ++h)
+              tma_load_4d(tile + h * L::kHalfBytes + lane * box_rows * 128, map, &full[slot], 64 * h, in_page, x.kh, page);
+          }
+          filled |= 1u << slot;
+          filled_phase = (filled_phase & ~(1u << slot)) | (phase << slot);
+        } else {
+          const char* base = static_cast<const char*>(kv == 0 ? p.k : p.v) + x.kh * (kv == 0 ? p.k_head : p.v_head) * 2 + 16 * chunk;
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            const int key = key0 + 32 * h + lane;
+            const int pg = key >= lo && key < hi ? page_of(key) : -1;
+            const uint32_t use = __ballot_sync(0xffffffffu, pg >= 0);
+            if (kv == 0 && lane == 0) s_mask[(block_count % kMaskRing) * 4 + h] = use;
+            // Where the lane's row stands, in units of p.unit bytes.
+            const uint32_t in_page = static_cast<uint32_t>(key - p.seqs.page_div.div(key) * p.page_size) * p.row_u;
+            const uint32_t at = pg >= 0 ? static_cast<uint32_t>(pg) * page_u + in_page : 0u;
+            const uint32_t dst = smem_u32(tile) + lane_dst + 32 * h * 128;
 #pragma unroll 4
-          for (int it = 0; it < 32 / kRowsAtOnce; ++it) {
-            const int r = it * kRowsAtOnce + sub;
-            const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, row_slot, r);
-            const int row = 32 * cw + r;
-            const bool in = pg >= 0;
-            copy16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
-                   in ? bases[kv] + pg * stride + static_cast<int64_t>(sl) * row_bytes + 16 * chunk : bases[kv], in);
+            for (int it = 0; it < 32 / kRowsAtOnce; ++it) {
+              const int r = it * kRowsAtOnce + sub;
+              const uint32_t row_at = __shfl_sync(0xffffffffu, at, r);
+              copy16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + static_cast<uint64_t>(row_at) * p.unit, ((use >> r) & 1u) != 0u);
+            }
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
-          ++issued;
-          if (issued - arrived > L::kLag) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(L::kLag) : "memory");
-            arrive_oldest();
-          }
-          if (++slot == L::kSlots) { slot = 0; phase ^= 1u; }
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[slot]);
         }
+        slot += 2;
+        if (slot >= L::kSlots) { slot -= L::kSlots; phase ^= 1u; }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      while (arrived < issued) arrive_oldest();
       t += x.n;
-      if (t < t_end) cur.next(p);
+      if (ok && t < t_end) cur.next(p);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else if (warp == 8 || warp == 9) {
-    reg_dealloc<kIssueRegs>();
-    // ---------------------------------------------------------- MMA issuers --
-    const int w = warp - 8;
+    if (!ok)   // the copies in flight are waited for
+      for (int i = 0; i < L::kSlots; ++i)
+        if ((filled >> i) & 1u) mbar_drain_wait(&full[i], (filled_phase >> i) & 1u, 200000000ull);
+  } else if (warp >= 8) {
+    reg_dealloc<kOtherRegs>();
+    // ----------------------------------------------------------- MMA issuer --
     const bool leader = elect_one_sync();
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return mbar_wait_warp(bar, parity, abort_flag, p.err, kErrPagedWait);
     };
-    const uint64_t qd = sw128_desc(smem_u32(sQ) + w * L::kSlotBytes, 16, 1024);
+    const uint64_t qd0 = sw128_desc(smem_u32(sQ), 16, 1024);
     const uint64_t kd0 = sw128_desc(smem_u32(sRing), 16, 1024);
     const uint64_t vd0 = sw128_desc(smem_u32(sRing), L::kHalfBytes, 1024);
-    const uint32_t d_s = tmem_base + L::kTmemS + w * 128;
-    const uint32_t d_o = tmem_base + L::kTmemO + w * D;
-    auto issue_s = [&](int slot) {
-      const uint64_t kd = kd0 + static_cast<uint64_t>(slot) * (L::kSlotBytes >> 4);
+    auto issue_s = [&](int w, int slot) {
+      const uint64_t qd = qd0 + w * (L::kSlotBytes >> 4), kd = kd0 + static_cast<uint64_t>(slot) * (L::kSlotBytes >> 4);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint64_t off = (kk >> 2) * (L::kHalfBytes >> 4) + 2 * (kk & 3);
-        umma_f16_ss(d_s, qd + off, kd + off, IDESC_S, kk > 0 ? 1u : 0u);
+        umma_f16_ss(tmem_base + L::kTmemS + w * 128, qd + off, kd + off, IDESC_S, kk > 0 ? 1u : 0u);
       }
     };
-    auto issue_pv = [&](int slot, bool first) {
+    auto issue_pv = [&](int w, int slot, bool first) {
       const uint64_t vd = vd0 + static_cast<uint64_t>(slot) * (L::kSlotBytes >> 4);
 #pragma unroll
       for (int kk = 0; kk < kBlock / 16; ++kk)
-        umma_f16_ts(d_o, d_s + kk * 8, vd + 128 * kk, IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+        umma_f16_ts(tmem_base + L::kTmemO + w * D, tmem_base + L::kTmemS + w * 128 + kk * 8, vd + 128 * kk, IDESC_PV,
+                    (!first || kk > 0) ? 1u : 0u);
     };
-    bool ok = true;
-    Cursor cur = s_cursor;
+    bool ok = warp == 8;              // (the warpgroup's other warp idles)
     uint32_t items = 0, blocks = 0;   // items and blocks so far
-    uint32_t used = 0;                // ring slots so far
-    for (int64_t t = t_first; ok && t < t_end; ++items) {
-      cur.clip(t_end - t);
-      const int n = cur.x.n;
+    int ks = 0;                       // ring slot of the next K, and its phase
+    uint32_t kp = 0;
+    for (int left = __shfl_sync(0xffffffffu, static_cast<int>(t_end - t_first), 0); ok && left > 0; ++items) {
       if (!wait(q_full, items & 1u)) { ok = false; break; }
-      for (int j = 0; j < n && ok; ++j, ++blocks) {
-        const int ks = static_cast<int>(used % L::kSlots), vs = static_cast<int>((used + 1) % L::kSlots);
-        const uint32_t kp = (used / L::kSlots) & 1u, vp = ((used + 1) / L::kSlots) & 1u;
-        // S of block j: K is there, and P V of the block before has read P
-        // (which shares S's columns).
-        if (!wait(&full[ks], kp)) { ok = false; break; }
-        if (j > 0 && !wait(&o_full[w], (blocks - 1) & 1u)) { ok = false; break; }
-        tc_fence_after();
-        if (leader) {
-          issue_s(ks);
-          umma_commit(&s_full[w]);
-          umma_commit(&empty[ks]);
-          if (j + 1 == n) umma_commit(q_free);
-        }
-        __syncwarp();
-        if (!wait(&full[vs], vp)) { ok = false; break; }
-        if (!wait(&p_ready[w], blocks & 1u)) { ok = false; break; }
-        // The item's first P V overwrites O: the item before must have been read.
-        if (j == 0 && items > 0 && !wait(&o_free[w], (items - 1) & 1u)) { ok = false; break; }
-        tc_fence_after();
-        if (leader) {
-          issue_pv(vs, j == 0);
-          umma_commit(&o_full[w]);
-          umma_commit(&empty[vs]);
-        }
-        __syncwarp();
-        used += 2;
+      // (The shuffle tells the compiler that the count, and with it the ring slot
+      // and the descriptors, are the same in all lanes.)
+      const int n = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s_blocks[items % kItemRing]), 0);
+      left -= n;
+      if (!wait(&full[ks], kp)) { ok = false; break; }
+      tc_fence_after();
+      if (leader) {
+        issue_s(0, ks);
+        umma_commit(&s_full[0]);
+        issue_s(1, ks);
+        umma_commit(&s_full[1]);
+        umma_commit(&empty[ks]);
+        if (n == 1) umma_commit(q_free);
       }
-      // The next item's S must not overwrite P before the last P V has read it.
-      if (ok && !wait(&o_full[w], (blocks - 1) & 1u)) ok = false;
-      t += n;
-      if (ok && t < t_end) cur.next(p);
-    }
-    if (!ok) {
-      if (leader) umma_commit(&drain_bar[w]);
       __syncwarp();
-      mbar_drain_wait(&drain_bar[w], 0, 1000000000ull);
+      for (int j = 0; j < n && ok; ++j, ++blocks) {
+        const int vs = ks + 1 == L::kSlots ? 0 : ks + 1, next = vs + 1 == L::kSlots ? 0 : vs + 1;
+        const uint32_t vp = vs == 0 ? kp ^ 1u : kp, np = next == 0 ? vp ^ 1u : vp;
+        const bool more = j + 1 < n;
+        if (!wait(&full[vs], vp)) { ok = false; break; }
+        if (more && !wait(&full[next], np)) { ok = false; break; }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (!wait(&p_ready[w], blocks & 1u)) { ok = false; break; }
+          // The item's first P V overwrites O: the item before must have been read.
+          if (j == 0 && items > 0 && !wait(&o_free[w], (items - 1) & 1u)) { ok = false; break; }
+          tc_fence_after();
+          if (leader) {
+            issue_pv(w, vs, j == 0);
+            umma_commit(&o_full[w]);
+            if (w == 1) umma_commit(&empty[vs]);
+            if (more) {
+              // S overwrites P, which shares its columns: the tensor core runs
+              // the products of one thread in their order of issue, so P V has
+              // read P by then.
+              issue_s(w, next);
+              umma_commit(&s_full[w]);
+              if (w == 1) {
+                umma_commit(&empty[next]);
+                if (j + 2 == n) umma_commit(q_free);
+              }
+            }
+          }
+          __syncwarp();
+        }
+        ks = next;
+        kp = np;
+      }
     }
-  } else if (warp >= 8) {
-    reg_dealloc<kIssueRegs>();   // idle warps of the issuers' warpgroup
+    if (!ok && warp == 8) {
+      if (leader) umma_commit(drain_bar);
+      __syncwarp();
+      mbar_drain_wait(drain_bar, 0, 1000000000ull);
+    }
   } else {
     reg_alloc<kSoftmaxRegs>();
     // ------------------------------------------------------------- softmax --
@@ -483,10 +528,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + L::kTmemS + w * 128;
     const uint32_t tO = tmem_base + lane_off + L::kTmemO + w * D;
-    // The maximum needs a positive factor: a negative scale turns the scores'
-    // signs, a zero one becomes too small to matter.
-    const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);
-    const bool negative = p.scale < 0.f;
+    // The maximum needs a positive factor (the scale is not negative here): a
+    // zero one becomes too small to matter.
+    const float sl2 = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);
     bool ok = true;
     Cursor cur = s_cursor;
     uint32_t blocks = 0;
@@ -513,12 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
         reg_fence(sc[2]);
         reg_fence(sc[3]);
         const int kv0 = (block0 + j) * kBlock;
-        if (negative) {
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) sc[cc][e] ^= 0x80000000u;
-        }
         const bool masked = (keep.x & keep.y & keep.z & keep.w) != ~0u || __any_sync(0xffffffffu, kv0 < lo || kv0 + kBlock > hi);
         if (masked) {
           const uint32_t words[4] = {keep.x, keep.y, keep.z, keep.w};
@@ -547,7 +585,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
         if (j == 0) {
           m = cand;
         } else if (__any_sync(0xffffffffu, !(cand <= m + kRescaleLog2))) {
-          // P V of the block before is complete (S of this block was issued after it).
+          // O is rescaled once P V of the block before has completed (as it has:
+          // S of this block ran after it).
+          if (!mbar_wait_warp(&o_full[w], (blocks - 1) & 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
+          tc_fence_after();
           const float next = fmax_nan(m, cand);
           const float alpha = next == -INFINITY ? 1.f : ex2_approx(m - next);
           l *= alpha;
@@ -595,19 +636,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
                 e2[q] = f2_pack(ex2_approx(v.x), ex2_approx(v.y));
               }
             }
-            if (masked) {
-              // The cubic gives 2^-126 for a masked score; it must count as nothing
-              // (a row whose block is all masked keeps its maximum of -inf).
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const int pair = g0 + q;
-                if (((pair * kPolyPairs) % 16) < kPolyPairs) {
-                  const int e = 2 * pair;
-                  const float2 v = f2_unpack(e2[q]);
-                  e2[q] = f2_pack(sc[c][e] == 0xFF800000u ? 0.f : v.x, sc[c][e + 1] == 0xFF800000u ? 0.f : v.y);
-                }
-              }
-            }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const int pair = g0 + q;
@@ -628,6 +656,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
       if (!ok) break;
       tc_fence_after();
       // ------------------------------------------------------------ results --
+      // A masked score adds 2^-126 at most (the cubic's smallest), which is
+      // nothing beside a row's largest, but the whole sum of a row that saw no
+      // key: such a row keeps its maximum of -inf.
+      if (m == -INFINITY) l = 0.f;
       const bool whole = x.first == 0 && n == x.item_blocks;
       const float f = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.f;
       const int head = x.kh * p.group + static_cast<int>((real ? row : rows - 1) - static_cast<int64_t>(i) * p.group);
@@ -689,6 +721,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(const __grid
   }
 }
 
+// Tensor map of the pages, a box of `rows` rows of 64 elements.
+bool encode_pages(CUtensorMap* map, const void* pages, int dtype, const PagedParams& p, int64_t page, int64_t head, int rows) {
+  auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(tensor_map_encoder());
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), static_cast<cuuint64_t>(p.page_size),
+                              static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.num_pages)};
+  // A dimension of extent 1 is never stepped: any stride will do.
+  const cuuint64_t row = static_cast<cuuint64_t>(p.dim) * 2;
+  const cuuint64_t strides[3] = {row, p.kv_heads == 1 ? row : static_cast<cuuint64_t>(head) * 2,
+                                 p.num_pages == 1 ? row : static_cast<cuuint64_t>(page) * 2};
+  for (cuuint64_t v : strides)
+    if (v == 0 || v % 16 != 0 || v >= (cuuint64_t{1} << 40)) return false;
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return encode(map, dtype == LUNARA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                const_cast<void*>(pages), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
   using L = Layout<D>;
@@ -700,6 +751,15 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
   if (fa.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;   // the setmaxnreg split counts on it
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
   if (e != cudaSuccess) return e;
+  // TMA where pages tile a 128-key block in boxes of whole swizzle atoms (8
+  // rows); row by row elsewhere (box_rows 0).
+  const int ps = p.page_size;
+  int box_rows = ps >= 8 && (ps % kBlock == 0 || kBlock % ps == 0) ? (ps < kBlock ? ps : kBlock) : 0;
+  CUtensorMap mk{}, mv{};
+  const int dtype = std::is_same<T, __nv_bfloat16>::value ? LUNARA_BF16 : LUNARA_F16;
+  if (box_rows > 0 && (!encode_pages(&mk, p.k, dtype, p, p.k_page, p.k_head, box_rows) ||
+                       !encode_pages(&mv, p.v, dtype, p, p.v_page, p.v_head, box_rows)))
+    box_rows = 0;
   const int batch = p.seqs.batch;
   const Seqs all = p.seqs;
   for (int b0 = 0; b0 < batch; b0 += kMaxBatch) {
@@ -707,7 +767,7 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
     p.seqs.page_table = all.page_table + b0 * all.table_stride;
     p.seqs.starts = all.starts + b0;
     p.seqs.lens = all.lens + b0;
-    e = launch_pdl(kern, dim3(p.workers), dim3(kThreads), static_cast<size_t>(L::kSmem), s, p);
+    e = launch_pdl(kern, dim3(p.workers), dim3(kThreads), static_cast<size_t>(L::kSmem), s, p, mk, mv, box_rows);
     if (e != cudaSuccess) return e;
     e = launch_pdl(paged_join_kernel<T, D>, dim3(join_blocks(p.workers), 16), dim3(kJoinThreads), 0, s, p, int{kItemRows});
     if (e != cudaSuccess) return e;
