@@ -11,12 +11,14 @@
 // one (no contraction into FMAs), so that the 4-bit codes made from them are
 // the same in any implementation of the definition.
 //
-// Work split. A lane holds the two 8-element vectors of one "unit" of a row
-// (both halves of 8 pairs, or 16 neighbouring elements), so a pair never
-// crosses lanes, rotation in place is safe and every access is 16 bytes. The
-// (cos, sin) of its 8 pairs stay in registers while the lane walks over kHeads
-// heads of the token: the fp32 table (64 bytes per lane) is read once for
-// them instead of once per head.
+// Work split. A lane holds two 8-element vectors of a row, one in each half of
+// the rotated elements (or of those behind them), so a pair of either layout
+// never crosses lanes, rotation in place is safe, and neighbouring lanes access
+// neighbouring 16 bytes. The (cos, sin) of its 8 pairs stay in registers while
+// the lane walks over kHeads heads of the token: the fp32 table (64 bytes per
+// lane) is read once for them instead of once per head. The rows are loaded
+// before anything is known of the position, so that the chain of dependent
+// loads is (sequence, page) or position, table, and nothing more.
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -129,32 +131,67 @@ __device__ __forceinline__ TokenPlace place_token(const RowsParams& p, int token
   return t;
 }
 
-template <typename T, int LAYOUT, bool NORM, bool PAGED, int HEADS>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ RowsParams p) {
+// The 4-bit form of a scale block of 16 elements.
+struct QuantParams {
+  RowsParams r;
+  void* scales[3];
+  int64_t sc_page[3], sc_head[3];
+  float inv_gain[3];
+  int blocks;   // dim / 16
+};
+
+// code = e2m1(y / s), the quotient rounded to nearest as IEEE division does:
+// with r = RN(1/s), q0 = RN(y r) and the exact remainder y - q0 s, RN(q0 +
+// remainder * r) is the correctly rounded quotient (Markstein, 1990; s has 4
+// significant bits, so the all-ones exception of the theorem cannot arise).
+__device__ __forceinline__ float quotient(float y, float s, float r) {
+  const float q0 = __fmul_rn(y, r);
+  return __fmaf_rn(__fmaf_rn(-q0, s, y), r, q0);
+}
+
+// The e4m3 scale of a block whose largest magnitude is amax (saturates at 448,
+// keeps NaN), and the codes of N of its elements, 4 bits each.
+template <int N>
+__device__ __forceinline__ uint32_t quantise(const float (&y)[N], int first, float amax, uint32_t& scale) {
+  scale = float_to_e4m3(__fdiv_rn(amax, 6.0f));
+  const float s = e4m3_to_float(scale);
+  uint32_t w = 0u;
+  if (s > 0.f) {
+    const float r = __frcp_rn(s);
+    const bool finite = amax < 1e30f;   // beyond, the remainder may overflow
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float lo = finite ? quotient(y[first + i], s, r) : __fdiv_rn(y[first + i], s);
+      const float hi = finite ? quotient(y[first + i + 1], s, r) : __fdiv_rn(y[first + i + 1], s);
+      w |= float2_to_e2m1x2(lo, hi) << (4 * i);
+    }
+  }
+  return w;
+}
+
+// QUANT: paged rows go to a 4-bit cache; a scale block belongs to two
+// neighbouring lanes.
+template <typename T, int LAYOUT, bool NORM, bool PAGED, bool QUANT, int HEADS>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ QuantParams q) {
+  const RowsParams& p = q.r;
   pdl_wait();
   pdl_launch_dependents();
   const int lanes = 1 << p.lanes_log2;
-  const int gid = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
+  const int token = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
   const int u = static_cast<int>(threadIdx.x) & (lanes - 1);
   int which = 0;
   while (which < 2 && static_cast<int>(blockIdx.y) >= p.group_end[which]) ++which;
   const RowSet& set = p.set[which];
   const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.group_end[which - 1] : 0)) * HEADS;
   const int nh = min(HEADS, set.heads - h0);
-  const TokenPlace t = place_token<PAGED>(p, gid, p.rot > 0);
-  const bool rotate = set.rotate && 16 * u < p.rot;
-  const bool active = t.owned && u < p.units;
-  int o0, o1;
-  if (LAYOUT == LUNARAD_ROTARY_HALF && 16 * u < p.rot) {
-    o0 = 8 * u;
-    o1 = p.rot / 2 + 8 * u;
-  } else {
-    o0 = 16 * u;
-    o1 = o0 + 8;
-  }
-  const T* src = static_cast<const T*>(set.src) + t.b * set.sb + t.s * set.ss + h0 * set.sh;
+  const bool lane_in = token < p.tokens && u < p.units;
+  const bool turns = 16 * u < p.rot;
+  const int o0 = turns ? 8 * u : p.rot / 2 + 8 * u;                                  // rot + 8 (u - rot / 16)
+  const int o1 = turns ? p.rot / 2 + 8 * u : p.dim / 2 + 8 * u;                      // rot + (dim - rot) / 2 + 8 (u - rot / 16)
   float a[HEADS][8], b[HEADS][8];
-  if (active && t.valid) {
+  if (lane_in) {
+    const int sb = PAGED ? 0 : token / p.seq, ss = PAGED ? token : token - sb * p.seq;
+    const T* src = static_cast<const T*>(set.src) + sb * set.sb + ss * set.ss + h0 * set.sh;
 #pragma unroll
     for (int h = 0; h < HEADS; ++h)
       if (h < nh) {
@@ -162,12 +199,16 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
         load8(src + h * set.sh + o1, b[h]);
       }
   }
+  const TokenPlace t = place_token<PAGED>(p, token, p.rot > 0);
+  const bool rotate = set.rotate && turns;
   float cs[16];
-  if (active && t.valid && rotate) {
-    const float4* row = reinterpret_cast<const float4*>(p.table + t.pos * p.rot + 16 * u);
+  if (lane_in && t.valid && rotate) {
+    const float* row = p.table + t.pos * p.rot;
+    const float* c0 = row + (LAYOUT == LUNARAD_ROTARY_HALF ? 16 * u : o0);
+    const float* c1 = LAYOUT == LUNARAD_ROTARY_HALF ? c0 + 8 : row + o1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 v = __ldg(row + i);
+      const float4 v = __ldg(reinterpret_cast<const float4*>(i < 2 ? c0 : c1) + (i & 1));
       cs[4 * i] = v.x; cs[4 * i + 1] = v.y; cs[4 * i + 2] = v.z; cs[4 * i + 3] = v.w;
     }
     if (p.inverse) {
@@ -177,22 +218,23 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
   }
   if constexpr (NORM) {
     float w0[8], w1[8];
-    if (active && set.weight != nullptr) {
+    if (lane_in && set.weight != nullptr) {
       load8(static_cast<const T*>(set.weight) + o0, w0);
       load8(static_cast<const T*>(set.weight) + o1, w1);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w0[i] = w1[i] = 1.f;
     }
+    const float inv_dim = 1.0f / static_cast<float>(p.dim);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
       float ss = 0.f;
-      if (active && t.valid && h < nh) {
+      if (lane_in && h < nh) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(a[h][i], a[h][i], fmaf(b[h][i], b[h][i], ss));
       }
       for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss / static_cast<float>(p.dim) + p.eps);
+      const float r = rsqrtf(fmaf(ss, inv_dim, p.eps));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         a[h][i] = a[h][i] * r * w0[i];
@@ -200,34 +242,55 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ 
       }
     }
   }
-  if (!active) return;
-  T* dst = static_cast<T*>(set.dst);
-  if (set.paged) {
-    if (!t.valid) return;
-    dst += t.page * set.db + h0 * set.dh + t.slot * set.ds;
-  } else {
-    dst += t.b * set.db + t.s * set.ds + h0 * set.dh;
-  }
+  const bool stores = lane_in && t.owned && (t.valid || !set.paged);
+  char* dst = static_cast<char*>(set.dst);
+  const int elem = QUANT && set.paged ? 1 : static_cast<int>(sizeof(T));
+  if (stores) dst += (set.paged ? t.page * set.db + t.slot * set.ds : t.b * set.db + t.s * set.ds) * elem + h0 * set.dh * elem;
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    if (h < nh) {
-      if (!t.valid) {
+    if (h >= nh) break;   // the same in all lanes
+    if (!t.valid) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[h][i] = b[h][i] = 0.f;
-      } else if (rotate) {
-        if (LAYOUT == LUNARAD_ROTARY_HALF) {
+      for (int i = 0; i < 8; ++i) a[h][i] = b[h][i] = 0.f;
+    } else if (rotate) {
+      if (LAYOUT == LUNARAD_ROTARY_HALF) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) turn(a[h][i], b[h][i], cs[2 * i], cs[2 * i + 1]);
-        } else {
+        for (int i = 0; i < 8; ++i) turn(a[h][i], b[h][i], cs[2 * i], cs[2 * i + 1]);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            turn(a[h][2 * i], a[h][2 * i + 1], cs[2 * i], cs[2 * i + 1]);
-            turn(b[h][2 * i], b[h][2 * i + 1], cs[8 + 2 * i], cs[8 + 2 * i + 1]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          turn(a[h][2 * i], a[h][2 * i + 1], cs[2 * i], cs[2 * i + 1]);
+          turn(b[h][2 * i], b[h][2 * i + 1], cs[8 + 2 * i], cs[8 + 2 * i + 1]);
         }
       }
-      store8(dst + h * set.dh + o0, a[h]);
-      store8(dst + h * set.dh + o1, b[h]);
+    }
+    char* row = dst + h * set.dh * elem;
+    if (QUANT && set.paged) {   // (the same in all lanes)
+      float top[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[h][i] = __fmul_rn(a[h][i], q.inv_gain[which]);
+        b[h][i] = __fmul_rn(b[h][i], q.inv_gain[which]);
+        top[0] = fmax_nan(top[0], fabsf(a[h][i]));
+        top[1] = fmax_nan(top[1], fabsf(b[h][i]));
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) top[k] = fmax_nan(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+      uint32_t s0, s1;
+      const uint32_t w0 = quantise(a[h], 0, top[0], s0), w1 = quantise(b[h], 0, top[1], s1);
+      if (stores) {
+        *reinterpret_cast<uint32_t*>(row + o0 / 2) = w0;
+        *reinterpret_cast<uint32_t*>(row + o1 / 2) = w1;
+        if ((u & 1) == 0) {
+          uint8_t* sc = static_cast<uint8_t*>(q.scales[which]) + t.page * q.sc_page[which] + (h0 + h) * q.sc_head[which] +
+                        static_cast<int64_t>(t.slot) * q.blocks;
+          sc[o0 / 16] = static_cast<uint8_t>(s0);
+          sc[o1 / 16] = static_cast<uint8_t>(s1);
+        }
+      }
+    } else if (stores) {
+      store8(reinterpret_cast<T*>(row) + o0, a[h]);
+      store8(reinterpret_cast<T*>(row) + o1, b[h]);
     }
   }
 }
@@ -284,31 +347,10 @@ __global__ void __launch_bounds__(kThreads) rows_any_kernel(const __grid_constan
 }
 
 // ------------------------------------------------- append to a 4-bit cache --
-// A thread makes the 16 elements of one scale block: rotates them (reading the
-// partner elements of the half layout as well; they are in L1 from the lane
-// that owns them), takes their largest magnitude, the e4m3 scale and the codes,
-// and writes 8 bytes of codes and one scale byte. Query rows go the same way
-// and are stored unquantised.
-struct QuantParams {
-  RowsParams r;
-  void* scales[3];
-  int64_t sc_page[3], sc_head[3];
-  float inv_gain[3];
-  int blocks;   // dim / 16
-};
-
-// code = e2m1(y / s), the quotient rounded to nearest as IEEE division does:
-// with r = RN(1/s), q0 = RN(y r) and the exact remainder y - q0 s, RN(q0 +
-// remainder * r) is the correctly rounded quotient (Markstein, 1990; s has 4
-// significant bits, so the all-ones exception of the theorem cannot arise, and
-// y / s <= 7 while y is finite, so nothing over- or underflows that matters).
-__device__ __forceinline__ float quotient(float y, float s, float r) {
-  const float q0 = __fmul_rn(y, r);
-  return __fmaf_rn(__fmaf_rn(-q0, s, y), r, q0);
-}
-
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) append_e2m1_kernel(const __grid_constant__ QuantParams q, int layout) {
+// Any rot and alignment: a thread makes the 16 elements of one scale block of a
+// cached row (fetching their partners too), element by element.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) append_e2m1_any_kernel(const __grid_constant__ QuantParams q, int layout) {
   pdl_wait();
   pdl_launch_dependents();
   const RowsParams& p = q.r;
@@ -320,75 +362,26 @@ __global__ void __launch_bounds__(kThreads) append_e2m1_kernel(const __grid_cons
   const RowSet& set = p.set[which];
   const int h = static_cast<int>(blockIdx.y) - (which ? p.group_end[which - 1] : 0);
   const TokenPlace t = place_token<true>(p, token, p.rot > 0);
-  if (!t.owned || u >= q.blocks || (set.paged && !t.valid)) return;
+  if (!t.owned || u >= q.blocks || !t.valid) return;
   const T* src = static_cast<const T*>(set.src) + t.s * set.ss + h * set.sh;
   const int d0 = 16 * u;
   float y[16];
-  if (!t.valid) {
+  const int rot = set.rotate ? p.rot : 0;
+  const float* row = p.table + t.pos * p.rot;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = 0.f;
-  } else {
-    const int rot = set.rotate ? p.rot : 0;
-    const float* row = p.table + t.pos * p.rot;
-    if constexpr (VEC) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int d = d0 + 8 * c;
-        float x[8];
-        load8(src + d, x);
-        if (d < rot) {
-          if (layout == LUNARAD_ROTARY_HALF) {
-            const bool first = d < rot / 2;
-            float z[8];
-            load8(src + (first ? d + rot / 2 : d - rot / 2), z);
-            const float* cs = row + 2 * (first ? d : d - rot / 2);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float a = first ? x[i] : z[i], b = first ? z[i] : x[i];
-              turn(a, b, __ldg(cs + 2 * i), __ldg(cs + 2 * i + 1));
-              x[i] = first ? a : b;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], __ldg(row + d + 2 * i), __ldg(row + d + 2 * i + 1));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[8 * c + i] = x[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int d = d0 + i;
-        float x = Io<T>::to_f(src[d]);
-        if (d < rot) {
-          const bool first = layout == LUNARAD_ROTARY_HALF ? d < rot / 2 : (d & 1) == 0;
-          const int other = layout == LUNARAD_ROTARY_HALF ? (first ? d + rot / 2 : d - rot / 2) : (d ^ 1);
-          const int pair = layout == LUNARAD_ROTARY_HALF ? (first ? d : d - rot / 2) : d >> 1;
-          const float z = Io<T>::to_f(src[other]);
-          float a = first ? x : z, b = first ? z : x;
-          turn(a, b, row[2 * pair], row[2 * pair + 1]);
-          x = first ? a : b;
-        }
-        y[i] = x;
-      }
+  for (int i = 0; i < 16; ++i) {
+    const int d = d0 + i;
+    float x = Io<T>::to_f(src[d]);
+    if (d < rot) {
+      const bool first = layout == LUNARAD_ROTARY_HALF ? d < rot / 2 : (d & 1) == 0;
+      const int other = layout == LUNARAD_ROTARY_HALF ? (first ? d + rot / 2 : d - rot / 2) : (d ^ 1);
+      const int pair = layout == LUNARAD_ROTARY_HALF ? (first ? d : d - rot / 2) : d >> 1;
+      const float z = Io<T>::to_f(src[other]);
+      float a = first ? x : z, b = first ? z : x;
+      turn(a, b, row[2 * pair], row[2 * pair + 1]);
+      x = first ? a : b;
     }
-  }
-  if (!set.paged) {
-    T* dst = static_cast<T*>(set.dst) + t.s * set.ds + h * set.dh + d0;
-#pragma unroll
-    for (int i = 0; i < 16; i += 8) {
-      if constexpr (VEC) {
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = y[i + j];
-        store8(dst + i, f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dst[i + j] = Io<T>::from_f(y[i + j]);
-      }
-    }
-    return;
+    y[i] = x;
   }
   float amax = 0.f;
 #pragma unroll
@@ -396,21 +389,10 @@ __global__ void __launch_bounds__(kThreads) append_e2m1_kernel(const __grid_cons
     y[i] = __fmul_rn(y[i], q.inv_gain[which]);
     amax = fmax_nan(amax, fabsf(y[i]));
   }
-  const uint32_t sb = float_to_e4m3(__fdiv_rn(amax, 6.0f));   // saturates at 448, keeps NaN
-  const float s = e4m3_to_float(sb);
-  uint32_t w[2] = {0u, 0u};
-  if (s > 0.f) {
-    const float r = __frcp_rn(s);
-    const bool finite = amax < 1e30f;   // beyond, the quotient's remainder may overflow
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float lo = finite ? quotient(y[i], s, r) : __fdiv_rn(y[i], s);
-      const float hi = finite ? quotient(y[i + 1], s, r) : __fdiv_rn(y[i + 1], s);
-      w[i >> 3] |= float2_to_e2m1x2(lo, hi) << (4 * (i & 7));
-    }
-  }
+  uint32_t sb;
+  const uint32_t w0 = quantise(y, 0, amax, sb), w1 = quantise(y, 8, amax, sb);
   uint8_t* dst = static_cast<uint8_t*>(set.dst) + t.page * set.db + h * set.dh + t.slot * set.ds + 8 * u;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
   static_cast<uint8_t*>(q.scales[which])[t.page * q.sc_page[which] + h * q.sc_head[which] +
                                          static_cast<int64_t>(t.slot) * q.blocks + u] = static_cast<uint8_t>(sb);
 }
@@ -427,14 +409,71 @@ struct ReadParams {
   unsigned int* err;
 };
 
-// blockIdx.y = head, blockIdx.z = 0 keys / 1 values; a lane moves 16 elements.
-template <typename T, bool E2M1, bool VEC>
+// blockIdx.y = group of HEADS heads, blockIdx.z = 0 keys / 1 values; a lane
+// moves 8 neighbouring elements of each head, so that both the codes and the
+// rows are accessed without gaps, and all heads' loads are in flight at once.
+template <typename T, bool E2M1, int HEADS>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const int lanes = 1 << p.lanes_log2;
   const int token = static_cast<int>(blockIdx.x) * (kThreads >> p.lanes_log2) + (static_cast<int>(threadIdx.x) >> p.lanes_log2);
-  const int u0 = static_cast<int>(threadIdx.x) & (lanes - 1);
+  if (token >= p.tokens) return;
+  const int h0 = static_cast<int>(blockIdx.y) * HEADS, kv = static_cast<int>(blockIdx.z), nh = min(HEADS, p.heads - h0);
+  int seq, slot = 0, page = -1;
+  int64_t pos;
+  if (!find_token(p.seqs, token, seq, pos)) return;
+  if (pos >= 0) page = find_page(p.seqs, seq, pos, p.num_pages, slot, p.err);
+  T* dst = static_cast<T*>(p.dst[kv]) + (static_cast<int64_t>(token) * p.heads + h0) * p.dim;
+  const int64_t at = page * p.page_stride[kv] + h0 * p.head_stride[kv];
+  for (int u = static_cast<int>(threadIdx.x) & (lanes - 1); u < p.units; u += lanes) {
+    if constexpr (E2M1) {
+      uint32_t w[HEADS], s[HEADS];
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+        w[h] = s[h] = 0u;
+        if (page >= 0 && h < nh) {
+          w[h] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.src[kv]) + at + h * p.head_stride[kv] +
+                                                         static_cast<int64_t>(slot) * (p.dim / 2)) + u);
+          s[h] = __ldg(static_cast<const uint8_t*>(p.scales[kv]) + page * p.sc_page[kv] + (h0 + h) * p.sc_head[kv] +
+                       static_cast<int64_t>(slot) * (p.dim / 16) + (u >> 1));
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h)
+        if (h < nh) {
+          const float scale = __fmul_rn(e4m3_to_float(s[h]), p.gain[kv]);
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = __half22float2(e2m1x2_to_half2((w[h] >> (8 * i)) & 0xFFu));
+            x[2 * i] = __fmul_rn(v.x, scale);
+            x[2 * i + 1] = __fmul_rn(v.y, scale);
+          }
+          store8(dst + h * p.dim + 8 * u, x);
+        }
+    } else {
+      float x[HEADS][8];
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[h][i] = 0.f;
+        if (page >= 0 && h < nh)
+          load8(static_cast<const T*>(p.src[kv]) + at + h * p.head_stride[kv] + static_cast<int64_t>(slot) * p.dim + 8 * u, x[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h)
+        if (h < nh) store8(dst + h * p.dim + 8 * u, x[h]);
+    }
+  }
+}
+
+// Any head dimension and alignment, element by element (4 bits: by scale blocks).
+template <typename T, bool E2M1>
+__global__ void __launch_bounds__(kThreads) read_any_kernel(const __grid_constant__ ReadParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int token = static_cast<int>(blockIdx.x) * (kThreads / 32) + (static_cast<int>(threadIdx.x) >> 5);
   if (token >= p.tokens) return;
   const int h = static_cast<int>(blockIdx.y), kv = static_cast<int>(blockIdx.z);
   int seq, slot = 0, page = -1;
@@ -443,46 +482,20 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   if (pos >= 0) page = find_page(p.seqs, seq, pos, p.num_pages, slot, p.err);
   T* dst = static_cast<T*>(p.dst[kv]) + (static_cast<int64_t>(token) * p.heads + h) * p.dim;
   const int64_t at = page * p.page_stride[kv] + h * p.head_stride[kv];
-  for (int u = u0; u < p.units; u += lanes) {
-    float f[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = 0.f;
-    if constexpr (E2M1) {
-      if (page >= 0) {
-        const uint8_t* c = static_cast<const uint8_t*>(p.src[kv]) + at + static_cast<int64_t>(slot) * (p.dim / 2) + 8 * u;
-        const uint32_t sb = static_cast<const uint8_t*>(p.scales[kv])[page * p.sc_page[kv] + h * p.sc_head[kv] +
-                                                                      static_cast<int64_t>(slot) * (p.dim / 16) + u];
-        const uint2 w = *reinterpret_cast<const uint2*>(c);
-        const float s = __fmul_rn(e4m3_to_float(sb), p.gain[kv]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 v = __half22float2(e2m1x2_to_half2(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFu));
-          f[2 * i] = __fmul_rn(v.x, s);
-          f[2 * i + 1] = __fmul_rn(v.y, s);
-        }
+  for (int d = static_cast<int>(threadIdx.x) & 31; d < p.dim; d += 32) {
+    T x = Io<T>::from_f(0.f);
+    if (page >= 0) {
+      if constexpr (E2M1) {
+        const uint8_t byte = static_cast<const uint8_t*>(p.src[kv])[at + static_cast<int64_t>(slot) * (p.dim / 2) + (d >> 1)];
+        const uint8_t sb = static_cast<const uint8_t*>(p.scales[kv])[page * p.sc_page[kv] + h * p.sc_head[kv] +
+                                                                     static_cast<int64_t>(slot) * (p.dim / 16) + (d >> 4)];
+        const float2 v = __half22float2(e2m1x2_to_half2(byte));
+        x = Io<T>::from_f(__fmul_rn(d & 1 ? v.y : v.x, __fmul_rn(e4m3_to_float(sb), p.gain[kv])));
+      } else {
+        x = static_cast<const T*>(p.src[kv])[at + static_cast<int64_t>(slot) * p.dim + d];
       }
     }
-    if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        float x[8];
-        if constexpr (E2M1) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = f[i + j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = 0.f;
-          if (page >= 0) load8(static_cast<const T*>(p.src[kv]) + at + static_cast<int64_t>(slot) * p.dim + 16 * u + i, x);
-        }
-        store8(dst + 16 * u + i, x);
-      }
-    } else {
-      for (int i = 0; i < 16 && 16 * u + i < p.dim; ++i) {
-        if constexpr (E2M1) dst[16 * u + i] = Io<T>::from_f(f[i]);
-        else dst[16 * u + i] = page >= 0 ? static_cast<const T*>(p.src[kv])[at + static_cast<int64_t>(slot) * p.dim + 16 * u + i]
-                                         : Io<T>::from_f(0.f);
-      }
-    }
+    dst[d] = x;
   }
 }
 
@@ -495,16 +508,21 @@ int log2_ceil(int n) {
   return l;
 }
 
-// Whether the 16-byte row kernel takes the sets: whole units, 16-byte aligned rows.
-bool rows_vector_ok(const RowsParams& p, int n_sets, int elem) {
-  if (p.dim % 16 != 0 || p.rot % 16 != 0 || p.dim > 512) return false;
+// Whether the 16-byte row kernel takes the sets: whole units (into a 4-bit cache
+// pairs of them), 16-byte aligned rows.
+bool rows_vector_ok(const RowsParams& p, int n_sets, int elem, bool quant) {
+  const int whole = quant ? 32 : 16;
+  if (p.dim % whole != 0 || p.rot % whole != 0 || p.dim > 512) return false;
   if (p.rot > 0 && !al16(p.table)) return false;
   const int64_t vec = 16 / elem;
   for (int i = 0; i < n_sets; ++i) {
     const RowSet& s = p.set[i];
-    if (!al16(s.src) || !al16(s.dst) || !al16(s.weight)) return false;
-    const int64_t st[6] = {s.sb, s.sh, s.ss, s.db, s.dh, s.ds};
-    for (int64_t v : st)
+    if (!al16(s.src) || !al16(s.weight)) return false;
+    for (int64_t v : {s.sb, s.sh, s.ss})
+      if (v % vec != 0) return false;
+    if (quant && s.paged) continue;   // words of codes: the library's entry has checked their alignment
+    if (!al16(s.dst)) return false;
+    for (int64_t v : {s.db, s.dh, s.ds})
       if (v % vec != 0) return false;
   }
   return true;
@@ -520,35 +538,58 @@ void set_groups(RowsParams& p, int n_sets, int per) {
 
 constexpr int kHeads = 4;
 
-template <typename T, bool NORM, bool PAGED>
-cudaError_t run_rows(RowsParams p, int n_sets, int layout, cudaStream_t s) {
+template <typename T, bool NORM, bool PAGED, bool QUANT, int HEADS>
+cudaError_t run_rows_vector(const QuantParams& q, int layout, dim3 grid, cudaStream_t s) {
+  return layout == LUNARAD_ROTARY_HALF
+             ? launch_pdl(rows_kernel<T, LUNARAD_ROTARY_HALF, NORM, PAGED, QUANT, HEADS>, grid, dim3(kThreads), 0, s, q)
+             : launch_pdl(rows_kernel<T, LUNARAD_ROTARY_INTERLEAVED, NORM, PAGED, QUANT, HEADS>, grid, dim3(kThreads), 0, s, q);
+}
+
+template <typename T, bool NORM, bool PAGED, bool QUANT>
+cudaError_t run_rows(QuantParams q, int n_sets, int layout, cudaStream_t s) {
+  RowsParams& p = q.r;
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;
-  if (!rows_vector_ok(p, n_sets, sizeof(T))) {
-    set_groups(p, n_sets, 1);
-    const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, kThreads / 32)), p.group_end[2]);
-    return launch_pdl(rows_any_kernel<T, NORM, PAGED>, grid, dim3(kThreads), 0, s, p, layout);
+  const bool vector = rows_vector_ok(p, n_sets, sizeof(T), QUANT);
+  if (!vector) {
+    if constexpr (QUANT) {
+      // The cached rows block by block, the query rows (which may be rotated in
+      // place) pair by pair.
+      set_groups(p, 2, 1);
+      q.blocks = p.dim / 16;
+      p.lanes_log2 = log2_ceil(q.blocks);
+      const dim3 blocks(static_cast<unsigned>(ceil_div64(p.tokens, kThreads >> p.lanes_log2)), p.group_end[2]);
+      const cudaError_t e = launch_pdl(append_e2m1_any_kernel<T>, blocks, dim3(kThreads), 0, s, q, layout);
+      if (e != cudaSuccess || n_sets < 3) return e;
+      QuantParams rest = q;
+      rest.r.set[0] = q.r.set[2];
+      return run_rows<T, NORM, PAGED, false>(rest, 1, layout, s);
+    } else {
+      set_groups(p, n_sets, 1);
+      const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, kThreads / 32)), p.group_end[2]);
+      return launch_pdl(rows_any_kernel<T, NORM, PAGED>, grid, dim3(kThreads), 0, s, p, layout);
+    }
   }
   p.units = p.dim / 16;
+  q.blocks = p.dim / 16;
   p.lanes_log2 = log2_ceil(p.units);
   const int per_block = kThreads >> p.lanes_log2;
   const unsigned gx = static_cast<unsigned>(ceil_div64(p.tokens, per_block));
+  // One head per lane while that leaves the SMs free slots (latency counts);
+  // several, so that the table is read less often, beyond.
   set_groups(p, n_sets, 1);
   const bool few = static_cast<int64_t>(gx) * p.group_end[2] <= int64_t{device_num_sms()} * 16;
   if (!few) set_groups(p, n_sets, kHeads);
   const dim3 grid(gx, p.group_end[2]);
-  if (layout == LUNARAD_ROTARY_HALF)
-    return few ? launch_pdl(rows_kernel<T, LUNARAD_ROTARY_HALF, NORM, PAGED, 1>, grid, dim3(kThreads), 0, s, p)
-               : launch_pdl(rows_kernel<T, LUNARAD_ROTARY_HALF, NORM, PAGED, kHeads>, grid, dim3(kThreads), 0, s, p);
-  return few ? launch_pdl(rows_kernel<T, LUNARAD_ROTARY_INTERLEAVED, NORM, PAGED, 1>, grid, dim3(kThreads), 0, s, p)
-             : launch_pdl(rows_kernel<T, LUNARAD_ROTARY_INTERLEAVED, NORM, PAGED, kHeads>, grid, dim3(kThreads), 0, s, p);
+  return few ? run_rows_vector<T, NORM, PAGED, QUANT, 1>(q, layout, grid, s)
+             : run_rows_vector<T, NORM, PAGED, QUANT, kHeads>(q, layout, grid, s);
 }
 
-template <bool NORM, bool PAGED>
-cudaError_t run_rows_dtype(const RowsParams& p, int n_sets, int layout, int64_t dtype, cudaStream_t s) {
-  if (dtype == LUNARA_F16) return run_rows<__half, NORM, PAGED>(p, n_sets, layout, s);
-  if (dtype == LUNARA_BF16) return run_rows<__nv_bfloat16, NORM, PAGED>(p, n_sets, layout, s);
-  return run_rows<float, NORM, PAGED>(p, n_sets, layout, s);
+template <bool NORM, bool PAGED, bool QUANT>
+cudaError_t run_rows_dtype(const QuantParams& q, int n_sets, int layout, int64_t dtype, cudaStream_t s) {
+  if (dtype == LUNARA_F16) return run_rows<__half, NORM, PAGED, QUANT>(q, n_sets, layout, s);
+  if (dtype == LUNARA_BF16) return run_rows<__nv_bfloat16, NORM, PAGED, QUANT>(q, n_sets, layout, s);
+  return run_rows<float, NORM, PAGED, QUANT>(q, n_sets, layout, s);
 }
 
 void set_rotary(RowsParams& p, const lunarad_rotary_table& r) {
@@ -573,53 +614,39 @@ RowSet view_set(const lunarad_view& in, const lunarad_view& out, const void* wei
   return s;
 }
 
-template <typename T>
-cudaError_t run_quant(QuantParams q, int n_sets, int layout, cudaStream_t s) {
-  RowsParams& p = q.r;
+template <typename T, bool E2M1>
+cudaError_t run_read(ReadParams p, cudaStream_t s) {
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;
-  q.blocks = p.dim / 16;
-  p.lanes_log2 = log2_ceil(q.blocks);
-  const int per_block = kThreads >> p.lanes_log2;
-  set_groups(p, n_sets, 1);
-  const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, per_block)), p.group_end[2]);
-  bool vec = p.rot % 16 == 0;
-  const int64_t e = 16 / sizeof(T);
-  for (int i = 0; i < n_sets; ++i) {
-    const RowSet& r = p.set[i];
-    vec = vec && al16(r.src) && r.sh % e == 0 && r.ss % e == 0;
-    if (!r.paged) vec = vec && al16(r.dst) && r.dh % e == 0 && r.ds % e == 0;
-  }
-  return vec ? launch_pdl(append_e2m1_kernel<T, true>, grid, dim3(kThreads), 0, s, q, layout)
-             : launch_pdl(append_e2m1_kernel<T, false>, grid, dim3(kThreads), 0, s, q, layout);
-}
-
-template <typename T>
-cudaError_t run_read(ReadParams p, bool e2m1, cudaStream_t s) {
-  p.err = device_error_word();
-  if (p.err == nullptr) return cudaErrorInvalidDevice;
-  p.units = (p.dim + 15) / 16;
-  p.lanes_log2 = log2_ceil(p.units);
-  if (p.lanes_log2 > 5) p.lanes_log2 = 5;
-  const int per_block = kThreads >> p.lanes_log2;
-  const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, per_block)), p.heads, 2);
   const int64_t e = 16 / sizeof(T);
   bool vec = p.dim % 16 == 0;
   for (int i = 0; i < 2; ++i) {
     vec = vec && al16(p.dst[i]);
-    if (!e2m1) vec = vec && al16(p.src[i]) && p.page_stride[i] % e == 0 && p.head_stride[i] % e == 0;
+    if (!E2M1) vec = vec && al16(p.src[i]) && p.page_stride[i] % e == 0 && p.head_stride[i] % e == 0;
   }
-  if (e2m1)
-    return vec ? launch_pdl(read_kernel<T, true, true>, grid, dim3(kThreads), 0, s, p)
-               : launch_pdl(read_kernel<T, true, false>, grid, dim3(kThreads), 0, s, p);
-  return vec ? launch_pdl(read_kernel<T, false, true>, grid, dim3(kThreads), 0, s, p)
-             : launch_pdl(read_kernel<T, false, false>, grid, dim3(kThreads), 0, s, p);
+  if (!vec) {
+    const dim3 grid(static_cast<unsigned>(ceil_div64(p.tokens, kThreads / 32)), p.heads, 2);
+    return launch_pdl(read_any_kernel<T, E2M1>, grid, dim3(kThreads), 0, s, p);
+  }
+  p.units = p.dim / 8;
+  p.lanes_log2 = log2_ceil(p.units);
+  if (p.lanes_log2 > 5) p.lanes_log2 = 5;
+  const unsigned gx = static_cast<unsigned>(ceil_div64(p.tokens, kThreads >> p.lanes_log2));
+  if (static_cast<int64_t>(gx) * p.heads * 2 <= int64_t{device_num_sms()} * 16)
+    return launch_pdl(read_kernel<T, E2M1, 1>, dim3(gx, p.heads, 2), dim3(kThreads), 0, s, p);
+  return launch_pdl(read_kernel<T, E2M1, kHeads>, dim3(gx, (p.heads + kHeads - 1) / kHeads, 2), dim3(kThreads), 0, s, p);
+}
+
+template <typename T>
+cudaError_t run_read_kind(const ReadParams& p, bool e2m1, cudaStream_t s) {
+  return e2m1 ? run_read<T, true>(p, s) : run_read<T, false>(p, s);
 }
 
 }  // namespace
 
 cudaError_t launch_rotary(const lunarad_rotary_args& a, cudaStream_t stream) {
-  RowsParams p{};
+  QuantParams q{};
+  RowsParams& p = q.r;
   p.set[0] = view_set(a.x, a.y, nullptr, a.heads);
   p.positions = a.positions;
   p.position_bytes = static_cast<int>(a.position_bytes);
@@ -629,11 +656,12 @@ cudaError_t launch_rotary(const lunarad_rotary_args& a, cudaStream_t stream) {
   p.tokens = static_cast<int>(a.batch * a.seq);
   p.seq = static_cast<int>(a.seq);
   p.inverse = a.inverse != 0;
-  return run_rows_dtype<false, false>(p, 1, static_cast<int>(a.rotary.layout), a.dtype, stream);
+  return run_rows_dtype<false, false, false>(q, 1, static_cast<int>(a.rotary.layout), a.dtype, stream);
 }
 
 cudaError_t launch_qk_norm_rotary(const lunarad_qk_norm_rotary_args& a, cudaStream_t stream) {
-  RowsParams p{};
+  QuantParams q{};
+  RowsParams& p = q.r;
   p.set[0] = view_set(a.q, a.q_out, a.q_weight, a.q_heads);
   p.set[1] = view_set(a.k, a.k_out, a.k_weight, a.k_heads);
   p.positions = a.positions;
@@ -644,7 +672,7 @@ cudaError_t launch_qk_norm_rotary(const lunarad_qk_norm_rotary_args& a, cudaStre
   p.tokens = static_cast<int>(a.batch * a.seq);
   p.seq = static_cast<int>(a.seq);
   p.eps = static_cast<float>(a.eps);
-  return run_rows_dtype<true, false>(p, 2, static_cast<int>(a.rotary.layout), a.dtype, stream);
+  return run_rows_dtype<true, false, false>(q, 2, static_cast<int>(a.rotary.layout), a.dtype, stream);
 }
 
 cudaError_t launch_kv_append(const lunarad_kv_append_args& a, cudaStream_t stream) {
@@ -684,10 +712,8 @@ cudaError_t launch_kv_append(const lunarad_kv_append_args& a, cudaStream_t strea
   p.tokens = static_cast<int>(a.seqs.tokens);
   p.seq = p.tokens;
   const int layout = static_cast<int>(a.rotary.layout);
-  if (!e2m1) return run_rows_dtype<false, true>(p, n, layout, a.dtype, stream);
-  if (a.dtype == LUNARA_F16) return run_quant<__half>(q, n, layout, stream);
-  if (a.dtype == LUNARA_BF16) return run_quant<__nv_bfloat16>(q, n, layout, stream);
-  return run_quant<float>(q, n, layout, stream);
+  return e2m1 ? run_rows_dtype<false, true, true>(q, n, layout, a.dtype, stream)
+              : run_rows_dtype<false, true, false>(q, n, layout, a.dtype, stream);
 }
 
 cudaError_t launch_kv_read(const lunarad_kv_read_args& a, cudaStream_t stream) {
@@ -715,9 +741,9 @@ cudaError_t launch_kv_read(const lunarad_kv_read_args& a, cudaStream_t stream) {
   p.num_pages = static_cast<int>(c.num_pages);
   p.tokens = static_cast<int>(a.seqs.tokens);
   const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
-  if (a.dtype == LUNARA_F16) return run_read<__half>(p, e2m1, stream);
-  if (a.dtype == LUNARA_BF16) return run_read<__nv_bfloat16>(p, e2m1, stream);
-  return run_read<float>(p, e2m1, stream);
+  if (a.dtype == LUNARA_F16) return run_read_kind<__half>(p, e2m1, stream);
+  if (a.dtype == LUNARA_BF16) return run_read_kind<__nv_bfloat16>(p, e2m1, stream);
+  return run_read_kind<float>(p, e2m1, stream);
 }
 
 }  // namespace lunara

@@ -268,6 +268,11 @@ def test_kv_append(lens, heads, q_heads, dim, rot, page, layout, bits, dtype):
         assert torch.equal(now.view(torch.uint8), x.contiguous().view(torch.uint8)), name
     if q_heads:
         within(out_q, want_q, tol_q, "queries")
+        # In place: the same rows, those behind the last sequence untouched.
+        here = dev[:, :q_heads]
+        before = here[p.owned:].clone()
+        ops.kv_append(dev[:, q_heads:q_heads + heads], dev[:, q_heads + heads:], cache, *where(p), table=table, layout=layout, Q=here, out_q=here)
+        assert torch.equal(here[:p.owned], out_q[:p.owned]) and torch.equal(here[p.owned:], before)
     assert ops.device_error() == 0
 
 
