@@ -882,7 +882,7 @@ bool prefill_ok(const lunarad_paged_attention_args& a) {
   const lunarad_cache& c = *a.cache;
   const int64_t group = a.q_heads / c.kv_heads;
   const int64_t most = a.max_q_len > 0 && a.max_q_len < a.seqs.tokens ? a.max_q_len : a.seqs.tokens;   // tokens of a sequence
-  return stream_ok(a) && a.scale >= 0 && c.kind != LUNARAD_KIND_E2M1 && (c.dim == 64 || c.dim == 128) && most * group >= kPrefillRows;
+  return stream_ok(a) && a.scale >= 0 && c.kind != LUNARAD_KIND_E2M1 && most * group >= kPrefillRows;
 }
 
 int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {

@@ -193,8 +193,8 @@ inline unsigned join_blocks(int workers) {
   return static_cast<unsigned>(workers < few ? workers : need > few ? need : few);
 }
 
-// Many query rows per sequence (paged_prefill.cu): 16-bit caches with head
-// dimension 64 or 128.
+// Many query rows per sequence (paged_prefill.cu): 16-bit caches, head dimension
+// a multiple of 8 up to 128, scale not negative.
 int64_t paged_prefill_workspace(int dim, int sms);
 cudaError_t launch_paged_prefill(PagedParams p, int dtype, void* workspace, cudaStream_t stream);
 

@@ -53,6 +53,8 @@ constexpr int kPolyPairs = 4;            // of 16 exponential pairs on the FMA p
 constexpr int kMaskRing = 16;            // blocks whose key masks are kept; more than the ring can run ahead
 constexpr int kItemRing = 4;             // items whose block counts are kept; the copies run one item ahead at most
 
+// D: the head dimension rounded up to 64 or 128; columns behind it are zeros in
+// shared memory (TMA fills what lies outside the tensor) and are not stored.
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;                       // 64-element column blocks of a tile
@@ -351,13 +353,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int row = row0 + 32 * h + lane;
           const uint32_t use = __ballot_sync(0xffffffffu, row < rows);
           const int i = (row < rows ? row : 0) / p.group, head = x.kh * p.group + (row < rows ? row : 0) - i * p.group;
+          const bool in_row = 8 * chunk < p.dim;
           const char* src = static_cast<const char*>(p.q) + ((x.s.first + i) * p.q_tok + head * p.q_head) * 2;
           const uint32_t src_lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src)), src_hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src) >> 32);
 #pragma unroll 4
           for (int it = 0; it < 32 / kRowsAtOnce; ++it) {
             const int r = it * kRowsAtOnce + sub;
             const uint64_t at = (static_cast<uint64_t>(__shfl_sync(0xffffffffu, src_hi, r)) << 32) | __shfl_sync(0xffffffffu, src_lo, r);
-            copy16(dst + (32 * h + r) * 128 + (((chunk & 7) ^ (r & 7)) << 4), reinterpret_cast<const char*>(at) + 16 * chunk, ((use >> r) & 1u) != 0u);
+            copy16(dst + (32 * h + r) * 128 + (((chunk & 7) ^ (r & 7)) << 4), reinterpret_cast<const char*>(at) + (in_row ? 16 * chunk : 0),
+                   ((use >> r) & 1u) != 0u && in_row);
           }
         }
       }
@@ -403,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           filled |= 1u << slot;
           filled_phase = (filled_phase & ~(1u << slot)) | (phase << slot);
         } else {
-          const char* base = static_cast<const char*>(kv == 0 ? p.k : p.v) + x.kh * (kv == 0 ? p.k_head : p.v_head) * 2 + 16 * chunk;
+          const bool in_row = 8 * chunk < p.dim;
+          const char* base = static_cast<const char*>(kv == 0 ? p.k : p.v) + x.kh * (kv == 0 ? p.k_head : p.v_head) * 2 + (in_row ? 16 * chunk : 0);
 #pragma unroll 1
           for (int h = 0; h < 4; ++h) {
             const int key = key0 + 32 * h + lane;
@@ -418,7 +423,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int it = 0; it < 32 / kRowsAtOnce; ++it) {
               const int r = it * kRowsAtOnce + sub;
               const uint32_t row_at = __shfl_sync(0xffffffffu, at, r);
-              copy16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + static_cast<uint64_t>(row_at) * p.unit, ((use >> r) & 1u) != 0u);
+              copy16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + static_cast<uint64_t>(row_at) * p.unit,
+                     ((use >> r) & 1u) != 0u && in_row);
             }
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
@@ -678,7 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(ov[8 * q + e]) * f;
-              *reinterpret_cast<uint4*>(out + 32 * c + 8 * q) =
+              if (32 * c + 8 * q < p.dim)
+                *reinterpret_cast<uint4*>(out + 32 * c + 8 * q) =
                   make_uint4(Io<T>::pack2(v[0], v[1]), Io<T>::pack2(v[2], v[3]), Io<T>::pack2(v[4], v[5]), Io<T>::pack2(v[6], v[7]));
             }
           } else {
@@ -778,17 +785,17 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
 }  // namespace
 
 int64_t paged_prefill_workspace(int dim, int sms) {
-  return int64_t{2} * sms * kItemRows * (dim + 2) * static_cast<int64_t>(sizeof(float)) + sms * static_cast<int64_t>(sizeof(Cut));
+  return int64_t{2} * sms * kItemRows * ((dim <= 64 ? 64 : 128) + 2) * static_cast<int64_t>(sizeof(float)) + sms * static_cast<int64_t>(sizeof(Cut));
 }
 
 cudaError_t launch_paged_prefill(PagedParams p, int dtype, void* workspace, cudaStream_t stream) {
   p.workers = device_num_sms();
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + int64_t{2} * p.workers * kItemRows * p.dim;
+  p.part_ml = p.part_o + int64_t{2} * p.workers * kItemRows * (p.dim <= 64 ? 64 : 128);
   p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * kItemRows * 2);
   if (dtype == LUNARA_BF16)
-    return p.dim == 64 ? run_prefill<__nv_bfloat16, 64>(p, stream) : run_prefill<__nv_bfloat16, 128>(p, stream);
-  return p.dim == 64 ? run_prefill<__half, 64>(p, stream) : run_prefill<__half, 128>(p, stream);
+    return p.dim <= 64 ? run_prefill<__nv_bfloat16, 64>(p, stream) : run_prefill<__nv_bfloat16, 128>(p, stream);
+  return p.dim <= 64 ? run_prefill<__half, 64>(p, stream) : run_prefill<__half, 128>(p, stream);
 }
 
 }  // namespace lunara

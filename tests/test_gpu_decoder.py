@@ -393,7 +393,8 @@ SEQS = {
     ("decode", 2, 1, 64, 16), ("decode", 2, 4, 128, 16), ("decode", 1, 8, 128, 64), ("decode", 1, 16, 64, 8),
     ("decode", 2, 3, 96, 24), ("mixed", 2, 4, 128, 16), ("mixed", 2, 2, 64, 1), ("mixed", 1, 7, 96, 32),
     ("mixed", 2, 1, 256, 16), ("mixed", 1, 20, 64, 16), ("mixed", 1, 2, 48, 16), ("long", 4, 8, 128, 128), ("long", 12, 1, 64, 16),
-    ("one", 1, 1, 64, 16), ("chunks", 2, 4, 128, 32), ("chunks", 3, 1, 64, 16), ("chunks", 1, 5, 128, 7),
+    ("one", 1, 1, 64, 16), ("chunks", 2, 4, 128, 32), ("chunks", 3, 1, 64, 16), ("chunks", 1, 5, 128, 7), ("chunks", 2, 4, 96, 16),
+    ("chunks", 1, 3, 32, 256), ("chunks", 2, 2, 64, 128), ("chunks", 2, 2, 128, 8),
 ])
 def test_paged_attention(lens, kv_heads, group, dim, page, bits, dtype):
     p = ref.Paged(SEQS[lens], kv_heads, dim, page, dtype, seed=dim + page + group, bits=bits, gain=0.5 if bits == 4 else 1.0,
