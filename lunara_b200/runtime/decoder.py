@@ -56,6 +56,9 @@ def _layout_code(layout: str) -> int:
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}") from None
 
 
+# These run on every call of a decode step, whose kernels take a few microseconds: each
+# tensor property is read once, and the messages are only made when they are needed.
+
 def _check_device(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
     """Index of the device that all the tensors are on."""
     assert like.is_cuda, "lunara kernels take CUDA tensors"
@@ -65,31 +68,48 @@ def _check_device(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
     return index
 
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _call(name: str, args: bytes, index: int, *more) -> None:
     """Run an entry point on the current stream of device `index`."""
-    if torch._C._cuda_getDevice() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return _call(name, args, index, *more)
-    rc = getattr(_lib.load(), name)(args, *more, torch._C._cuda_getCurrentRawStream(index))
+    rc = getattr(_lib.load(), name)(args, *more, _current_stream(index))
     if rc:
         _lib.check(rc)
 
 
-def _unit(t: torch.Tensor, name: str) -> None:
-    assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs a unit inner stride"
+def _rows(t: torch.Tensor, name: str):
+    """(lunarad_view, (batch, heads, seq, dim)) of [B, H, S, D] or [tokens, H, D]."""
+    shape, st = t.shape, t.stride()
+    if len(shape) == 4:
+        batch, heads, seq, dim = shape
+        view = (t.data_ptr(), st[0], st[1], st[2])
+    else:
+        assert len(shape) == 3, f"{name} must be [B, H, S, D] or [tokens, H, D]"
+        batch, (seq, heads, dim) = 1, shape
+        view = (t.data_ptr(), 0, st[1], st[0])
+    assert st[-1] == 1 or dim <= 1, f"{name} needs a unit inner stride"
+    return view, (batch, heads, seq, dim)
 
 
-def _view(t: torch.Tensor) -> Tuple[int, int, int, int]:
-    """lunarad_view of [batch, heads, seq, dim], or of [tokens, heads, dim]."""
-    st = t.stride()
-    if len(st) == 4:
-        return t.data_ptr(), st[0], st[1], st[2]
-    return t.data_ptr(), 0, st[1], st[0]
-
-
-def _writable(t: torch.Tensor, name: str) -> None:
-    for n, s in zip(t.shape, t.stride()):
-        assert s != 0 or n <= 1, f"{name} is an expanded view; it cannot be written"
+def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    """(output, its lunarad_view); a new one is dense, in the order of like's strides."""
+    if out is None:
+        out = torch.empty_like(like)
+        st = out.stride()
+        if st[-1] != 1:
+            out = torch.empty_like(like, memory_format=torch.contiguous_format)
+            st = out.stride()
+    else:
+        assert out.shape == like.shape and out.dtype == like.dtype, f"{name} must be {tuple(like.shape)} {like.dtype}"
+        st = out.stride()
+        assert st[-1] == 1 or out.shape[-1] <= 1, f"{name} needs a unit inner stride"
+        assert 0 not in st or all(s != 0 or n <= 1 for n, s in zip(out.shape, st)), \
+            f"{name} is an expanded view; it cannot be written"
+    return out, (out.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (out.data_ptr(), 0, st[1], st[0])
 
 
 # ───────────────────────────────────────────────────────────── rotary ──
@@ -149,46 +169,25 @@ def _table(table: Optional[torch.Tensor], dim: int, layout: str) -> Tuple[int, i
     code = _layout_code(layout)
     if table is None:
         return 0, 0, 0, code
-    assert table.dim() == 3 and table.shape[2] == 2 and table.dtype == torch.float32 and table.is_contiguous(), \
+    shape = table.shape
+    assert len(shape) == 3 and shape[2] == 2 and table.dtype is torch.float32 and table.is_contiguous(), \
         "table must be a contiguous float32 [positions, rot_dim / 2, 2] (rotary_table)"
-    rot = 2 * table.shape[1]
+    rot = 2 * shape[1]
     assert rot <= dim, f"the table rotates {rot} elements of a head of {dim}"
-    return table.data_ptr(), table.shape[0], rot, code
+    return table.data_ptr(), shape[0], rot, code
 
 
 def _positions(positions: torch.Tensor, batch: int, seq: int, rank: int) -> Tuple[int, int, int]:
-    if positions.dtype == torch.int64:
-        size = 8
-    else:
-        assert positions.dtype == torch.int32, "positions must be int32 or int64"
-        size = 4
-    shape = positions.shape
+    dtype, shape, st = positions.dtype, positions.shape, positions.stride()
+    assert dtype is torch.int64 or dtype is torch.int32, "positions must be int32 or int64"
     if len(shape) == 1:
         assert shape[0] == seq, f"positions must be [{seq}], got {tuple(shape)}"
         stride = 0
     else:
         assert rank == 4 and shape == (batch, seq), f"positions must be [{seq}] or [{batch}, {seq}], got {tuple(shape)}"
-        stride = positions.stride(0)
-    assert positions.stride(-1) == 1 or seq <= 1, "positions need a unit inner stride"
-    return positions.data_ptr(), size, stride
-
-
-def _dense(x: torch.Tensor, name: str) -> Tuple[int, int, int, int]:
-    """(batch, heads, seq, dim) of [B, H, S, D] or [tokens, H, D]."""
-    assert x.dim() in (3, 4), f"{name} must be [B, H, S, D] or [tokens, H, D]"
-    _unit(x, name)
-    s = x.shape
-    return (s[0], s[1], s[2], s[3]) if len(s) == 4 else (1, s[1], s[0], s[2])
-
-
-def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
-    if out is None:
-        out = torch.empty_like(like)   # dense, in the order of like's strides
-        return out if out.stride(-1) == 1 else torch.empty_like(like, memory_format=torch.contiguous_format)
-    assert out.shape == like.shape and out.dtype == like.dtype, f"{name} must be {tuple(like.shape)} {like.dtype}"
-    _unit(out, name)
-    _writable(out, name)
-    return out
+        stride = st[0]
+    assert st[-1] == 1 or seq <= 1, "positions need a unit inner stride"
+    return positions.data_ptr(), 8 if dtype is torch.int64 else 4, stride
 
 
 def rotary(X: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, layout: str = "half",
@@ -201,22 +200,21 @@ def rotary(X: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, layout
     ``positions`` int32 or int64, [S] or [B, S] ([tokens] for a 3-D X). ``out`` may be X.
     ``inverse`` turns back (the gradient). A position outside the table records a device
     error and its row is zero-filled."""
-    batch, heads, seq, dim = _dense(X, "X")
-    rot = _table(table, dim, layout)
+    x, sizes = _rows(X, "X")
+    rot = _table(table, sizes[3], layout)
     assert table is not None, "rotary needs a table"
-    pos = _positions(positions, batch, seq, X.dim())
+    pos = _positions(positions, sizes[0], sizes[2], X.dim())
     code = _dtype_code(X)
     device = _check_device(X, positions, table, out)
-    out = _output(out, X, "out")
-    _call("lunarad_rotary", _ROTARY.pack(*_view(X), *_view(out), *pos, *rot, batch, heads, seq, dim, 1 if inverse else 0,
-                                         code), device)
+    out, y = _output(out, X, "out")
+    _call("lunarad_rotary", _ROTARY.pack(*x, *y, *pos, *rot, *sizes, 1 if inverse else 0, code), device)
     return out
 
 
 def _weight(w: Optional[torch.Tensor], like: torch.Tensor, dim: int, name: str) -> int:
     if w is None:
         return 0
-    assert w.shape == (dim,) and w.dtype == like.dtype and w.is_contiguous(), f"{name} must be [{dim}] {like.dtype}, contiguous"
+    assert w.dim() == 1 and w.numel() == dim and w.dtype is like.dtype and w.is_contiguous(), f"{name} must be [{dim}] {like.dtype}, contiguous"
     return w.data_ptr()
 
 
@@ -228,18 +226,20 @@ def qk_norm_rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, ta
     one launch. Q [B, Hq, S, D] and K [B, Hk, S, D], or [tokens, H, D], any strides (views of a
     fused projection); weights [D] or None; ``table=None`` normalises only. Statistics and
     rotation in fp32, one rounding. Outputs may be the inputs."""
-    batch, q_heads, seq, dim = _dense(Q, "Q")
-    kb, k_heads, ks, kd = _dense(K, "K")
-    assert K.dim() == Q.dim() and (kb, ks, kd) == (batch, seq, dim), "Q and K must agree in batch, positions and head dim"
-    assert Q.dtype == K.dtype, "Q and K must share a dtype"
+    q, (batch, q_heads, seq, dim) = _rows(Q, "Q")
+    k, (kb, k_heads, ks, kd) = _rows(K, "K")
+    rank = Q.dim()
+    assert kb == batch and ks == seq and kd == dim and K.dim() == rank, "Q and K must agree in batch, positions and head dim"
+    assert Q.dtype is K.dtype, "Q and K must share a dtype"
     rot = _table(table, dim, layout)
-    pos = _positions(positions, batch, seq, Q.dim())
+    pos = _positions(positions, batch, seq, rank)
     code = _dtype_code(Q)
     device = _check_device(Q, K, positions, table, q_weight, k_weight, out_q, out_k)
     wq, wk = _weight(q_weight, Q, dim, "q_weight"), _weight(k_weight, Q, dim, "k_weight")
-    out_q, out_k = _output(out_q, Q, "out_q"), _output(out_k, K, "out_k")
-    _call("lunarad_qk_norm_rotary", _QK_NORM.pack(*_view(Q), *_view(K), *_view(out_q), *_view(out_k), wq, wk, *pos, *rot, batch,
-                                                  q_heads, k_heads, seq, dim, code, eps), device)
+    out_q, oq = _output(out_q, Q, "out_q")
+    out_k, ok = _output(out_k, K, "out_k")
+    _call("lunarad_qk_norm_rotary", _QK_NORM.pack(*q, *k, *oq, *ok, wq, wk, *pos, *rot, batch, q_heads, k_heads, seq, dim, code,
+                                                  eps), device)
     return out_q, out_k
 
 
@@ -247,12 +247,12 @@ def qk_norm_rotary(Q: torch.Tensor, K: torch.Tensor, positions: torch.Tensor, ta
 
 def _sequences(page_table: torch.Tensor, seq_starts: torch.Tensor, seq_lens: torch.Tensor, tokens: int) -> Tuple[int, ...]:
     shape, stride = page_table.shape, page_table.stride()
-    batch = seq_lens.shape[0]
+    batch = seq_lens.numel()
     assert len(shape) == 2 and shape[0] == batch and seq_lens.dim() == 1, "page_table must be [batch, max_pages] and seq_lens [batch]"
-    assert seq_starts.shape == (batch + 1,), f"seq_starts must be [{batch + 1}], got {tuple(seq_starts.shape)}"
+    assert seq_starts.dim() == 1 and seq_starts.numel() == batch + 1, f"seq_starts must be [{batch + 1}], got {tuple(seq_starts.shape)}"
     i32 = torch.int32
     assert page_table.dtype is i32 and seq_starts.dtype is i32 and seq_lens.dtype is i32, "page_table, seq_starts and seq_lens must be int32"
-    assert (stride[1] == 1 or shape[1] <= 1) and (seq_lens.stride(0) == 1 or batch <= 1) and (seq_starts.stride(0) == 1 or batch < 1), \
+    assert (stride[1] == 1 or shape[1] <= 1) and seq_lens.is_contiguous() and seq_starts.is_contiguous(), \
         "page_table, seq_starts and seq_lens need a unit inner stride"
     return page_table.data_ptr(), seq_starts.data_ptr(), seq_lens.data_ptr(), stride[0], shape[1], batch, tokens
 
@@ -266,29 +266,25 @@ def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table:
     count the new tokens. A 4-bit cache gets the e2m1 codes and e4m3 scales of the values times
     ``1 / gain``. Two tokens of one call must not share a slot (sequences may share pages that
     nobody writes to)."""
-    tokens = K.shape[0]
-    dim = cache.head_dim
-    assert K.shape == (tokens, cache.kv_heads, dim) and V.shape == K.shape, \
-        f"K and V must be [tokens, {cache.kv_heads}, {dim}], got {tuple(K.shape)} and {tuple(V.shape)}"
-    assert V.dtype == K.dtype and (cache.dtype is None or K.dtype == cache.dtype), "K, V and the cache must share a dtype"
-    _unit(K, "K")
-    _unit(V, "V")
+    k, (_, heads, tokens, dim) = _rows(K, "K")
+    v, v_sizes = _rows(V, "V")
+    assert K.dim() == 3 and V.dim() == 3 and heads == cache.kv_heads and dim == cache.head_dim and v_sizes == (1, heads, tokens, dim), \
+        f"K and V must be [tokens, {cache.kv_heads}, {cache.head_dim}], got {tuple(K.shape)} and {tuple(V.shape)}"
+    dtype = K.dtype
+    assert V.dtype is dtype and (cache.dtype is None or dtype is cache.dtype), "K, V and the cache must share a dtype"
     rot = _table(table, dim, layout)
     code = _dtype_code(K)
     q_heads, q, o = 0, (0, 0, 0, 0), (0, 0, 0, 0)
     if Q is not None:
-        assert Q.dim() == 3 and Q.shape[0] == tokens and Q.shape[2] == dim and Q.dtype == K.dtype, \
-            f"Q must be [{tokens}, q_heads, {dim}] {K.dtype}"
-        _unit(Q, "Q")
-        q_heads = Q.shape[1]
+        q, (_, q_heads, q_tokens, q_dim) = _rows(Q, "Q")
+        assert Q.dim() == 3 and q_tokens == tokens and q_dim == dim and Q.dtype is dtype, f"Q must be [{tokens}, q_heads, {dim}] {dtype}"
     else:
         assert out_q is None, "out_q without Q"
     seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
     device = _check_device(cache.k_pages, K, V, table, Q, out_q, page_table, seq_starts, seq_lens)
     if Q is not None:
-        out_q = _output(out_q, Q, "out_q")
-        q, o = _view(Q), _view(out_q)
-    _call("lunarad_kv_append", _APPEND.pack(*_view(K), *_view(V), *q, *o, cache._address, *seqs, *rot, q_heads, code), device)
+        out_q, o = _output(out_q, Q, "out_q")
+    _call("lunarad_kv_append", _APPEND.pack(*k, *v, *q, *o, cache._address, *seqs, *rot, q_heads, code), device)
     return out_q
 
 
@@ -303,7 +299,7 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Ten
     assert tokens >= 0, "tokens must not be negative"
     seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
     device = _check_device(cache.k_pages, page_table, seq_starts, seq_lens)
-    k = torch.empty((tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    k = cache.k_pages.new_empty((tokens, cache.kv_heads, cache.head_dim), dtype=dtype)
     v = torch.empty_like(k)
     _call("lunarad_kv_read", _READ.pack(k.data_ptr(), v.data_ptr(), cache._address, *seqs, _dtype_code(k)), device)
     return k, v
@@ -319,18 +315,17 @@ def paged_attention(Q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     head h reads key head ``h // (q_heads // kv_heads)``. ``scale`` defaults to ``1 / sqrt(D)``.
     fp32 softmax; a row that sees no key is zero. ``max_q_len``, the most tokens any sequence
     has here, is a hint that steers the choice of kernels (default: any number)."""
-    assert Q.dim() == 3 and Q.shape[2] == cache.head_dim, f"Q must be [tokens, q_heads, {cache.head_dim}], got {tuple(Q.shape)}"
-    tokens, q_heads, dim = Q.shape
-    assert cache.dtype is None or Q.dtype == cache.dtype, "Q and the cache must share a dtype"
+    q, (_, q_heads, tokens, dim) = _rows(Q, "Q")
+    assert Q.dim() == 3 and dim == cache.head_dim, f"Q must be [tokens, q_heads, {cache.head_dim}], got {tuple(Q.shape)}"
+    assert cache.dtype is None or Q.dtype is cache.dtype, "Q and the cache must share a dtype"
     assert q_heads > 0 and q_heads % cache.kv_heads == 0, f"{q_heads} query heads are no multiple of {cache.kv_heads} key heads"
-    _unit(Q, "Q")
     code = _dtype_code(Q)
     seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
     device = _check_device(cache.k_pages, Q, out, page_table, seq_starts, seq_lens)
-    out = _output(out, Q, "out")
+    out, o = _output(out, Q, "out")
     if scale is None:
         scale = dim ** -0.5
-    args = _ATTENTION.pack(*_view(Q), *_view(out), cache._address, *seqs, q_heads, window, max_q_len or 0, code, scale)
+    args = _ATTENTION.pack(*q, *o, cache._address, *seqs, q_heads, window, max_q_len or 0, code, scale)
     need = _lib.load().lunarad_paged_attention_workspace(args, device)
     if need < 0:
         _lib.check(-need)
