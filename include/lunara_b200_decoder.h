@@ -157,7 +157,11 @@ int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream);
  * them). Q and O [tokens, q_heads, dim] (head_stride, seq_stride); query head h
  * reads key head h / (q_heads / kv_heads). fp32 softmax and sums, one rounding
  * of O (16-bit products round the probabilities to the query dtype as
- * well). A row that sees no key is zero. Keys of a page outside the cache
+ * well; with an e2m1 cache the products are f16). A row that sees no key, or
+ * whose scores are all -inf, is zero. What the cache holds behind a sequence's
+ * end, in other pages and outside every row's window has no influence, NaN
+ * included. A value (not a key) that is not finite and that only some of the
+ * call's tokens of a sequence see may also reach those that do not. Keys of a page outside the cache
  * (0x502) are left out, and a length outside the page table (0x503) is cut.
  * max_q_len: the longest sequence's number of tokens if known (0 = unknown);
  * it only steers the choice of kernels.

@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           copy_async(at + S::kKBytes + v_place<S, true>(local, piece), place(vl, va), in);
         }
         // The scales of a group of 8 keys are srow / 2 pieces of 16 bytes. A
-        // group with a masked key is copied whole; see clear_scales below.
+        // group with a masked key is copied whole; V's are cleared below.
         constexpr int kScalePieces = DP / 32, kAll = 2 * (KT / 8) * kScalePieces;
         const int kv = lane / (kAll / 2), rest = lane % (kAll / 2), grp = rest / kScalePieces, sp = rest % kScalePieces;
         const uint32_t ka = __shfl_sync(0xffffffffu, ks_at, g0 + grp), va = __shfl_sync(0xffffffffu, vs_at, g0 + grp);
@@ -502,9 +502,9 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // Times 2^-e for 2^e <= top < 2^(e + 1), and the scores times 2^e;
-        // rows of zeros and rows at fp32's ends stay as they are.
+        // rows of zeros or subnormals and rows at fp32's upper end stay as they are.
         const uint32_t e = __float_as_uint(top) >> 23;
-        const bool use = e > 64u && e < 190u;
+        const bool use = e > 0u && e < 254u;
         const float down = use ? __uint_as_float((254u - e) << 23) : 1.f;
         up = use ? __uint_as_float(e << 23) : 1.f;
 #pragma unroll
@@ -530,7 +530,11 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
       for (int j = 0; j < kMTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
-    float m[NT][2], l[NT][2];   // per column: maximum (scaled, log2), and this lane's part of the sum
+    // Per column: maximum of the unscaled scores, and this lane's part of the sum.
+    // Exponents are (score - maximum) * factor, so the largest is exactly 0
+    // however large the scores are (score * factor - maximum * factor in one FMA
+    // is off by the rounding of the maximum's product).
+    float m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -650,8 +654,8 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
             x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmax_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            top[n][r] = x * sl2[n][r];
-            grown |= !(top[n][r] <= m[n][r] + kRescaleLog2);
+            top[n][r] = x;
+            grown |= !((x - m[n][r]) * sl2[n][r] <= kRescaleLog2);   // (true for NaN, and while a row has seen no key)
           }
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -659,7 +663,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const float next = fmax_nan(m[n][r], top[n][r]);
-              const float alpha = next == -INFINITY ? 1.f : ex2_approx(m[n][r] - next);
+              const float alpha = next == -INFINITY ? 1.f : ex2_approx((m[n][r] - next) * sl2[n][r]);
               m[n][r] = next;
               l[n][r] *= alpha;
 #pragma unroll
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           for (int a = 0; a < KT / 16; ++a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              sc[n][a][e] = ex2_approx(fmaf(sc[n][a][e], sl2[n][e & 1], (e & 1) == 0 ? -off0 : -off1));
+              sc[n][a][e] = ex2_approx((sc[n][a][e] - ((e & 1) == 0 ? off0 : off1)) * sl2[n][e & 1]);
             l[n][0] += sc[n][a][0] + sc[n][a][2];
             l[n][1] += sc[n][a][1] + sc[n][a][3];
             pf[n][a][0] = transpose8x8(Io<M>::pack2(sc[n][a][0], sc[n][a][1]));
@@ -799,7 +803,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
               }
             }
           if (!whole && g == 0)
-            *reinterpret_cast<float2*>(p.part_ml + (part * S::kRows + in_tile) * 2) = make_float2(m[n][r], l[n][r]);
+            *reinterpret_cast<float2*>(p.part_ml + (part * S::kRows + in_tile) * 2) = make_float2(m[n][r] * sl2[n][r], l[n][r]);
         }
       }
     t += n_tiles;
@@ -829,8 +833,9 @@ int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
 
 // 8-row tiles that share the keys: one where a sequence is likely to have no
 // more than 8 query rows (by the caller's hint, else by the mean), two else. With
-// one the products, exponentials and accumulators are half as many (four
-// 131072-key 4-bit contexts of 4 rows: @NT1@ us, with two @NT2@).
+// one the products, exponentials and accumulators are half as many, and 16
+// instead of 12 warps fit an SM with 4 bits (four 131072-key 4-bit contexts of 4
+// rows: 155 us with two, 132 with one when the change was made).
 int row_tiles_of(const lunarad_paged_attention_args& a) {
   const int64_t mean = (a.seqs.tokens + a.seqs.batch - 1) / a.seqs.batch;
   return (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / a.cache->kv_heads) <= 8 ? 1 : 2;

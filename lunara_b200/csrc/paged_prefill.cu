@@ -311,9 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int worker = static_cast<int>(blockIdx.x);
   int64_t t_first = 0, t_end = 0;
   clear_empty<T>(p);
-  if (worker >= workers) {
-    if (threadIdx.x == 0) p.cuts[worker].parts = 0;
-  } else {
+  if (threadIdx.x == 0) p.cuts[worker].parts = 0;   // until the run's end says otherwise
+  if (worker < workers) {
     t_first = run_start(total, workers, worker);
     t_end = run_start(total, workers, worker + 1);
     if (threadIdx.x == 0) s_cursor.seek(p, prefix, t_first);
@@ -550,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int lo, hi;
       visible(p, x.s.pos0 + i, lo, hi);
       const int n = x.n, block0 = x.block0;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;   // maximum (scaled, log2) and sum
+      float top = -INFINITY;          // the score that gave the maximum
       for (int j = 0; j < n; ++j, ++blocks) {
         if (!mbar_wait_warp(&s_full[w], blocks & 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
         tc_fence_after();
@@ -590,12 +590,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float cand = mx * sl2;
         if (j == 0) {
           m = cand;
+          top = mx;
         } else if (__any_sync(0xffffffffu, !(cand <= m + kRescaleLog2))) {
           // O is rescaled once P V of the block before has completed (as it has:
           // S of this block ran after it).
           if (!mbar_wait_warp(&o_full[w], (blocks - 1) & 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
           tc_fence_after();
           const float next = fmax_nan(m, cand);
+          top = fmax_nan(top, mx);
           const float alpha = next == -INFINITY ? 1.f : ex2_approx(m - next);
           l *= alpha;
           m = next;
@@ -618,7 +620,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_32x32b_x16(tO + c * 16, ov);
           }
         }
-        const float off = m == -INFINITY ? 0.f : m;
+        float off = m == -INFINITY ? 0.f : m;
+        // score * factor - maximum in one FMA is off by the rounding of the
+        // maximum, 2^-24 of it: where that matters, the largest score is taken
+        // off the scores first.
+        if (__any_sync(0xffffffffu, fabsf(off) > 8192.f)) {
+          const float sub = off == 0.f ? 0.f : top;
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[cc][e] = __float_as_uint(__uint_as_float(sc[cc][e]) - sub);
+          off = 0.f;
+        }
         const uint64_t sl2x2 = f2_pack(sl2, sl2), neg2 = f2_pack(-off, -off);
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll

@@ -505,12 +505,25 @@ def test_paged_attention_bad_pages(lens, bits):
     assert ops.device_error() in (0x502, 0x503)
 
 
-def test_paged_attention_extreme_scores():
-    """Scores around +-60000 (bf16 values at their ends) neither overflow nor underflow the softmax."""
-    for bits in (16, 4):
-        p = ref.Paged([(1, 200), (4, 77)], 2, 128, 16, BF16, seed=13, bits=bits)
-        q = p.queries(4) * 600
-        check_attention(p, 4, q=q, what="extreme scores")
+@pytest.mark.parametrize("size", [600.0, 2.0 ** 100, 2.0 ** -80, 0.0])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lens", [[(1, 200), (4, 77)], [(64, 200), (150, 300)]])
+def test_paged_attention_extreme_scores(lens, bits, size):
+    """Scores far beyond the 16-bit ranges, and queries far below them, neither overflow nor lose the softmax."""
+    p = ref.Paged(lens, 2, 128, 16, BF16, seed=13, bits=bits)
+    q = p.queries(4) * size
+    if size == 2.0 ** 100:   # one-hot rows: a rounding of the score cannot change which key is the largest
+        ops = _ops()
+        cache, _ = cache_of(p)
+        out = ops.paged_attention(q.cuda(), cache, *where(p)).cpu().double()
+        at = 0
+        for b, (n, whole) in enumerate(p.lens):
+            k, v = p.seqs[b]
+            want = ref.attend(q[at:at + n], k, v, whole - n, 128 ** -0.5)[0]
+            assert ((out[at:at + n] - want).abs() <= half_step(BF16) * want.abs() + TINY).all()
+            at += n
+        return
+    check_attention(p, 4, q=q, what="extreme scores")
 
 
 @pytest.mark.parametrize("bits,dim", [(16, 64), (16, 128), (4, 128), (16, 20)])
