@@ -903,8 +903,8 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(kWarps) * S::kRingBytes + prefix;
   static_assert(kWarps * S::kRingBytes + 8 * (kMaxBatch + 2) + 1280 <= 228 * 1024 / S::kCtasPerSm, "shared memory per SM");
   auto kern = paged_stream_kernel<T, E2M1, DP, NT, EXACT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kWarps * S::kRingBytes + 8 * (kMaxBatch + 2));
+  static std::atomic<uint64_t> prepared{0};
+  cudaError_t e = prepare_once(kern, prepared, kWarps * S::kRingBytes + 8 * (kMaxBatch + 2), 0);
   if (e != cudaSuccess) return e;
   const int batch = p.seqs.batch;
   const Seqs all = p.seqs;

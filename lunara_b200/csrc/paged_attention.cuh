@@ -1,6 +1,8 @@
 // Parameters and helpers shared by the kernels of the paged attention.
 #pragma once
 
+#include <atomic>
+
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -191,6 +193,28 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 inline unsigned join_blocks(int workers) {
   const int few = 2 * device_num_sms(), need = (workers + 31) / 32;
   return static_cast<unsigned>(workers < few ? workers : need > few ? need : few);
+}
+
+// Prepares a kernel (its shared memory, and with regs > 0 a check that it was
+// built with that many registers) once per device: the calls cost a microsecond
+// or two, which a decode step would pay every time. `done` is the caller's, one
+// per kernel, a bit for each device.
+template <typename Kernel>
+cudaError_t prepare_once(Kernel kern, std::atomic<uint64_t>& done, int smem, int regs) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  if (regs > 0) {
+    cudaFuncAttributes fa{};
+    e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs != regs) return cudaErrorInvalidConfiguration;
+  }
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // Many query rows per sequence (paged_prefill.cu): 16-bit caches, head dimension

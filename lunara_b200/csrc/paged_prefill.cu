@@ -765,11 +765,8 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
   using L = Layout<D>;
   static_assert(L::kSmem + 1024 <= 227 * 1024 && 8 * (kMaxBatch + 1) <= L::kSlots * L::kSlotBytes, "shared memory");
   auto kern = paged_prefill_kernel<T, D>;
-  cudaFuncAttributes fa{};
-  cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-  if (e != cudaSuccess) return e;
-  if (fa.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;   // the setmaxnreg split counts on it
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+  static std::atomic<uint64_t> prepared{0};
+  cudaError_t e = prepare_once(kern, prepared, static_cast<int>(L::kSmem), kLaunchRegs);   // the setmaxnreg split counts on the registers
   if (e != cudaSuccess) return e;
   // TMA where pages tile a 128-key block in boxes of whole swizzle atoms (8
   // rows); row by row elsewhere (box_rows 0).

@@ -172,7 +172,9 @@ __device__ __forceinline__ float quotient(float y, float s, float r) {
 // keeps NaN), and the codes of N of its elements, 4 bits each.
 template <int N>
 __device__ __forceinline__ uint32_t quantise(const float (&y)[N], int first, float amax, uint32_t& scale) {
-  scale = float_to_e4m3(__fdiv_rn(amax, 6.0f));
+  // amax / 6 correctly rounded in the same way (beyond 1e30 it saturates anyway).
+  const float top = amax > 1e30f ? 1e30f : amax;
+  scale = float_to_e4m3(quotient(top, 6.0f, 1.0f / 6.0f));
   const float s = e4m3_to_float(scale);
   uint32_t w = 0u;
   if (s > 0.f) {

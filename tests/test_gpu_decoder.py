@@ -304,6 +304,29 @@ def test_kv_append_4bit_extremes():
         assert k[0, 0, 48:64].isnan().all() and not k[0, 0, 64:].isnan().any()
 
 
+def test_kv_append_4bit_every_scale():
+    """Blocks of every e4m3 scale and of the largest magnitudes around its rounding, elements around every code's ties."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(17)
+    scales = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    amax = torch.cat([scales * 6 * (1 + k * 2.0 ** -23) for k in (-1, 0, 1)] + [(scales[1:] + scales[:-1]) * 3 * (1 + k * 2.0 ** -23) for k in (-1, 0, 1)])
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]).repeat(2) * torch.tensor([1.0] * 7 + [-1.0] * 7)
+    x = torch.zeros(len(amax), 16)
+    x[:, 0] = amax
+    s = ref.quantise(x, 1.0)[1].view(torch.float8_e4m3fn).float()
+    x[:, 1:15] = ties * s * (1 + torch.randint(-2, 3, (len(amax), 14), generator=g) * 2.0 ** -23)
+    x[:, 15] = torch.randn(len(amax), generator=g) * amax / 3
+    x = torch.nn.functional.pad(x, (0, 0, 0, (-len(x)) % 4)).view(-1, 1, 64)
+    n = len(x)
+    cache = ops.PagedKVCache.allocate((n + 7) // 8, 1, 8, 64, dtype="e2m1")
+    tab = torch.arange((n + 7) // 8, dtype=torch.int32, device="cuda")[None]
+    starts, lens = torch.tensor([0, n], dtype=torch.int32, device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda")
+    ops.kv_append(x.cuda(), x.cuda(), cache, tab, starts, lens)
+    codes, scale_bytes = ref.quantise(x, 1.0)
+    assert torch.equal(cache.k_pages.view(-1, 32)[:n].cpu(), ref.pack(codes)[:, 0])
+    assert torch.equal(cache.v_scales.view(torch.uint8).view(-1, 4)[:n].cpu(), scale_bytes[:, 0])
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("heads,dim,page", [(2, 128, 16), (3, 64, 1), (1, 96, 24), (2, 48, 7), (2, 1024, 4)])
