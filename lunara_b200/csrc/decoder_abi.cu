@@ -116,8 +116,8 @@ int check_attention(const char* fn, const lunarad_paged_attention_args* a) {
   if (a->q_heads > kMaxHeads || a->seqs.tokens * a->q_heads >= kMaxSlots)
     return fail(LUNARA_ERR_UNSUPPORTED, "%s: more than 65535 heads or 2^31 query rows", fn);
   if (c.dim > 256) return fail(LUNARA_ERR_UNSUPPORTED, "%s: head dim %lld > 256", fn, (long long)c.dim);
-  if (c.page_size * a->seqs.max_pages >= kMaxSlots)
-    return fail(LUNARA_ERR_UNSUPPORTED, "%s: page table covers 2^31 positions or more", fn);
+  if (c.page_size * a->seqs.max_pages >= kMaxSlots - 4096)   // (the kernels look a batch of keys ahead)
+    return fail(LUNARA_ERR_UNSUPPORTED, "%s: page table covers nearly 2^31 positions or more", fn);
   if (a->window < 0 || a->window >= kMaxSlots) return fail(LUNARA_ERR_INVALID_ARG, "%s: bad window", fn);
   if (a->max_q_len < 0) return fail(LUNARA_ERR_INVALID_ARG, "%s: negative max_q_len", fn);
   if (!std::isfinite(a->scale)) return fail(LUNARA_ERR_INVALID_ARG, "%s: scale is not finite", fn);

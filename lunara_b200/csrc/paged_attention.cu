@@ -4,20 +4,23 @@
 //   query's position sees: j <= p, and with a window j > p - window.
 //
 // Streaming kernel (16-bit and 4-bit caches): the query rows of one sequence
-// and key head (its tokens times the query heads of the group) make tiles of
+// and key head (its tokens times the query heads of the group) make tiles of 8 or
 // 16 rows; their keys are cut into tiles of KT, and all tiles of the batch, in
 // the order (sequence, key head, row tile, key tile), are dealt to the warps of
 // a persistent grid in equal contiguous runs. Bound by HBM: a decode step reads
-// each cached byte once for group * 4 operations per element.
+// each cached byte once for group * 4 operations per element. Measured on B200:
+// 64 sequences of up to 8191 keys, 32/8 heads of 128 in bf16, 188 us for 1.18 GB
+// (6.3 TB/s); with 4 bits by issue slots: 438 MB of codes in 108 us (4.0 TB/s).
 //   * Every warp works alone (no block barrier after the start): it copies its
 //     tiles with cp.async into a ring of its own in shared memory. The order of
-//     the head dimension inside Q K^T and of the columns of V inside P V is
-//     free; it is chosen so that a lane's mma fragments are contiguous in
-//     memory, and no ldmatrix is needed.
-//   * S = Q K^T and O += P V by mma.sync m16n8k16 with fp32 accumulators. At
-//     16 rows these products need a fraction of the legacy tensor rate while
-//     HBM delivers its 23 bytes per clock and SM; tcgen05 needs 64 rows or more
-//     (paged_prefill.cu takes those).
+//     the head dimension inside the scores and of the columns of V is free; it is
+//     chosen so that a lane's mma fragments are contiguous in memory, and no
+//     ldmatrix is needed.
+//   * S^T = K Q^T and O^T += V^T P^T by mma.sync m16n8k16 with fp32 accumulators:
+//     keys and elements fill the 16 rows of an instruction, so that 8 query rows
+//     fill the rest. These products need a fraction of the legacy tensor rate
+//     while HBM delivers its 23 bytes per clock and SM; where there are enough
+//     rows for tcgen05, paged_prefill.cu takes them.
 //   * The running maximum is raised only when a row's maximum grows by more
 //     than 2^8 (a warp vote), so O is rescaled a few times per row in all.
 //   * 4-bit caches: codes become f16 pairs by one cvt per pair, times their
@@ -831,14 +834,23 @@ cudaError_t run_simple(const PagedParams& p, cudaStream_t s) {
 
 int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
 
-// 8-row tiles that share the keys: one where a sequence is likely to have no
-// more than 8 query rows (by the caller's hint, else by the mean), two else. With
-// one the products, exponentials and accumulators are half as many, and 16
-// instead of 12 warps fit an SM with 4 bits (four 131072-key 4-bit contexts of 4
-// rows: 155 us with two, 132 with one when the change was made).
+// 8-row tiles that share the keys, by the likely query rows of a sequence (the
+// caller's hint, else the mean). One tile needs half the accumulators and
+// exponentials and leaves room for more warps, two read the keys once for 16 rows.
+// With 4 bits each key is converted again for every row tile, so two pay from 9
+// rows on (four 131072-key contexts of 4 rows: 155 us with two, 132 with one). With
+// 16 bits they pay from 17 rows on where the second reading comes from L2 (8 x 4096
+// keys, 8 key heads of 128, 134 MB: 16 rows 42 us with one, 54 with two; 32 rows 64
+// and 57), and from 9 on in larger caches (32 sequences of up to 4096 keys, at most
+// 537 MB: 16 rows 98 and 89; 2 x 32768 keys, 268 MB: 108 and 109, 32 rows 183 and
+// 106). The page table bounds the size.
 int row_tiles_of(const lunarad_paged_attention_args& a) {
+  const lunarad_cache& c = *a.cache;
   const int64_t mean = (a.seqs.tokens + a.seqs.batch - 1) / a.seqs.batch;
-  return (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / a.cache->kv_heads) <= 8 ? 1 : 2;
+  const int64_t rows = (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / c.kv_heads);
+  const double bytes = 4.0 * static_cast<double>(c.kv_heads * c.dim) * static_cast<double>(c.page_size * a.seqs.max_pages) *
+                       static_cast<double>(a.seqs.batch);
+  return rows <= (c.kind != LUNARAD_KIND_E2M1 && bytes < 200e6 ? 16 : 8) ? 1 : 2;
 }
 int stream_workers(bool e2m1, int nt, int sms) { return sms * kWarps * ((e2m1 ? 3 : 2) + (nt == 1 ? 1 : 0)); }
 
@@ -880,8 +892,10 @@ bool stream_ok(const lunarad_paged_attention_args& a) {
 }
 
 // Sequences with this many query rows go to the tcgen05 kernel where it takes
-// the cache.
-constexpr int64_t kPrefillRows = 64;
+// the cache: there the streaming kernel would read the keys a third time (8 x 4096
+// keys, 8 key heads of 128: 32 rows 57 us streaming, 68 on tcgen05, 48 rows 73 and
+// 69; 2 x 32768 keys: 106 and 95, 165 and 96).
+constexpr int64_t kPrefillRows = 33;
 
 bool prefill_ok(const lunarad_paged_attention_args& a) {
   const lunarad_cache& c = *a.cache;
