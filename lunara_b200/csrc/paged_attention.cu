@@ -900,7 +900,11 @@ constexpr int64_t kPrefillRows = 33;
 bool prefill_ok(const lunarad_paged_attention_args& a) {
   const lunarad_cache& c = *a.cache;
   const int64_t group = a.q_heads / c.kv_heads;
-  const int64_t most = a.max_q_len > 0 && a.max_q_len < a.seqs.tokens ? a.max_q_len : a.seqs.tokens;   // tokens of a sequence
+  // Tokens of a sequence at most, as far as is known. No more tokens than
+  // sequences: a decode step, which the second pair of launches would cost 8 us
+  // (the streaming kernel is right for any sequence).
+  int64_t most = a.seqs.tokens <= a.seqs.batch ? 1 : a.seqs.tokens;
+  if (a.max_q_len > 0) most = a.max_q_len < a.seqs.tokens ? a.max_q_len : a.seqs.tokens;
   return stream_ok(a) && a.scale >= 0 && c.kind != LUNARAD_KIND_E2M1 && most * group >= kPrefillRows;
 }
 
