@@ -38,6 +38,7 @@
 
 #include "kernels.h"
 #include "paged_attention.cuh"
+#include "scale_copy.h"
 
 namespace lunara {
 namespace {
@@ -425,14 +426,13 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         }
         // The scales of a group of 8 keys are srow / 2 pieces of 16 bytes. A
         // group with a masked key is copied whole; V's are cleared below.
-        constexpr int kScalePieces = DP / 32, kAll = 2 * (KT / 8) * kScalePieces;
-        const int kv = lane / (kAll / 2), rest = lane % (kAll / 2), grp = rest / kScalePieces, sp = rest % kScalePieces;
-        const uint32_t ka = __shfl_sync(0xffffffffu, ks_at, g0 + grp), va = __shfl_sync(0xffffffffu, vs_at, g0 + grp);
-        if (lane < kAll) {
-          const bool in = ((ok >> (8 * grp)) & 0xFFu) != 0u && (EXACT || 2 * sp < srow);
-          const uint8_t* src = kv == 0 ? static_cast<const uint8_t*>(p.ks) + kh * p.ks_head + static_cast<uint64_t>(ka) * 16
-                                       : static_cast<const uint8_t*>(p.vs) + kh * p.vs_head + static_cast<uint64_t>(va) * 16;
-          copy_async(at + S::kKBytes + S::kVBytes + kv * S::kScaleBytes + grp * (8 * srow) + 16 * sp, src + 16 * sp, in);
+        const ScaleCopy sc = scale_copy<KT, DP>(lane, srow);
+        const uint32_t ka = __shfl_sync(0xffffffffu, ks_at, g0 + sc.group), va = __shfl_sync(0xffffffffu, vs_at, g0 + sc.group);
+        if (sc.copies) {
+          const bool in = ((ok >> (8 * sc.group)) & 0xFFu) != 0u;
+          const uint8_t* src = sc.kv == 0 ? static_cast<const uint8_t*>(p.ks) + kh * p.ks_head + static_cast<uint64_t>(ka) * 16
+                                          : static_cast<const uint8_t*>(p.vs) + kh * p.vs_head + static_cast<uint64_t>(va) * 16;
+          copy_async(at + S::kKBytes + S::kVBytes + sc.kv * S::kScaleBytes + sc.place, src + 16 * sc.piece, in);
         }
       } else {
         constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
