@@ -26,3 +26,24 @@ def test_4bit_scales_of_every_group(dim, page, heads, dtype):
             x = (torch.randn(whole, heads, dim // 16, 16, generator=p.g) * size).flatten(2).to(dtype)
             p.seqs[b][i] = p.put(name, b, torch.arange(whole), x)
     check_attention(p, 4 * heads)
+
+
+def test_kv_append_4bit_signs_of_zero():
+    """A negative zero keeps its sign in the code, as its quotient by the scale does; in a block of zeros there is no quotient."""
+    ops = _ops()
+    x = torch.randn(8, 2, 64, generator=torch.Generator().manual_seed(21))
+    x[:, :, ::3] = -0.0
+    x[:, :, 1::6] = 0.0
+    x[3] = -0.0
+    for dtype in (F32, F16, BF16):
+        for skip in (0, 1):   # 16-byte aligned rows, and others
+            flat = torch.zeros(x.numel() + 1, dtype=dtype, device="cuda")
+            rows = flat[skip:skip + x.numel()].view(8, 2, 64)
+            rows.copy_(x)
+            cache = ops.PagedKVCache.allocate(1, 2, 8, 64, dtype="e2m1")
+            tab, starts, lens = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0]], [0, 8], [8]))
+            ops.kv_append(rows, rows, cache, tab, starts, lens)
+            codes, scales = ref.quantise(x.to(dtype).float(), 1.0)
+            assert (codes == 8).any()
+            assert torch.equal(cache.k_pages[0].cpu(), ref.pack(codes).transpose(0, 1)), (dtype, skip)
+            assert torch.equal(cache.v_scales.view(torch.uint8)[0].cpu(), scales.transpose(0, 1))
