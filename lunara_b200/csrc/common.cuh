@@ -609,6 +609,12 @@ __device__ __forceinline__ uint64_t ex2_poly2_clamped(uint64_t x2) {
                  __uint_as_float(__float_as_uint(pv.y) + (__float_as_uint(tv.y) << 23)));
 }
 
+// What ex2_poly2_clamped gives at -126 and below: the cubic's constant term times
+// 2^-126, the smallest of its results.
+__device__ __forceinline__ float ex2_poly2_floor() {
+  return __uint_as_float(__float_as_uint(0.9999280572f) - (126u << 23));
+}
+
 // ex2_poly for a pair with MUFU's range behaviour (0 below -126, NaN kept).
 __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
   const float2 x = f2_unpack(x2);

@@ -651,7 +651,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 8; ++q) {
               const int pair = g0 + q;
               if (((pair * kPolyPairs) % 16) < kPolyPairs) {
+                // The cubic's result below -126, masked scores' too, is dropped by
+                // fp16's rounding. bf16 would hold it, and values may be as large
+                // (2^-126 of a finite 2^121 is 1/32): there it is taken off, which
+                // leaves exactly 0 and moves no other result by more than it.
                 e2[q] = ex2_poly2_clamped(x2[q]);
+                if constexpr (kBF16) e2[q] = f2_add(e2[q], f2_pack(-ex2_poly2_floor(), -ex2_poly2_floor()));
               } else {
                 const float2 v = f2_unpack(x2[q]);
                 e2[q] = f2_pack(ex2_approx(v.x), ex2_approx(v.y));
@@ -677,8 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       // ------------------------------------------------------------ results --
-      // A masked score adds 2^-126 at most (the cubic's smallest), which is
-      // nothing beside a row's largest, but the whole sum of a row that saw no
+      // With fp16 a masked score adds 2^-126 at most (the cubic's smallest), which
+      // is nothing beside a row's largest, but the whole sum of a row that saw no
       // key: such a row keeps its maximum of -inf.
       if (m == -INFINITY) l = 0.f;
       const bool whole = x.first == 0 && n == x.item_blocks;

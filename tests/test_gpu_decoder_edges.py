@@ -47,3 +47,34 @@ def test_kv_append_4bit_signs_of_zero():
             assert (codes == 8).any()
             assert torch.equal(cache.k_pages[0].cpu(), ref.pack(codes).transpose(0, 1)), (dtype, skip)
             assert torch.equal(cache.v_scales.view(torch.uint8)[0].cpu(), scales.transpose(0, 1))
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (80, 7)])
+@pytest.mark.parametrize("lens", [[(100, 100), (128, 128), (64, 128)], [(4, 100), (2, 128), (1, 100)]])
+def test_huge_values_behind_a_row_do_not_reach_it(lens, dim, page):
+    """Values of the order of 2^121 at the last ten positions, which only the last tokens see. (All keys stand in one block of
+    128, so probabilities before the division are at most 1, and ten such values stay below fp32's largest number.)"""
+    p = ref.Paged(lens, 2, dim, page, BF16, seed=dim + page)
+    for b, (_, whole) in enumerate(p.lens):
+        pos = torch.arange(whole - 10, whole)
+        x = (2.0 ** 121 * (1 + torch.rand(10, 2, dim, generator=p.g))).to(BF16)
+        p.seqs[b][1][pos] = p.put("v", b, pos, x)
+    check_attention(p, 4)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (80, 7)])
+@pytest.mark.parametrize("lens,size", [([(100, 228), (40, 200)], 2.0 ** 126), ([(3, 228)], 2.0 ** 121)])
+def test_huge_values_of_far_lower_scores_do_not_count(lens, size, dim, page):
+    """Huge values whose keys' scores lie 200 below the others': weights of e^-200 leave nothing of them. (Where a part of the
+    work has no other keys, their weights in it are 1, and 32 of them have to sum to an fp32 number.)"""
+    p = ref.Paged(lens, 2, dim, page, BF16, seed=dim + page)
+    scale = 0.125
+    for b, (_, whole) in enumerate(p.lens):
+        k, v = (x.clone() for x in p.seqs[b])
+        k[:, :, 0] = 0
+        k[:40, :, 0] = -100
+        v[:40] = size
+        p.seqs[b] = [p.put(name, b, torch.arange(whole), x.to(BF16)) for name, x in (("k", k), ("v", v))]
+    q = p.queries(4)
+    q[:, :, 0] = 16
+    check_attention(p, 4, q=q, scale=scale)
