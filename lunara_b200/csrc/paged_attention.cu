@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
               }
             }
           if (!whole && g == 0)
-            *reinterpret_cast<float2*>(p.part_ml + (part * S::kRows + in_tile) * 2) = make_float2(m[n][r] * sl2[n][r], l[n][r]);
+            *reinterpret_cast<float4*>(p.part_ml + (part * S::kRows + in_tile) * kPartMl) = make_float4(m[n][r], l[n][r], sl2[n][r], 0.f);
         }
       }
     t += n_tiles;
@@ -911,7 +911,7 @@ bool prefill_ok(const lunarad_paged_attention_args& a) {
 int64_t stream_workspace(const lunarad_paged_attention_args& a, int sms) {
   const int nt = row_tiles_of(a);
   const int64_t rows = int64_t{2} * stream_workers(a.cache->kind == LUNARAD_KIND_E2M1, nt, sms) * 8 * nt;
-  return rows * (padded_dim(a.cache->dim) + 2) * static_cast<int64_t>(sizeof(float)) + rows / (16 * nt) * static_cast<int64_t>(sizeof(Cut));
+  return rows * (padded_dim(a.cache->dim) + kPartMl) * static_cast<int64_t>(sizeof(float)) + rows / (16 * nt) * static_cast<int64_t>(sizeof(Cut));
 }
 
 template <typename T, bool E2M1, int DP, int NT, bool EXACT>
@@ -1011,7 +1011,7 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
     p.workers = stream_workers(e2m1, p.nt, device_num_sms());
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + int64_t{2} * p.workers * 8 * p.nt * padded_dim(c.dim);
-    p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * 8 * p.nt * 2);
+    p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * 8 * p.nt * kPartMl);
   }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;

@@ -29,12 +29,18 @@ struct PagedParams {
   int64_t min_rows, max_rows;
   int nt;   // 8-row tiles per row tile of the streaming kernel
   // Split work: partial results of each worker (two slots of a row tile).
-  float* part_o;
-  float* part_ml;
+  float* part_o;    // unnormalised output rows
+  float* part_ml;   // kPartMl floats per row: largest score, sum, factor
   struct Cut* cuts;   // of each worker
   int workers;
   unsigned int* err;
 };
+
+// A part's exponents are (score - largest score) * factor, in log2; its row's
+// parts have the same factor. The largest score is kept as it is, not times the
+// factor: for scores of 2^17 that product's rounding would move a part's weight
+// by half a percent against the other parts'.
+constexpr int kPartMl = 4;
 
 // One sequence as the attention kernels see it.
 struct SeqInfo {
@@ -126,20 +132,21 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       auto at = [&](int i) {   // row r of part i
         return (static_cast<int64_t>(w0 + i) * 2 + (i == 0 ? cut.slot : 0)) * tile_rows + r;
       };
-      float m = -INFINITY, l = 0.f, o[kE];
+      float m = -INFINITY, l = 0.f, factor = 0.f, o[kE];
 #pragma unroll
       for (int e = 0; e < kE; ++e) o[e] = 0.f;
       if (use) {
         for (int i0 = split; i0 < cut.parts; i0 += 32 * splits) {
           // Lane k: part i0 + k splits.
           const int n = min(32, (cut.parts - i0 + splits - 1) / splits);
-          float2 ml = make_float2(-INFINITY, 0.f);
-          if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at(i0 + lane * splits));
+          float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+          if (lane < n) ml = *reinterpret_cast<const float4*>(p.part_ml + kPartMl * at(i0 + lane * splits));
+          factor = __shfl_sync(0xffffffffu, ml.z, 0);
           float top = ml.x;
 #pragma unroll
           for (int k = 16; k > 0; k >>= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, k));
           const float next = fmax_nan(m, top), base = next == -INFINITY ? 0.f : next;
-          const float keep = ex2_approx(m - base), f = ex2_approx(ml.x - base);
+          const float keep = ex2_approx((m - base) * factor), f = ex2_approx((ml.x - base) * factor);
           m = next;
           l = l * keep + ml.y * f;   // of this lane's parts, summed below
 #pragma unroll
@@ -170,7 +177,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
           for (int k = 1; k < splits; ++k) {
             const float2 ml = s_ml[warp + k * at_once];
             const float next = fmax_nan(m, ml.x), base = next == -INFINITY ? 0.f : next;
-            const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base);
+            const float fa = ex2_approx((m - base) * factor), fb = ex2_approx((ml.x - base) * factor);   // (split 0 has had a part)
             m = next;
             l = l * fa + ml.y * fb;
 #pragma unroll

@@ -551,8 +551,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       int lo, hi;
       visible(p, x.s.pos0 + i, lo, hi);
       const int n = x.n, block0 = x.block0;
-      float m = -INFINITY, l = 0.f;   // maximum (scaled, log2) and sum
-      float top = -INFINITY;          // the score that gave the maximum
+      // The largest score so far (as of the last rescaling), its product with the
+      // factor, and the sum. Exponents are score * factor - off in one FMA, off by
+      // the rounding of `off`, 2^-24 of it. That cancels out as long as all of a
+      // row's terms share it; where it could be felt in the differences (|off|
+      // above 8192: "far"), `top` is taken off the scores first.
+      float top = -INFINITY, off = -INFINITY, l = 0.f;
+      auto far_off = [](float x) { return fabsf(x) > 8192.f; };
+      // What the exponents' base is above top * factor.
+      auto excess = [&](float t, float x) { return far_off(x) ? 0.f : fmaf(-t, sl2, x); };
       for (int j = 0; j < n; ++j, ++blocks) {
         if (!mbar_wait_warp(&s_full[w], blocks & 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
         tc_fence_after();
@@ -589,20 +596,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; e += 2)
             mxp[(e >> 1) & 7] = fmax3_nan(mxp[(e >> 1) & 7], __uint_as_float(sc[cc][e]), __uint_as_float(sc[cc][e + 1]));
         const float mx = fmax3_nan(fmax3_nan(mxp[0], mxp[1], mxp[2]), fmax3_nan(mxp[3], mxp[4], mxp[5]), fmax_nan(mxp[6], mxp[7]));
-        const float cand = mx * sl2;
         if (j == 0) {
-          m = cand;
           top = mx;
-        } else if (__any_sync(0xffffffffu, !(cand <= m + kRescaleLog2))) {
+          off = mx * sl2;
+        } else if (__any_sync(0xffffffffu, !(mx <= top || (mx - top) * sl2 <= kRescaleLog2))) {
           // O is rescaled once P V of the block before has completed (as it has:
           // S of this block ran after it).
           if (!mbar_wait_warp(&o_full[w], (blocks - 1) & 1u, abort_flag, p.err, kErrPagedWait)) { ok = false; break; }
           tc_fence_after();
-          const float next = fmax_nan(m, cand);
-          top = fmax_nan(top, mx);
-          const float alpha = next == -INFINITY ? 1.f : ex2_approx(m - next);
+          const float next = fmax_nan(top, mx), next_off = next * sl2;
+          const float alpha = next == -INFINITY ? 1.f : ex2_approx(fmaf(top - next, sl2, excess(top, off) - excess(next, next_off)));
           l *= alpha;
-          m = next;
+          top = next;
+          off = next_off;
           const uint64_t a2 = f2_pack(alpha, alpha);
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
@@ -622,19 +628,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_32x32b_x16(tO + c * 16, ov);
           }
         }
-        float off = m == -INFINITY ? 0.f : m;
-        // score * factor - maximum in one FMA is off by the rounding of the
-        // maximum, 2^-24 of it: where that matters, the largest score is taken
-        // off the scores first.
-        if (__any_sync(0xffffffffu, fabsf(off) > 8192.f)) {
-          const float sub = off == 0.f ? 0.f : top;
+        const bool far = far_off(off);   // (a row that has seen no key too: nothing is taken off its -inf)
+        if (__any_sync(0xffffffffu, far)) {
+          const float sub = far && top != -INFINITY ? top : 0.f;
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
             for (int e = 0; e < 32; ++e) sc[cc][e] = __float_as_uint(__uint_as_float(sc[cc][e]) - sub);
-          off = 0.f;
         }
-        const uint64_t sl2x2 = f2_pack(sl2, sl2), neg2 = f2_pack(-off, -off);
+        const float minus = far ? 0.f : -off;
+        const uint64_t sl2x2 = f2_pack(sl2, sl2), neg2 = f2_pack(minus, minus);
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -685,9 +688,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // With fp16 a masked score adds 2^-126 at most (the cubic's smallest), which
       // is nothing beside a row's largest, but the whole sum of a row that saw no
       // key: such a row keeps its maximum of -inf.
-      if (m == -INFINITY) l = 0.f;
+      if (top == -INFINITY) l = 0.f;
       const bool whole = x.first == 0 && n == x.item_blocks;
-      const float f = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.f;
+      // A part's exponents are brought to the base top * factor, the same in all parts.
+      const float f = l == 0.f ? 0.f : whole ? 1.0f / l : ex2_approx(excess(top, off));
       const int head = x.kh * p.group + static_cast<int>((real ? row : rows - 1) - static_cast<int64_t>(i) * p.group);
       T* out = static_cast<T*>(p.o) + (x.s.first + i) * p.o_tok + head * p.o_head;
       const int64_t part = (static_cast<int64_t>(worker) * 2 + (t == t_first ? 0 : 1)) * kItemRows + w * kTileRows + r;
@@ -713,13 +717,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < 8; ++q) {
               const bool none = l == 0.f;
               *reinterpret_cast<float4*>(po + 32 * c + 4 * q) =
-                  make_float4(none ? 0.f : __uint_as_float(ov[4 * q]), none ? 0.f : __uint_as_float(ov[4 * q + 1]),
-                              none ? 0.f : __uint_as_float(ov[4 * q + 2]), none ? 0.f : __uint_as_float(ov[4 * q + 3]));
+                  make_float4(none ? 0.f : __uint_as_float(ov[4 * q]) * f, none ? 0.f : __uint_as_float(ov[4 * q + 1]) * f,
+                              none ? 0.f : __uint_as_float(ov[4 * q + 2]) * f, none ? 0.f : __uint_as_float(ov[4 * q + 3]) * f);
             }
           }
         }
       }
-      if (real && !whole) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
+      if (real && !whole) *reinterpret_cast<float4*>(p.part_ml + part * kPartMl) = make_float4(top, l * f, sl2, 0.f);
       tc_fence_before();
       mbar_arrive(&o_free[w]);
       if (t + n >= t_end && threadIdx.x == 0) {
@@ -802,14 +806,14 @@ cudaError_t run_prefill(PagedParams p, cudaStream_t s) {
 }  // namespace
 
 int64_t paged_prefill_workspace(int dim, int sms) {
-  return int64_t{2} * sms * kItemRows * ((dim <= 64 ? 64 : 128) + 2) * static_cast<int64_t>(sizeof(float)) + sms * static_cast<int64_t>(sizeof(Cut));
+  return int64_t{2} * sms * kItemRows * ((dim <= 64 ? 64 : 128) + kPartMl) * static_cast<int64_t>(sizeof(float)) + sms * static_cast<int64_t>(sizeof(Cut));
 }
 
 cudaError_t launch_paged_prefill(PagedParams p, int dtype, void* workspace, cudaStream_t stream) {
   p.workers = device_num_sms();
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + int64_t{2} * p.workers * kItemRows * (p.dim <= 64 ? 64 : 128);
-  p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * kItemRows * 2);
+  p.cuts = reinterpret_cast<Cut*>(p.part_ml + int64_t{2} * p.workers * kItemRows * kPartMl);
   if (dtype == LUNARA_BF16)
     return p.dim <= 64 ? run_prefill<__nv_bfloat16, 64>(p, stream) : run_prefill<__nv_bfloat16, 128>(p, stream);
   return p.dim <= 64 ? run_prefill<__half, 64>(p, stream) : run_prefill<__half, 128>(p, stream);

@@ -78,3 +78,58 @@ def test_huge_values_of_far_lower_scores_do_not_count(lens, size, dim, page):
     q = p.queries(4)
     q[:, :, 0] = 16
     check_attention(p, 4, q=q, scale=scale)
+
+
+# Scores of the order of 2^17 that are exact in fp32 (2^17 and sixteenths), so that what an output can be off by
+# has no score term: half a step of it and of the probabilities, 2^-13 for the exponential (1.2e-4), and a 2^-24 for
+# each key's sum and for the factors.
+
+def _far_pair(factor=1.4426950408889634):
+    """Two offsets whose products with the factor are rounded farthest apart in fp32."""
+    x = np.arange(0, 8, 1 / 16)
+    off = ((131072 + x).astype(np.float32) * np.float32(factor)).astype(np.float64) - (131072 + x) * float(np.float32(factor))
+    best = max(((abs(off[i] - off[j]), i, j) for i in range(len(x)) for j in range(len(x)) if abs(x[i] - x[j]) <= 1), key=lambda t: t[0])
+    assert best[0] > 0.01
+    return float(x[best[1]]), float(x[best[2]])
+
+
+def _far_scores(lens, tall, split):
+    """One key head of 64: keys (256, x, 0 ..) with x of two values, `split` keys of the first; queries (512, 1 or `tall`, 0 ..)."""
+    p = ref.Paged(lens, 1, 64, 16, F16, seed=31)
+    a, b = _far_pair()
+    for s, (_, whole) in enumerate(p.lens):
+        k = torch.zeros(whole, 1, 64)
+        k[:, 0, 0] = 256
+        k[:, 0, 1] = torch.where(torch.arange(whole) < split, min(a, b), max(a, b))
+        v = torch.zeros(whole, 1, 64)
+        v[:split] = 1
+        v[:, 0, 5] = torch.randn(whole, generator=p.g)
+        p.seqs[s] = [p.put("k", s, torch.arange(whole), k.half()), p.put("v", s, torch.arange(whole), v.half())]
+    q = torch.zeros(p.tokens, 1, 64)
+    q[:, 0, 0], q[:, 0, 1] = 512, 1
+    q[1::2, 0, 1] = tall
+    return p, q.half()
+
+
+def _check_far(p, q):
+    ops = _ops()
+    cache, _ = cache_of(p)
+    out = ops.paged_attention(q.cuda(), cache, *where(p), scale=1.0)
+    at, h = 0, half_step(F16)
+    for b, (n, whole) in enumerate(p.lens):
+        k, v = p.seqs[b]
+        want, spread, _ = ref.attend(q[at:at + n], k, v, whole - n, 1.0)
+        tol = h * want.abs() + (1 + h) * (h + 2.0 ** -13 + (whole + 16) * 2.0 ** -24) * spread + (1 + whole) * TINY
+        within(out[at:at + n], want, tol, f"sequence {b}")
+        at += n
+
+
+@pytest.mark.parametrize("n", [1, 4, 12, 64, 300])
+def test_far_scores_of_cut_rows(n):
+    """One sequence, cut into many parts that have one of two maxima."""
+    _check_far(*_far_scores([(n, 4096 + n)], 1.0, 2048))
+
+
+def test_far_scores_of_whole_rows():
+    """Prompts of two key blocks, many of them to a run; every second row's maximum grows far, so that all rows are rescaled."""
+    _check_far(*_far_scores([(40, 256)] * 300, 60.0, 128))
