@@ -160,13 +160,14 @@ struct QuantParams {
 };
 
 // code = e2m1(y / s), the quotient rounded to nearest as IEEE division does:
-// with r = RN(1/s), q0 = RN(y r) and the exact remainder y - q0 s, RN(q0 +
+// with r = RN(1/s), q0 = RN(y r) and the exact remainder q0 s - y, RN(q0 -
 // remainder * r) is the correctly rounded quotient (Markstein, 1990; s has 4
 // significant bits, so the all-ones exception of the theorem cannot arise).
-// The sign is y's (s is positive): the sums would make +0 of a negative zero.
+// The remainder is taken with this sign so that a negative zero stays one: its
+// remainder is +0, and -0 - 0 r = -0 (with y - q0 s the sum would be +0).
 __device__ __forceinline__ float quotient(float y, float s, float r) {
   const float q0 = __fmul_rn(y, r);
-  return copysignf(__fmaf_rn(__fmaf_rn(-q0, s, y), r, q0), y);
+  return __fmaf_rn(-__fmaf_rn(q0, s, -y), r, q0);
 }
 
 // The e4m3 scale of a block whose largest magnitude is amax (saturates at 448,
