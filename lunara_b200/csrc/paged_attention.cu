@@ -474,9 +474,9 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
     // Q^T as the B operand: the lane holds query row g of each 8-row tile.
     uint32_t qf[NT][S::kSteps][2];
     // The maximum below needs a positive factor: a negative scale turns the
-    // queries' signs instead, and a zero one becomes too small to matter.
+    // queries' signs instead.
     float sl2[NT][2];   // of the columns 2 c, 2 c + 1
-    const float scale_log2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);
+    const float scale_log2 = fabsf(p.scale) * 1.4426950408889634f;
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           }
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) sl2[n][r] = scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * c + r));
+      for (int r = 0; r < 2; ++r) sl2[n][r] = exponent_factor(scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * c + r)));
     }
 
     // ---------------------------------------------------------- key tiles --

@@ -42,6 +42,14 @@ struct PagedParams {
 // by half a percent against the other parts'.
 constexpr int kPartMl = 4;
 
+// The factor of a row's exponents, (score - largest score) * factor in log2: the
+// scale times log2(e), and times what its queries were divided by. It takes part
+// as a positive fp32 number of any size. Zero would make NaN of the distance of
+// the first score from -inf: it becomes the smallest number, which leaves every
+// distance between fp32 numbers at nothing, as zero would. Infinity, which only
+// scores beyond fp32 can need, becomes the largest.
+__device__ __forceinline__ float exponent_factor(float f) { return fminf(fmaxf(f, 1.4e-45f), 3.402823466e38f); }
+
 // One sequence as the attention kernels see it.
 struct SeqInfo {
   int first;      // its first token

@@ -535,9 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + L::kTmemS + w * 128;
     const uint32_t tO = tmem_base + lane_off + L::kTmemO + w * D;
-    // The maximum needs a positive factor (the scale is not negative here): a
-    // zero one becomes too small to matter.
-    const float sl2 = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);
+    const float sl2 = exponent_factor(p.scale * 1.4426950408889634f);   // (the scale is not negative here)
     bool ok = true;
     Cursor cur = s_cursor;
     uint32_t blocks = 0;

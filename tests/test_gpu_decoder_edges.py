@@ -133,3 +133,13 @@ def test_far_scores_of_cut_rows(n):
 def test_far_scores_of_whole_rows():
     """Prompts of two key blocks, many of them to a run; every second row's maximum grows far, so that all rows are rescaled."""
     _check_far(*_far_scores([(40, 256)] * 300, 60.0, 128))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lens", [[(1, 200), (4, 77), (1, 3000)], [(64, 200), (150, 300)]])
+@pytest.mark.parametrize("scale,size", [(0.0, 2.0 ** -110), (0.0, 2.0 ** 110), (2.0 ** -110, 2.0 ** 100), (2.0 ** -100, 2.0 ** -60),
+                                        (2.0 ** -110, 2.0 ** 110), (-2.0 ** -105, 2.0 ** 105), (2.0 ** 100, 2.0 ** -100)])
+def test_scales_near_the_ends(scale, size, lens, bits):
+    """The scale takes its part at any size, zero included; queries make up for it, or do not."""
+    p = ref.Paged(lens, 2, 128, 16, BF16, seed=16, bits=bits)
+    check_attention(p, 4, scale=scale, q=p.queries(4) * size)
