@@ -504,11 +504,12 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // Times 2^-e for 2^e <= top < 2^(e + 1), and the scores times 2^e;
-        // rows of zeros or subnormals and rows at fp32's upper end stay as they are.
-        const uint32_t e = __float_as_uint(top) >> 23;
-        const bool use = e > 0u && e < 254u;
-        const float down = use ? __uint_as_float((254u - e) << 23) : 1.f;
+        // Times 2^-e for 2^e <= top < 2^(e + 1), and the scores times 2^e; rows of
+        // zeros or subnormals stay as they are. An infinite element stays one, and
+        // the finite ones beside it come into f16's range like those of 2^127.
+        const uint32_t e = min(__float_as_uint(top) >> 23, 254u);
+        const bool use = e > 0u;
+        const float down = use ? __uint_as_float(e < 254u ? (254u - e) << 23 : 0x00400000u) : 1.f;   // 2^-127 is subnormal
         up = use ? __uint_as_float(e << 23) : 1.f;
 #pragma unroll
         for (int w = 0; w < S::kSteps; ++w)

@@ -143,3 +143,13 @@ def test_scales_near_the_ends(scale, size, lens, bits):
     """The scale takes its part at any size, zero included; queries make up for it, or do not."""
     p = ref.Paged(lens, 2, 128, 16, BF16, seed=16, bits=bits)
     check_attention(p, 4, scale=scale, q=p.queries(4) * size)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_4bit_queries_at_the_upper_end(dim):
+    """Rows with an element of 2^127 and more, the others far below."""
+    p = ref.Paged([(1, 200), (3, 50), (40, 90)], 2, dim, 16, BF16, seed=17, bits=4)
+    q = torch.randn(p.tokens, 4, dim, generator=p.g) * 2.0 ** 124
+    q = q.clamp(-2.0 ** 126, 2.0 ** 126)
+    q[:, :, 3] = 1.5 * 2.0 ** 127 * (1 - 2 * torch.randint(0, 2, q.shape[:2], generator=p.g))
+    check_attention(p, 4, scale=2.0 ** -126, q=q.to(BF16))
