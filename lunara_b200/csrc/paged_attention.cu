@@ -98,8 +98,9 @@ __global__ void __launch_bounds__(kSimpleThreads) paged_simple_kernel(const __gr
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const float m_new = fmax_nan(m, s);
     const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = __expf(m - base);
-    const float pj = __expf(s - base);
+    // expf is off by 2 ulp at any argument, so that fp32 calls get fp32 weights.
+    const float corr = expf(m - base);
+    const float pj = expf(s - base);
     l = l * corr + pj;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {

@@ -135,6 +135,31 @@ def test_far_scores_of_whole_rows():
     _check_far(*_far_scores([(40, 256)] * 300, 60.0, 128))
 
 
+@pytest.mark.parametrize("dim", [32, 20])
+def test_fp32_weights_are_fp32(dim):
+    """Two keys with scores 0 and -x, values 0 and 1: the output is e^-x / (1 + e^-x), every product exact. Off by the
+    exponential (2 ulp), the sum, the rescaling product, the division and its product: below 8 roundings of 2^-24."""
+    ops = _ops()
+    n = 60
+    p = ref.Paged([(1, 2)] * n, 1, dim, 8, F32, seed=4)
+    q = torch.zeros(n, 1, dim)
+    q[:, 0, 0] = 1
+    want = torch.empty(n, dtype=torch.float64)
+    for b in range(n):
+        x = b / 2 + 0.25
+        k, v = torch.zeros(2, 1, dim), torch.zeros(2, 1, dim)
+        far = b % 2   # which of the two keys comes first
+        k[far, 0, 0] = -x
+        v[far] = 1
+        p.put("k", b, torch.arange(2), k)
+        p.put("v", b, torch.arange(2), v)
+        want[b] = np.exp(-x) / (1 + np.exp(-x))
+    cache, _ = cache_of(p)
+    out = ops.paged_attention(q.cuda(), cache, *where(p), scale=1.0)
+    want = want[:, None, None].expand(n, 1, dim)
+    within(out, want, 2.0 ** -21 * want, "weights")
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("lens", [[(1, 200), (4, 77), (1, 3000)], [(64, 200), (150, 300)]])
 @pytest.mark.parametrize("scale,size", [(0.0, 2.0 ** -110), (0.0, 2.0 ** 110), (2.0 ** -110, 2.0 ** 100), (2.0 ** -100, 2.0 ** -60),
