@@ -33,6 +33,12 @@ extern "C" {
  * even element in the low nibble) with one e4m3 scale byte per 16 elements. */
 #define LUNARAD_KIND_E2M1 16
 
+/* Or-ed into `dtype` of lunarad_kv_append, lunarad_kv_read and
+ * lunarad_paged_attention: output rows of tokens that belong to no sequence are
+ * zeroed instead of left alone (for outputs in fresh memory). Refused for tokens
+ * without any sequence (batch 0), where no kernel runs. */
+#define LUNARAD_ZERO_REST 0x100
+
 /* Pairs that are turned together: (i, i + rot/2) or (2i, 2i + 1). */
 typedef enum lunarad_rotary_layout {
   LUNARAD_ROTARY_HALF = 0,
@@ -108,8 +114,9 @@ typedef struct lunarad_cache {
  * of sequence b are seq_starts[b] .. seq_starts[b + 1] - 1 and are the last
  * ones of its seq_lens[b] positions. Position p of sequence b lies in page
  * page_table[b][p / page_size], slot p % page_size. A token with a negative
- * position (seq_lens[b] below its number of tokens) is padding; tokens from
- * seq_starts[batch] on belong to no sequence and are left alone. */
+ * position (seq_lens[b] below its number of tokens) is padding; tokens before
+ * seq_starts[0] and from seq_starts[batch] on belong to no sequence, and their
+ * rows are left alone unless LUNARAD_ZERO_REST is given. */
 typedef struct lunarad_sequences {
   const int32_t* page_table;  /* [batch, max_pages], row stride table_stride */
   const int32_t* seq_starts;  /* [batch + 1] */
@@ -136,7 +143,7 @@ typedef struct lunarad_kv_append_args {
   lunarad_sequences seqs;
   lunarad_rotary_table rotary;
   int64_t q_heads;
-  int64_t dtype;  /* of k, v, q, q_out */
+  int64_t dtype;  /* of k, v, q, q_out; | LUNARAD_ZERO_REST for q_out */
 } lunarad_kv_append_args;
 int lunarad_kv_append(const lunarad_kv_append_args* args, void* stream);
 
@@ -148,7 +155,7 @@ typedef struct lunarad_kv_read_args {
   void* v_out;
   const lunarad_cache* cache;
   lunarad_sequences seqs;
-  int64_t dtype;
+  int64_t dtype;  /* | LUNARAD_ZERO_REST */
 } lunarad_kv_read_args;
 int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream);
 
@@ -176,7 +183,7 @@ typedef struct lunarad_paged_attention_args {
   int64_t q_heads;
   int64_t window;
   int64_t max_q_len;
-  int64_t dtype;
+  int64_t dtype;  /* | LUNARAD_ZERO_REST */
   double scale;
 } lunarad_paged_attention_args;
 int lunarad_paged_attention(const lunarad_paged_attention_args* args, void* workspace, int64_t workspace_bytes,

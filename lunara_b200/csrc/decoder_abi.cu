@@ -102,7 +102,6 @@ int check_sequences(const char* fn, const lunarad_sequences& s) {
 }
 
 int check_attention(const char* fn, const lunarad_paged_attention_args* a) {
-  if (a == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
   int rc = check_cache(fn, a->cache);
   if (rc == LUNARA_OK) rc = check_sequences(fn, a->seqs);
   if (rc != LUNARA_OK) return rc;
@@ -122,6 +121,21 @@ int check_attention(const char* fn, const lunarad_paged_attention_args* a) {
   if (a->max_q_len < 0) return fail(LUNARA_ERR_INVALID_ARG, "%s: negative max_q_len", fn);
   if (!std::isfinite(a->scale)) return fail(LUNARA_ERR_INVALID_ARG, "%s: scale is not finite", fn);
   return LUNARA_OK;
+}
+
+// The arguments with a bare dtype, and whether LUNARAD_ZERO_REST was in it.
+template <typename Args>
+Args take_zero_rest(const Args& a, bool& zero_rest) {
+  Args bare = a;
+  zero_rest = (a.dtype & LUNARAD_ZERO_REST) != 0;
+  bare.dtype &= ~int64_t{LUNARAD_ZERO_REST};
+  return bare;
+}
+
+// A call without sequences or without tokens: nothing runs.
+int no_work(const char* fn, const lunarad_sequences& s, bool zero_rest) {
+  if (zero_rest && s.tokens > 0) return fail(LUNARA_ERR_INVALID_ARG, "%s: rows of no sequence are zeroed beside a sequence's only", fn);
+  return ok();
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
@@ -166,9 +180,11 @@ int lunarad_qk_norm_rotary(const lunarad_qk_norm_rotary_args* a, void* stream) {
   return from_cuda(launch_qk_norm_rotary(*a, as_stream(stream)), fn);
 }
 
-int lunarad_kv_append(const lunarad_kv_append_args* a, void* stream) {
+int lunarad_kv_append(const lunarad_kv_append_args* args, void* stream) {
   static const char* fn = "lunarad_kv_append";
-  if (a == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  if (args == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  bool zero_rest;
+  const lunarad_kv_append_args bare = take_zero_rest(*args, zero_rest), *a = &bare;
   int rc = check_cache(fn, a->cache);
   if (rc == LUNARA_OK) rc = check_sequences(fn, a->seqs);
   if (rc != LUNARA_OK) return rc;
@@ -182,52 +198,61 @@ int lunarad_kv_append(const lunarad_kv_append_args* a, void* stream) {
   if (a->q_heads + 2 * c.kv_heads > kMaxHeads) return fail(LUNARA_ERR_UNSUPPORTED, "%s: more than 65535 heads", fn);
   if (c.kind == LUNARAD_KIND_E2M1 && c.dim > 512)
     return fail(LUNARA_ERR_UNSUPPORTED, "%s: head dim %lld > 512 into a 4-bit cache", fn, (long long)c.dim);
-  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return ok();
+  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return no_work(fn, a->seqs, zero_rest);
   rc = check_view(fn, "K", a->k, a->dtype);
   if (rc == LUNARA_OK) rc = check_view(fn, "V", a->v, a->dtype);
   if (rc == LUNARA_OK && a->q_heads > 0) rc = check_view(fn, "Q", a->q, a->dtype);
   if (rc == LUNARA_OK && a->q_heads > 0) rc = check_view(fn, "Q's output", a->q_out, a->dtype);
   if (rc != LUNARA_OK) return rc;
-  return from_cuda(launch_kv_append(*a, as_stream(stream)), fn);
+  return from_cuda(launch_kv_append(*a, zero_rest, as_stream(stream)), fn);
 }
 
-int lunarad_kv_read(const lunarad_kv_read_args* a, void* stream) {
+int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream) {
   static const char* fn = "lunarad_kv_read";
-  if (a == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  if (args == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  bool zero_rest;
+  const lunarad_kv_read_args bare = take_zero_rest(*args, zero_rest), *a = &bare;
   int rc = check_cache(fn, a->cache);
   if (rc == LUNARA_OK) rc = check_sequences(fn, a->seqs);
   if (rc != LUNARA_OK) return rc;
   if (!valid_dtype(a->dtype)) return fail(LUNARA_ERR_INVALID_ARG, "%s: bad dtype %lld", fn, (long long)a->dtype);
   if (a->cache->kind != LUNARAD_KIND_E2M1 && a->cache->kind != a->dtype)
     return fail(LUNARA_ERR_INVALID_ARG, "%s: output and cache differ in dtype", fn);
-  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return ok();
+  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return no_work(fn, a->seqs, zero_rest);
   if (a->k_out == nullptr || a->v_out == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: output is NULL", fn);
   if (!aligned(a->k_out, dtype_bytes(a->dtype)) || !aligned(a->v_out, dtype_bytes(a->dtype)))
     return fail(LUNARA_ERR_INVALID_ARG, "%s: output is not aligned to its elements", fn);
-  return from_cuda(launch_kv_read(*a, as_stream(stream)), fn);
+  return from_cuda(launch_kv_read(*a, zero_rest, as_stream(stream)), fn);
 }
 
-int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* a, int device) {
-  const int rc = check_attention("lunarad_paged_attention_workspace", a);
+int64_t lunarad_paged_attention_workspace(const lunarad_paged_attention_args* args, int device) {
+  static const char* fn = "lunarad_paged_attention_workspace";
+  if (args == nullptr) return -fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  bool zero_rest;
+  const lunarad_paged_attention_args bare = take_zero_rest(*args, zero_rest), *a = &bare;
+  const int rc = check_attention(fn, a);
   if (rc != LUNARA_OK) return -rc;
   ok();
   if (a->seqs.batch == 0 || a->seqs.tokens == 0) return 0;
   return paged_attention_workspace(*a, device_num_sms_of(device));
 }
 
-int lunarad_paged_attention(const lunarad_paged_attention_args* a, void* workspace, int64_t workspace_bytes,
+int lunarad_paged_attention(const lunarad_paged_attention_args* args, void* workspace, int64_t workspace_bytes,
                             void* stream) {
   static const char* fn = "lunarad_paged_attention";
+  if (args == nullptr) return fail(LUNARA_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  bool zero_rest;
+  const lunarad_paged_attention_args bare = take_zero_rest(*args, zero_rest), *a = &bare;
   int rc = check_attention(fn, a);
   if (rc != LUNARA_OK) return rc;
-  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return ok();
+  if (a->seqs.batch == 0 || a->seqs.tokens == 0) return no_work(fn, a->seqs, zero_rest);
   rc = check_view(fn, "Q", a->q, a->dtype);
   if (rc == LUNARA_OK) rc = check_view(fn, "O", a->o, a->dtype);
   if (rc != LUNARA_OK) return rc;
   const int64_t need = paged_attention_workspace(*a, device_num_sms());
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(LUNARA_ERR_INVALID_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
-  return from_cuda(launch_paged_attention(*a, workspace, as_stream(stream)), fn);
+  return from_cuda(launch_paged_attention(*a, zero_rest, workspace, as_stream(stream)), fn);
 }
 
 }  // extern "C"

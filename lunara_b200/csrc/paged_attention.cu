@@ -68,7 +68,11 @@ __global__ void __launch_bounds__(kSimpleThreads) paged_simple_kernel(const __gr
   if (token >= p.seqs.tokens) return;
   int seq;
   int64_t pos;
-  if (!find_token(p.seqs, token, seq, pos)) return;
+  if (!find_token(p.seqs, token, seq, pos)) {
+    if (p.zero_behind)
+      for (int d = lane; d < p.dim; d += 32) static_cast<T*>(p.o)[token * p.o_tok + h * p.o_head + d] = Io<T>::from_f(0.f);
+    return;
+  }
   const T* q = static_cast<const T*>(p.q) + token * p.q_tok + h * p.q_head;
   float qv[kPer], ov[kPer];
 #pragma unroll
@@ -926,13 +930,15 @@ cudaError_t run_stream(PagedParams p, cudaStream_t s) {
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = prepare_once(kern, prepared, kWarps * S::kRingBytes + 8 * (kMaxBatch + 2), 0);
   if (e != cudaSuccess) return e;
-  const int batch = p.seqs.batch;
+  const int batch = p.seqs.batch, zero_rest = p.zero_behind;
   const Seqs all = p.seqs;
   for (int b0 = 0; b0 < batch; b0 += kMaxBatch) {   // more sequences than the prefix sums hold: one after the other
     p.seqs.batch = batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch;
     p.seqs.page_table = all.page_table + b0 * all.table_stride;
     p.seqs.starts = all.starts + b0;
     p.seqs.lens = all.lens + b0;
+    p.zero_before = zero_rest && b0 == 0;
+    p.zero_behind = zero_rest && b0 + p.seqs.batch == batch;
     e = launch_pdl(kern, dim3(p.workers / kWarps), dim3(kStreamThreads), smem, s, p);
     if (e != cudaSuccess) return e;
     e = launch_pdl(paged_join_kernel<T, DP>, dim3(join_blocks(p.workers), 4), dim3(kJoinThreads), 0, s, p, int{S::kRows});
@@ -966,7 +972,7 @@ int64_t paged_attention_workspace(const lunarad_paged_attention_args& a, int sms
   return stream_workspace(a, sms) + (prefill_ok(a) ? paged_prefill_workspace(static_cast<int>(a.cache->dim), sms) : 0);
 }
 
-cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* workspace, cudaStream_t stream) {
+cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, bool zero_rest, void* workspace, cudaStream_t stream) {
   const lunarad_cache& c = *a.cache;
   PagedParams p{};
   p.q = a.q.data;
@@ -1017,13 +1023,14 @@ cudaError_t launch_paged_attention(const lunarad_paged_attention_args& a, void* 
   }
   p.err = device_error_word();
   if (p.err == nullptr) return cudaErrorInvalidDevice;
-  if (prefill_ok(a)) {
+  if (prefill_ok(a)) {   // (the rows of no sequence are the other kernel's)
     PagedParams q = p;
     q.min_rows = p.max_rows = kPrefillRows;
     const cudaError_t e = launch_paged_prefill(q, static_cast<int>(a.dtype),
                                                static_cast<char*>(workspace) + stream_workspace(a, device_num_sms()), stream);
     if (e != cudaSuccess) return e;
   }
+  p.zero_before = p.zero_behind = zero_rest;
   if (a.dtype == LUNARA_F16) return run<__half>(p, stream_kernel, e2m1, stream);
   if (a.dtype == LUNARA_BF16) return run<__nv_bfloat16>(p, stream_kernel, e2m1, stream);
   return run<float>(p, stream_kernel, e2m1, stream);

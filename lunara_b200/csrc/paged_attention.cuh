@@ -28,6 +28,7 @@ struct PagedParams {
   // Sequences with min_rows <= (their tokens * group) < max_rows are this kernel's.
   int64_t min_rows, max_rows;
   int nt;   // 8-row tiles per row tile of the streaming kernel
+  int zero_before, zero_behind;   // clear the rows before the first sequence, behind the last
   // Split work: partial results of each worker (two slots of a row tile).
   float* part_o;    // unnormalised output rows
   float* part_ml;   // kPartMl floats per row: largest score, sum, factor
@@ -86,18 +87,29 @@ struct Cut {
   int pad[2];
 };
 
+// Clears the output rows of token; by a whole block.
+template <typename T>
+__device__ __forceinline__ void clear_token(const PagedParams& p, int token) {
+  const int width = p.q_heads * p.dim;
+  for (int e = threadIdx.x; e < width; e += blockDim.x)
+    static_cast<T*>(p.o)[token * p.o_tok + e / p.dim * p.o_head + e % p.dim] = Io<T>::from_f(0.f);
+}
+
 // Clears the output rows of the sequences that are this kernel's and have no
-// keys; by whole blocks, each its share of the sequences.
+// keys, and of the tokens that no sequence owns where that is asked for; by
+// whole blocks, each its share.
 template <typename T>
 __device__ __forceinline__ void clear_empty(const PagedParams& p) {
+  if (p.zero_before)
+    for (int token = blockIdx.x, end = min(p.seqs.starts[0], p.seqs.tokens); token < end; token += gridDim.x) clear_token<T>(p, token);
+  if (p.zero_behind)
+    for (int64_t token = int64_t{max(p.seqs.starts[p.seqs.batch], 0)} + blockIdx.x; token < p.seqs.tokens; token += gridDim.x)
+      clear_token<T>(p, static_cast<int>(token));
   for (int b = blockIdx.x; b < p.seqs.batch; b += gridDim.x) {
     const SeqInfo s = load_seq(p, b);
     const int64_t rows = static_cast<int64_t>(s.n) * p.group;
     if (rows < p.min_rows || rows >= p.max_rows || s.hi > s.lo) continue;
-    const int width = p.q_heads * p.dim;
-    for (int token = s.first; token < s.first + s.n; ++token)
-      for (int e = threadIdx.x; e < width; e += blockDim.x)
-        static_cast<T*>(p.o)[token * p.o_tok + e / p.dim * p.o_head + e % p.dim] = Io<T>::from_f(0.f);
+    for (int token = s.first; token < s.first + s.n; ++token) clear_token<T>(p, token);
   }
 }
 

@@ -105,6 +105,7 @@ struct RowsParams {
   int rot, dim, units, lanes_log2;
   int tokens, seq;         // tokens = batch * seq
   int inverse;
+  int zero_rest;           // rows of tokens that no sequence owns: zero, not left alone
   float eps;
   unsigned int* err;
 };
@@ -131,8 +132,11 @@ __device__ __forceinline__ TokenPlace place_token(const RowsParams& p, int token
   if (!t.owned) return t;
   if constexpr (PAGED) {
     int seq;
-    t.owned = find_token(p.seqs, token, seq, t.pos);
-    if (!t.owned || t.pos < 0) return t;
+    if (!find_token(p.seqs, token, seq, t.pos)) {
+      t.owned = p.zero_rest != 0;
+      return t;
+    }
+    if (t.pos < 0) return t;
     t.page = find_page(p.seqs, seq, t.pos, p.num_pages, t.slot, p.err);
     t.valid = t.page >= 0;
   } else {
@@ -437,7 +441,7 @@ struct ReadParams {
   int64_t page_stride[2], head_stride[2], sc_page[2], sc_head[2];
   float gain[2];
   void* dst[2];
-  int heads, dim, units, lanes_log2, num_pages, tokens;
+  int heads, dim, units, lanes_log2, num_pages, tokens, zero_rest;
   unsigned int* err;
 };
 
@@ -454,7 +458,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   const int h0 = static_cast<int>(blockIdx.y) * HEADS, kv = static_cast<int>(blockIdx.z), nh = min(HEADS, p.heads - h0);
   int seq, slot = 0, page = -1;
   int64_t pos;
-  if (!find_token(p.seqs, token, seq, pos)) return;
+  if (!find_token(p.seqs, token, seq, pos)) {
+    if (!p.zero_rest) return;
+    pos = -1;
+  }
   if (pos >= 0) page = find_page(p.seqs, seq, pos, p.num_pages, slot, p.err);
   T* dst = static_cast<T*>(p.dst[kv]) + (static_cast<int64_t>(token) * p.heads + h0) * p.dim;
   const int64_t at = page * p.page_stride[kv] + h0 * p.head_stride[kv];
@@ -510,7 +517,10 @@ __global__ void __launch_bounds__(kThreads) read_any_kernel(const __grid_constan
   const int h = static_cast<int>(blockIdx.y), kv = static_cast<int>(blockIdx.z);
   int seq, slot = 0, page = -1;
   int64_t pos;
-  if (!find_token(p.seqs, token, seq, pos)) return;
+  if (!find_token(p.seqs, token, seq, pos)) {
+    if (!p.zero_rest) return;
+    pos = -1;
+  }
   if (pos >= 0) page = find_page(p.seqs, seq, pos, p.num_pages, slot, p.err);
   T* dst = static_cast<T*>(p.dst[kv]) + (static_cast<int64_t>(token) * p.heads + h) * p.dim;
   const int64_t at = page * p.page_stride[kv] + h * p.head_stride[kv];
@@ -710,7 +720,7 @@ cudaError_t launch_qk_norm_rotary(const lunarad_qk_norm_rotary_args& a, cudaStre
   return run_rows_dtype<true, false, false>(q, 2, static_cast<int>(a.rotary.layout), a.dtype, stream);
 }
 
-cudaError_t launch_kv_append(const lunarad_kv_append_args& a, cudaStream_t stream) {
+cudaError_t launch_kv_append(const lunarad_kv_append_args& a, bool zero_rest, cudaStream_t stream) {
   const lunarad_cache& c = *a.cache;
   const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
   QuantParams q{};
@@ -746,12 +756,13 @@ cudaError_t launch_kv_append(const lunarad_kv_append_args& a, cudaStream_t strea
   p.dim = static_cast<int>(c.dim);
   p.tokens = static_cast<int>(a.seqs.tokens);
   p.seq = p.tokens;
+  p.zero_rest = zero_rest;
   const int layout = static_cast<int>(a.rotary.layout);
   return e2m1 ? run_rows_dtype<false, true, true>(q, n, layout, a.dtype, stream)
               : run_rows_dtype<false, true, false>(q, n, layout, a.dtype, stream);
 }
 
-cudaError_t launch_kv_read(const lunarad_kv_read_args& a, cudaStream_t stream) {
+cudaError_t launch_kv_read(const lunarad_kv_read_args& a, bool zero_rest, cudaStream_t stream) {
   const lunarad_cache& c = *a.cache;
   ReadParams p{};
   p.seqs = make_seqs(a.seqs, c.page_size);
@@ -775,6 +786,7 @@ cudaError_t launch_kv_read(const lunarad_kv_read_args& a, cudaStream_t stream) {
   p.dim = static_cast<int>(c.dim);
   p.num_pages = static_cast<int>(c.num_pages);
   p.tokens = static_cast<int>(a.seqs.tokens);
+  p.zero_rest = zero_rest;
   const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
   if (a.dtype == LUNARA_F16) return run_read_kind<__half>(p, e2m1, stream);
   if (a.dtype == LUNARA_BF16) return run_read_kind<__nv_bfloat16>(p, e2m1, stream);

@@ -26,6 +26,8 @@ B_KN, B_NK = 0, 1
 # lunarad_rotary_layout and the cache kind beside lunara_dtype
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 KIND_E2M1 = 16
+# Flag beside the dtype: output rows of no sequence are zeroed
+ZERO_REST = 0x100
 
 # Every exported symbol with its ctypes signature; the header declares exactly these.
 _p, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float

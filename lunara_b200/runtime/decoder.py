@@ -13,8 +13,8 @@ Ragged batches: the tokens of all sequences stand one behind the other;
 [batch] how long each sequence is with them, ``page_table`` int32 [batch, max_pages] which
 page holds its positions ``page_size * i`` onwards. Token ``i`` of ``n`` has position
 ``seq_len - n + i``; a negative one marks padding (written nowhere, zero in outputs).
-Tokens behind ``seq_starts[batch]`` belong to no sequence; their output rows are left as
-they were. All three live on the device, so a captured graph follows their contents. What
+Tokens behind ``seq_starts[batch]`` belong to no sequence; their rows are left as they were
+in an output that is given, and zero in one that the call allocates. All three live on the device, so a captured graph follows their contents. What
 is wrong in them (a page outside the cache, a position outside the tables) is kept as a
 device error (``ops.device_error()``) and treated as padding, never as an access out of
 bounds.
@@ -110,6 +110,15 @@ def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
         assert 0 not in st or all(s != 0 or n <= 1 for n, s in zip(out.shape, st)), \
             f"{name} is an expanded view; it cannot be written"
     return out, (out.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (out.data_ptr(), 0, st[1], st[0])
+
+
+def _zero_rest(out: torch.Tensor, batch: int) -> int:
+    """For an output in fresh memory: the flag that zeroes the rows of no sequence. Where there is no
+    sequence at all no kernel runs, and the rows are cleared here."""
+    if batch == 0:
+        out.zero_()
+        return 0
+    return _lib.ZERO_REST
 
 
 # ───────────────────────────────────────────────────────────── rotary ──
@@ -282,9 +291,13 @@ def kv_append(K: torch.Tensor, V: torch.Tensor, cache: PagedKVCache, page_table:
         assert out_q is None, "out_q without Q"
     seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
     device = _check_device(cache.k_pages, K, V, table, Q, out_q, page_table, seq_starts, seq_lens)
+    rest = 0
     if Q is not None:
+        fresh = out_q is None
         out_q, o = _output(out_q, Q, "out_q")
-    _call("lunarad_kv_append", _APPEND.pack(*k, *v, *q, *o, cache._address, *seqs, *rot, q_heads, code), device)
+        if fresh:
+            rest = _zero_rest(out_q, seqs[5])
+    _call("lunarad_kv_append", _APPEND.pack(*k, *v, *q, *o, cache._address, *seqs, *rot, q_heads, code | rest), device)
     return out_q
 
 
@@ -292,7 +305,7 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Ten
             dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of the last ``seq_starts[b + 1] - seq_starts[b]`` positions of each
     sequence as dense [tokens, kv_heads, D] tensors, in the cache's dtype (``dtype``, float16 by
-    default, for a 4-bit one)."""
+    default, for a 4-bit one); zeros where a token is padding or no sequence's."""
     if dtype is None:
         dtype = torch.float16 if cache.dtype is None else cache.dtype
     assert cache.dtype is None or dtype == cache.dtype, f"a {cache.dtype} cache is read as such, not as {dtype}"
@@ -301,7 +314,8 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, seq_starts: torch.Ten
     device = _check_device(cache.k_pages, page_table, seq_starts, seq_lens)
     k = cache.k_pages.new_empty((tokens, cache.kv_heads, cache.head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    _call("lunarad_kv_read", _READ.pack(k.data_ptr(), v.data_ptr(), cache._address, *seqs, _dtype_code(k)), device)
+    code = _dtype_code(k) | _zero_rest(k, seqs[5]) | _zero_rest(v, seqs[5])
+    _call("lunarad_kv_read", _READ.pack(k.data_ptr(), v.data_ptr(), cache._address, *seqs, code), device)
     return k, v
 
 
@@ -323,10 +337,12 @@ def paged_attention(Q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     code = _dtype_code(Q)
     seqs = _sequences(page_table, seq_starts, seq_lens, tokens)
     device = _check_device(cache.k_pages, Q, out, page_table, seq_starts, seq_lens)
+    fresh = out is None
     out, o = _output(out, Q, "out")
+    rest = _zero_rest(out, seqs[5]) if fresh else 0
     if scale is None:
         scale = dim ** -0.5
-    args = _ATTENTION.pack(*q, *o, cache._address, *seqs, q_heads, window, max_q_len or 0, code, scale)
+    args = _ATTENTION.pack(*q, *o, cache._address, *seqs, q_heads, window, max_q_len or 0, code | rest, scale)
     need = _lib.load().lunarad_paged_attention_workspace(args, device)
     if need < 0:
         _lib.check(-need)

@@ -1,0 +1,28 @@
+"""More of the decoder operators on CPU: flags and refusals of the C ABI."""
+
+from lunara_b200.runtime import _lib, decoder
+from test_decoder_cpu import SEQS, VIEW, append, attention, cache, err, qk_norm, read, rotary
+
+
+def test_zero_rest_is_a_flag_of_the_ragged_calls():
+    flag = _lib.ZERO_REST
+    for call in (append, read, attention):
+        assert call(seqs=(16, 16, 16, 8, 8, 2, 0), dtype=flag) == _lib.OK
+        assert call(seqs=(0, 0, 0, 8, 8, 0, 5), dtype=flag) == _lib.ERR_INVALID_ARG and "no sequence" in err()
+        assert call(dtype=flag | 7) == _lib.ERR_INVALID_ARG and "dtype" in err()
+        assert call(dtype=flag << 1) == _lib.ERR_INVALID_ARG and "dtype" in err()
+        assert call(dtype=flag | _lib.BF16) == _lib.ERR_INVALID_ARG and "differ" in err()
+    for call in (rotary, qk_norm):
+        assert call(dtype=flag) == _lib.ERR_INVALID_ARG and "dtype" in err()
+    c = cache()
+    packed = [decoder._ATTENTION.pack(*VIEW, *VIEW, c, *SEQS, 4, 0, 0, f, 0.1) for f in (0, flag)]
+    lib = _lib.load()
+    assert lib.lunarad_paged_attention_workspace(packed[0], 0) == lib.lunarad_paged_attention_workspace(packed[1], 0) > 0
+
+
+def test_null_arguments_refused():
+    lib = _lib.load()
+    for call in (lib.lunarad_rotary, lib.lunarad_qk_norm_rotary, lib.lunarad_kv_append, lib.lunarad_kv_read):
+        assert call(None, None) == _lib.ERR_INVALID_ARG and "NULL" in err()
+    assert lib.lunarad_paged_attention(None, None, 0, None) == _lib.ERR_INVALID_ARG and "NULL" in err()
+    assert lib.lunarad_paged_attention_workspace(None, 0) == -_lib.ERR_INVALID_ARG and "NULL" in err()

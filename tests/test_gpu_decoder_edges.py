@@ -178,3 +178,29 @@ def test_4bit_queries_at_the_upper_end(dim):
     q = q.clamp(-2.0 ** 126, 2.0 ** 126)
     q[:, :, 3] = 1.5 * 2.0 ** 127 * (1 - 2 * torch.randint(0, 2, q.shape[:2], generator=p.g))
     check_attention(p, 4, scale=2.0 ** -126, q=q.to(BF16))
+
+
+@pytest.mark.parametrize("bits,dim,dtype", [(16, 64, BF16), (4, 128, F16), (16, 20, F16), (16, 64, F32), (4, 48, BF16)])
+@pytest.mark.parametrize("lens", [[(1, 17), (0, 3), (1, 300)], [(100, 130), (0, 0)], [(0, 5), (0, 0)], []])
+def test_rows_of_no_sequence_are_zero_in_new_outputs(lens, bits, dim, dtype):
+    """Padded batches: memory that the call allocates holds nothing of what stood there before."""
+    ops = _ops()
+    p = ref.Paged(lens, 2, dim, 16, dtype, seed=18, bits=bits, extra_tokens=5)
+    cache, _ = cache_of(p)
+    k = torch.randn(p.tokens, 2, dim, generator=p.g).to(dtype).cuda()
+    q = p.queries(4).cuda()
+
+    def fresh(call, shape):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        dirt = [torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(4)]
+        del dirt
+        got = call()
+        for out in got if isinstance(got, tuple) else (got,):
+            assert out.shape == shape and (out[p.owned:] == 0).all()
+            assert torch.isfinite(out).all()
+
+    fresh(lambda: ops.kv_append(k, k, cache, *where(p), Q=q, table=ops.rotary_table(400, 16)), tuple(q.shape))
+    fresh(lambda: ops.kv_read(cache, *where(p), tokens=p.tokens, dtype=dtype), (p.tokens, 2, dim))
+    fresh(lambda: ops.paged_attention(q, cache, *where(p)), tuple(q.shape))
+    assert ops.device_error() == 0
