@@ -23,7 +23,9 @@ _CACHE = struct.Struct("17q2d")   # lunarad_cache
 class PagedKVCache:
     """Keys and values of one layer. The tensors stay the caller's and may be views
     (for instance ``all_layers[i]`` or ``kv[:, 0]``) as long as each page's head holds
-    its ``[page_size, head_dim]`` contiguously."""
+    its ``[page_size, head_dim]`` contiguously. What the kernels take (addresses, strides,
+    sizes, gains) is packed once, so a handle's attributes cannot be assigned to: a pool
+    that has grown gets a new handle."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: Optional[torch.Tensor] = None,
                  v_scales: Optional[torch.Tensor] = None, k_gain: float = 1.0, v_gain: float = 1.0):
@@ -68,6 +70,15 @@ class PagedKVCache:
             v_pages.stride(1), stride(ks, 0), stride(ks, 1), stride(vs, 0), stride(vs, 1), self.num_pages, self.kv_heads,
             self.page_size, self.head_dim, kind, self.k_gain, self.v_gain)
         self._address = _lib.address_of(self._args)
+        self._packed = True
+
+    def __setattr__(self, name: str, value) -> None:
+        if "_packed" in self.__dict__:
+            raise AttributeError(f"a PagedKVCache keeps its tensors' addresses: make a new one instead of assigning {name}")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name: str) -> None:
+        raise AttributeError(f"a PagedKVCache keeps its tensors' addresses: {name} cannot be deleted")
 
     @staticmethod
     def _check_inner(t: torch.Tensor) -> None:

@@ -1,6 +1,8 @@
-"""More of the decoder operators on CPU: flags and refusals of the C ABI."""
+"""More of the decoder operators on CPU: flags and refusals of the C ABI, the cache handle."""
+import pytest
+import torch
 
-from lunara_b200.runtime import _lib, decoder
+from lunara_b200.runtime import _lib, decoder, ops
 from test_decoder_cpu import SEQS, VIEW, append, attention, cache, err, qk_norm, read, rotary
 
 
@@ -26,3 +28,16 @@ def test_null_arguments_refused():
         assert call(None, None) == _lib.ERR_INVALID_ARG and "NULL" in err()
     assert lib.lunarad_paged_attention(None, None, 0, None) == _lib.ERR_INVALID_ARG and "NULL" in err()
     assert lib.lunarad_paged_attention_workspace(None, 0) == -_lib.ERR_INVALID_ARG and "NULL" in err()
+
+
+def test_cache_handles_cannot_be_changed():
+    """The kernels get packed addresses: another tensor in an attribute would be ignored, and the old one's memory freed."""
+    for kind in (torch.float16, "e2m1"):
+        c = ops.PagedKVCache.allocate(4, 2, 8, 64, dtype=kind, device="cpu")
+        pages = c.k_pages
+        for name in ("k_pages", "v_pages", "k_scales", "v_scales", "k_gain", "num_pages", "page_size", "head_dim", "dtype", "other"):
+            with pytest.raises(AttributeError, match="new one"):
+                setattr(c, name, torch.zeros(8, 2, 8, 64))
+        with pytest.raises(AttributeError):
+            del c.k_pages
+        assert c.k_pages is pages and c.num_pages == 4
