@@ -80,6 +80,10 @@ class PagedKVCache:
     def __delattr__(self, name: str) -> None:
         raise AttributeError(f"a PagedKVCache keeps its tensors' addresses: {name} cannot be deleted")
 
+    def __reduce__(self):
+        """Copies and unpickled handles are made anew, from their own tensors' addresses."""
+        return type(self), (self.k_pages, self.v_pages, self.k_scales, self.v_scales, self.k_gain, self.v_gain)
+
     @staticmethod
     def _check_inner(t: torch.Tensor) -> None:
         _, _, slots, width = t.shape

@@ -1,8 +1,12 @@
 """More of the decoder operators on CPU: flags and refusals of the C ABI, the cache handle."""
+import copy
+import ctypes
+import pickle
+
 import pytest
 import torch
 
-from lunara_b200.runtime import _lib, decoder, ops
+from lunara_b200.runtime import _lib, decoder, kv_cache, ops
 from test_decoder_cpu import SEQS, VIEW, append, attention, cache, err, qk_norm, read, rotary
 
 
@@ -41,3 +45,21 @@ def test_cache_handles_cannot_be_changed():
         with pytest.raises(AttributeError):
             del c.k_pages
         assert c.k_pages is pages and c.num_pages == 4
+
+
+@pytest.mark.parametrize("kind", [torch.float32, "e2m1"])
+def test_copies_of_cache_handles_have_their_own_addresses(kind):
+    """A deep copy, and a handle that was pickled, point at their own tensors; a shallow one shares them."""
+    c = ops.PagedKVCache.allocate(4, 2, 8, 64, dtype=kind, device="cpu")
+    if kind == "e2m1":   # scales as bytes: torch does not load float8 tensors from a plain pickle
+        c = ops.PagedKVCache(c.k_pages, c.v_pages, c.k_scales.view(torch.uint8), c.v_scales.view(torch.uint8), k_gain=0.5, v_gain=3.0)
+    c.k_pages.random_(0, 200)
+    shallow = copy.copy(c)
+    assert shallow.k_pages is c.k_pages and shallow._args == c._args
+    for other in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert torch.equal(other.k_pages, c.k_pages) and other.k_pages.data_ptr() != c.k_pages.data_ptr()
+        fields = kv_cache._CACHE.unpack(other._args)
+        tensors = (other.k_pages, other.v_pages) + ((other.k_scales, other.v_scales) if kind == "e2m1" else ())
+        assert fields[:len(tensors)] == tuple(t.data_ptr() for t in tensors)
+        assert fields[4:] == kv_cache._CACHE.unpack(c._args)[4:]
+        assert ctypes.string_at(other._address, len(other._args)) == other._args
