@@ -71,7 +71,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: int, scale:
     """One sequence in 64 bits: q [n, heads, dim] at positions first.., k and v [length, kv_heads, dim].
 
     Returns (o, spread, reach): the output, sum_j p_j |v_j| (what a relative error of the
-    probabilities can move it by), and the largest scale * sum |q||k| over visible keys
+    probabilities can move it by), and the largest |scale| sum |q||k| over visible keys
     (what rounding moves a score by, times its relative error). A row that sees no key is 0."""
     n, heads, dim = q.shape
     group = heads // k.shape[1]
@@ -87,7 +87,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: int, scale:
     p = torch.exp(s - torch.where(torch.isinf(top), torch.zeros_like(top), top))
     p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
     p = p * seen
-    reach = (q.abs() @ k.abs().transpose(1, 2) * scale * seen).amax(-1) if s.shape[-1] else torch.zeros(heads, n, dtype=F64)
+    reach = (q.abs() @ k.abs().transpose(1, 2) * abs(scale) * seen).amax(-1) if s.shape[-1] else torch.zeros(heads, n, dtype=F64)
     # Unseen values take no part even where they are not finite.
     return ((p @ torch.nan_to_num(v)).transpose(0, 1), (p @ torch.nan_to_num(v).abs()).transpose(0, 1), reach.transpose(0, 1))
 

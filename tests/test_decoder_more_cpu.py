@@ -1,4 +1,5 @@
-"""More of the decoder operators on CPU: flags and refusals of the C ABI, the cache handle."""
+"""More of the decoder operators on CPU: flags and refusals of the C ABI, the cache handle, the oracle's
+bounds."""
 import copy
 import ctypes
 import pickle
@@ -7,6 +8,7 @@ import pytest
 import torch
 
 from lunara_b200.runtime import _lib, decoder, kv_cache, ops
+from oracle import decoder as ref
 from test_decoder_cpu import SEQS, VIEW, append, attention, cache, err, qk_norm, read, rotary
 
 
@@ -63,3 +65,15 @@ def test_copies_of_cache_handles_have_their_own_addresses(kind):
         assert fields[:len(tensors)] == tuple(t.data_ptr() for t in tensors)
         assert fields[4:] == kv_cache._CACHE.unpack(c._args)[4:]
         assert ctypes.string_at(other._address, len(other._args)) == other._args
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.3])
+def test_the_oracles_reach_bounds_every_score(scale):
+    """`reach`, from which the attention's tolerance takes the scores' rounding, is scale's magnitude times sum |q||k|, whatever its sign."""
+    g = torch.Generator().manual_seed(1)
+    q, k = torch.randn(3, 2, 16, generator=g), torch.randn(7, 1, 16, generator=g)
+    reach = ref.attend(q, k, k, 4, scale)[2]
+    for i in range(3):
+        for h in range(2):
+            sums = [float((q[i, h].double().abs() * k[j, 0].double().abs()).sum()) for j in range(4 + i + 1)]
+            assert float(reach[i, h]) == pytest.approx(0.3 * max(sums), rel=1e-12)
