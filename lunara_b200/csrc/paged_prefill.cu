@@ -593,7 +593,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2)
             mxp[(e >> 1) & 7] = fmax3_nan(mxp[(e >> 1) & 7], __uint_as_float(sc[cc][e]), __uint_as_float(sc[cc][e + 1]));
-        const float mx = fmax3_nan(fmax3_nan(mxp[0], mxp[1], mxp[2]), fmax3_nan(mxp[3], mxp[4], mxp[5]), fmax_nan(mxp[6], mxp[7]));
+        float mx = fmax3_nan(fmax3_nan(mxp[0], mxp[1], mxp[2]), fmax3_nan(mxp[3], mxp[4], mxp[5]), fmax_nan(mxp[6], mxp[7]));
+        // inf - inf makes NaN of a row with a score of +inf, as its softmax is; the
+        // cubic's clamp would drop it where such a key stands in its columns.
+        if (mx == INFINITY) mx = NAN;
         if (j == 0) {
           top = mx;
           off = mx * sl2;

@@ -204,3 +204,43 @@ def test_rows_of_no_sequence_are_zero_in_new_outputs(lens, bits, dim, dtype):
     fresh(lambda: ops.kv_read(cache, *where(p), tokens=p.tokens, dtype=dtype), (p.tokens, 2, dim))
     fresh(lambda: ops.paged_attention(q, cache, *where(p)), tuple(q.shape))
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (64, F16), (20, BF16), (64, F32)])
+@pytest.mark.parametrize("lens", [[(100, 300), (40, 128)], [(2, 300), (1, 128)]])
+def test_infinite_scores(lens, dim, dtype):
+    """A row with a score of +inf, or 0 * inf, has no softmax and is NaN, in whichever column of a block that key stands;
+    a score of -inf weighs nothing; a row whose scores are all -inf is zero."""
+    ops = _ops()
+    p = ref.Paged(lens, 1, dim, 16, dtype, seed=22)
+    keys = [0, 1, 7, 8, 9, 16, 33, 64, 70, 101, 127]
+    for at in keys:   # one at a time; the queries' first elements are +1, -1 and 0 in turn
+        q = p.queries(3)
+        q[:, :, 0] = torch.tensor([1.0, -1.0, 0.0])
+        for b, (_, whole) in enumerate(p.lens):
+            k = p.seqs[b][0].clone().to(dtype)
+            k[at, 0, 0] = float("inf")
+            p.put("k", b, torch.arange(whole), k)
+        cache, _ = cache_of(p)
+        out = ops.paged_attention(q.cuda(), cache, *where(p)).cpu()
+        row = 0
+        for b, (n, whole) in enumerate(p.lens):
+            k, v = p.seqs[b]
+            for i in range(n):
+                pos = whole - n + i
+                if pos < at:
+                    assert torch.isfinite(out[row]).all(), (at, b, i)
+                else:
+                    assert out[row, 0].isnan().all() and out[row, 2].isnan().all(), (at, b, i)
+                    keep = [j for j in range(pos + 1) if j != at]
+                    want = ref.attend(q[row:row + 1, 1:2], k[keep], v[keep], len(keep) - 1, dim ** -0.5)[0] if keep else torch.zeros(1, 1, dim)
+                    assert ((out[row, 1].double() - want[0, 0]).abs() <= 2.0 ** -6 * (want[0, 0].abs() + 1)).all(), (at, b, i)
+                row += 1
+    for b, (_, whole) in enumerate(p.lens):
+        k = p.seqs[b][0].clone().to(dtype)
+        k[:, 0, 0] = float("inf")
+        p.put("k", b, torch.arange(whole), k)
+    q = p.queries(3)
+    q[:, :, 0] = -1
+    cache, _ = cache_of(p)
+    assert (ops.paged_attention(q.cuda(), cache, *where(p)) == 0).all()
