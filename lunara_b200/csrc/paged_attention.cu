@@ -419,8 +419,9 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         constexpr int kPieces = DP / 32;   // 16-byte pieces of a row of codes
         const int piece = lane % kPieces, in_group = (lane / kPieces) & 7;
         const bool lane_in = EXACT || 16 * piece < row_bytes;
-        const char* kl = kb + in_group * row_bytes + 16 * piece;
-        const char* vl = vb + in_group * row_bytes + 16 * piece;
+        const int from = in_group * row_bytes + (lane_in ? 16 * piece : 0);   // (a copy of nothing names a place in the cache too)
+        const char* kl = kb + from;
+        const char* vl = vb + from;
 #pragma unroll
         for (int j = 0; j < KT * kPieces / 32; ++j) {
           const int local = (lane + 32 * j) / kPieces, src = g0 + (local >> 3);
@@ -443,11 +444,12 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
         constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
         const int piece = lane % kPieces, sub = lane / kPieces;
         const bool lane_in = EXACT || 16 * piece < row_bytes;
+        const int from = lane_in ? 16 * piece : 0;
 #pragma unroll
         for (int i8 = 0; i8 < KT / 8; ++i8) {
           const uint32_t ka = __shfl_sync(0xffffffffu, k_at, (g0 + i8) & 31), va = __shfl_sync(0xffffffffu, v_at, (g0 + i8) & 31);
-          const char* kg = place(kb + sub * row_bytes + 16 * piece, ka);
-          const char* vg = place(vb + sub * row_bytes + 16 * piece, va);
+          const char* kg = place(kb + sub * row_bytes + from, ka);
+          const char* vg = place(vb + sub * row_bytes + from, va);
 #pragma unroll
           for (int it = 0; it < 8 / kAtOnce; ++it) {
             const int r = it * kAtOnce + sub, local = 8 * i8 + r;
@@ -455,8 +457,8 @@ __global__ void __launch_bounds__(kStreamThreads, Shape<E2M1, DP, NT>::kCtasPerS
             const char* ksrc = kg + it * kAtOnce * row_bytes;
             const char* vsrc = vg + it * kAtOnce * row_bytes;
             if (!grouped) {   // every row by its own page
-              ksrc = place(kb + 16 * piece, __shfl_sync(0xffffffffu, k_at, local));
-              vsrc = place(vb + 16 * piece, __shfl_sync(0xffffffffu, v_at, local));
+              ksrc = place(kb + from, __shfl_sync(0xffffffffu, k_at, local));
+              vsrc = place(vb + from, __shfl_sync(0xffffffffu, v_at, local));
             }
             copy_async(at + k_place<S, false>(local, piece), ksrc, in);
             copy_async(at + S::kKBytes + v_place<S, false>(local, piece), vsrc, in);
@@ -882,11 +884,12 @@ int place_unit(const lunarad_cache& c) {
 }
 
 // 16-byte copies of whole rows: aligned bases and strides, rows of 16-byte
-// pieces; for 4 bits also pages of whole groups of 8 keys.
+// pieces; for 4 bits also pages of whole groups of 8 keys. A cache without pages
+// has no place that a copy of nothing could name.
 bool stream_ok(const lunarad_paged_attention_args& a) {
   const lunarad_cache& c = *a.cache;
   const bool e2m1 = c.kind == LUNARAD_KIND_E2M1;
-  if (a.dtype == LUNARA_F32 || c.dim > 128) return false;
+  if (a.dtype == LUNARA_F32 || c.dim > 128 || c.num_pages == 0) return false;
   if (!al16(a.q.data) || a.q.head_stride % 8 || a.q.seq_stride % 8) return false;
   if (!al16(a.o.data) || a.o.head_stride % 8 || a.o.seq_stride % 8) return false;
   if (!al16(c.k) || !al16(c.v) || place_unit(c) == 0) return false;

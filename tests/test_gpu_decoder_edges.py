@@ -244,3 +244,18 @@ def test_infinite_scores(lens, dim, dtype):
     q[:, :, 0] = -1
     cache, _ = cache_of(p)
     assert (ops.paged_attention(q.cuda(), cache, *where(p)) == 0).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_cache_without_pages(bits):
+    """Every key's page is outside the cache: recorded, and all rows are zero."""
+    ops = _ops()
+    cache = ops.PagedKVCache.allocate(0, 2, 16, 64, dtype="e2m1" if bits == 4 else F16)
+    tab, starts, lens = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0] * 8], [0, 60], [100]))
+    q = torch.randn(60, 4, 64, device="cuda", dtype=F16)
+    out = ops.paged_attention(q, cache, tab, starts, lens)
+    assert ops.device_error() == 0x502 and (out == 0).all()
+    assert ops.kv_append(q[:, :2], q[:, 2:], cache, tab, starts, lens) is None
+    assert ops.device_error() == 0x502
+    k, v = ops.kv_read(cache, tab, starts, lens, tokens=60, dtype=F16)
+    assert ops.device_error() == 0x502 and (k == 0).all() and (v == 0).all()
