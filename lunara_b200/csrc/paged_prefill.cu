@@ -319,7 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     t_end = run_start(total, workers, worker + 1);
     if (threadIdx.x == 0) s_cursor.seek(p, prefix, t_first);
   }
-  __syncthreads();   // the prefix sums are used up: the ring may be written
+  // The prefix sums are used up: the ring may be written, by TMA too, whose
+  // writes have no order with the plain ones before them without the fence.
+  fence_proxy_async_smem();
+  __syncthreads();
 
   if (warp >= 10) {
     reg_dealloc<kOtherRegs>();
