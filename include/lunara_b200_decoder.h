@@ -170,6 +170,7 @@ int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream);
  * included. A value (not a key) that is not finite and that only some of the
  * call's tokens of a sequence see may also reach those that do not. Keys of a page outside the cache
  * (0x502) are left out, and a length outside the page table (0x503) is cut.
+ * scale, times the keys' gain of an e2m1 cache and log2(e), is a finite fp32 number.
  * max_q_len: the longest sequence's number of tokens if known (0 = unknown);
  * it only steers the choice of kernels.
  * workspace: device memory of lunarad_paged_attention_workspace() bytes or

@@ -120,6 +120,10 @@ int check_attention(const char* fn, const lunarad_paged_attention_args* a) {
   if (a->window < 0 || a->window >= kMaxSlots) return fail(LUNARA_ERR_INVALID_ARG, "%s: bad window", fn);
   if (a->max_q_len < 0) return fail(LUNARA_ERR_INVALID_ARG, "%s: negative max_q_len", fn);
   if (!std::isfinite(a->scale)) return fail(LUNARA_ERR_INVALID_ARG, "%s: scale is not finite", fn);
+  // The kernels hold scale * gain, and that times log2(e), in fp32.
+  const double factor = a->scale * (c.kind == LUNARAD_KIND_E2M1 ? c.k_gain : 1.0);
+  if (!std::isfinite(static_cast<float>(1.4426950408889634 * factor)))
+    return fail(LUNARA_ERR_INVALID_ARG, "%s: scale %g (with the keys' gain %g) is not finite in fp32", fn, a->scale, factor);
   return LUNARA_OK;
 }
 

@@ -77,3 +77,11 @@ def test_the_oracles_reach_bounds_every_score(scale):
         for h in range(2):
             sums = [float((q[i, h].double().abs() * k[j, 0].double().abs()).sum()) for j in range(4 + i + 1)]
             assert float(reach[i, h]) == pytest.approx(0.3 * max(sums), rel=1e-12)
+
+
+@pytest.mark.parametrize("scale,gain,ok", [(1e39, 1.0, False), (-1e300, 1.0, False), (3e38, 1.0, False), (1e30, 1e10, False), (2e38, 1.0, True),
+                                           (1e39, 0.1, True), (1e-300, 1.0, True), (0.0, 1.0, True)])
+def test_scales_beyond_fp32_refused(scale, gain, ok):
+    """Accepted ones get as far as the workspace that these calls lack."""
+    for kind in (_lib.KIND_E2M1, _lib.F16) if gain == 1.0 else (_lib.KIND_E2M1,):
+        assert attention(c=cache(kind=kind, gain=gain), scale=scale) == _lib.ERR_INVALID_ARG and ("workspace" if ok else "fp32") in err(), err()
