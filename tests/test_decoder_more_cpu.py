@@ -2,6 +2,7 @@
 bounds."""
 import copy
 import ctypes
+import math
 import pickle
 
 import pytest
@@ -85,3 +86,28 @@ def test_scales_beyond_fp32_refused(scale, gain, ok):
     """Accepted ones get as far as the workspace that these calls lack."""
     for kind in (_lib.KIND_E2M1, _lib.F16) if gain == 1.0 else (_lib.KIND_E2M1,):
         assert attention(c=cache(kind=kind, gain=gain), scale=scale) == _lib.ERR_INVALID_ARG and ("workspace" if ok else "fp32") in err(), err()
+
+
+@pytest.mark.parametrize("rot,base,original,factor,fast,slow", [(128, 10000.0, 4096, 16.0, 32.0, 1.0), (64, 500000.0, 8192, 8.0, 32.0, 1.0),
+                                                                 (80, 10000.0, 2048, 4.0, 24.0, 2.0)])
+def test_yarn_ramp(rot, base, original, factor, fast, slow):
+    """Every frequency against the definition, by bisection instead of logarithms: frequency i turns
+    original / (2 pi) * base^(-2 i / rot) times. Indices up to the last whole one with at least `fast` turns are kept, those from
+    the first whole one with at most `slow` turns on are divided by the factor, a straight line lies between."""
+    turns = lambda i: original / (2 * math.pi) * base ** (-2 * i / rot)  # noqa: E731
+    low = max(i for i in range(rot) if turns(i) >= fast)
+    high = min(i for i in range(rot) if turns(i) <= slow)
+    assert 0 < low < high < rot // 2 + 8
+    scaling = {"type": "yarn", "factor": factor, "original_positions": original, "beta_fast": fast, "beta_slow": slow, "amplitude": 1.0}
+    t = ops.rotary_table(2, rot, base=base, scaling=scaling, device="cpu")
+    got = torch.atan2(t[1, :, 1].double(), t[1, :, 0].double())
+    seen = set()
+    for i in range(rot // 2):
+        f = base ** (-2 * i / rot)
+        share = 0.0 if i <= low else 1.0 if i >= high else (i - low) / (high - low)
+        seen.add(0 < share < 1)
+        want = f * (1 - share) + f / factor * share
+        # An entry is off by half a step: 2^-24 of it, 2^-25 at most (below 1); the angle by no more than both together.
+        assert abs(float(got[i]) - want) <= 2.0 ** -24, i
+        assert abs(float(t[1, i, 1]) - math.sin(want)) <= 2.0 ** -24 * abs(math.sin(want)) + 1e-15, i
+    assert seen == {True, False}

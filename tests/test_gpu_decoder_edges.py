@@ -206,6 +206,30 @@ def test_rows_of_no_sequence_are_zero_in_new_outputs(lens, bits, dim, dtype):
     assert ops.device_error() == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_sequences_with_prompts_among_them(dim):
+    """More sequences than one launch plans for, with prompts (tcgen05) among single tokens in each share of them."""
+    g = torch.Generator().manual_seed(19)
+    lens = [(int(n), int(n) + int(w)) for n, w in zip(torch.randint(0, 3, (2100,), generator=g), torch.randint(0, 40, (2100,), generator=g))]
+    for b, pair in {3: (40, 300), 1023: (70, 70), 1024: (33, 500), 1500: (17, 400), 1501: (200, 1000), 2047: (16, 90), 2048: (130, 130),
+                    2099: (64, 700)}.items():
+        lens[b] = pair
+    p = ref.Paged(lens, 1, dim, 8, F16, seed=20, extra_tokens=2)
+    check_attention(p, 2)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("n,group", [(1, 1), (1, 8), (2, 8)])
+def test_one_long_sequence_of_one_key_head(n, group, bits):
+    """All of the GPU's warps share one row tile, whose join has over a thousand parts."""
+    ops = _ops()
+    p = ref.Paged([(n, 50000)], 1, 128, 32, BF16, seed=n + group, bits=bits)
+    q = p.queries(group)
+    out = check_attention(p, group, q=q)
+    cache, _ = cache_of(p)
+    assert torch.equal(ops.paged_attention(q.cuda(), cache, *where(p)), out)
+
+
 @pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (64, F16), (20, BF16), (64, F32)])
 @pytest.mark.parametrize("lens", [[(100, 300), (40, 128)], [(2, 300), (1, 128)]])
 def test_infinite_scores(lens, dim, dtype):
@@ -244,6 +268,44 @@ def test_infinite_scores(lens, dim, dtype):
     q[:, :, 0] = -1
     cache, _ = cache_of(p)
     assert (ops.paged_attention(q.cuda(), cache, *where(p)) == 0).all()
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, BF16), (4, BF16), (16, F32)])
+def test_caches_beyond_4_gib(bits, dtype):
+    """Pages whose bytes stand beyond 2^32: the operators do there what they do in a small cache."""
+    ops = _ops()
+    heads, dim, page = 2, 128, 16
+    row = {(16, BF16): 256, (4, BF16): 64, (16, F32): 512}[bits, dtype]
+    far = (5 << 30) // (heads * page * row)
+    small = ops.PagedKVCache.allocate(64, heads, page, dim, dtype="e2m1" if bits == 4 else dtype)
+    tensors = [t for t in (small.k_pages, small.v_pages, small.k_scales, small.v_scales) if t is not None]
+    big = ops.PagedKVCache(*(torch.empty(far + 64, *t.shape[1:], dtype=t.dtype, device="cuda") for t in tensors))
+    g = torch.Generator().manual_seed(23)
+    order = torch.randperm(64, generator=g).int()
+    tab = torch.full((3, 20), -1, dtype=torch.int32)
+    lens, new = [300, 17, 260], [200, 17, 1]
+    at = 0
+    for b, n in enumerate(lens):
+        need = -(-n // page)
+        tab[b, :need] = order[at:at + need]
+        at += need
+    starts = torch.tensor([0] + lens).cumsum(0).int().cuda()
+    whole = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(sum(lens), heads, dim, generator=g).to(dtype).cuda() for _ in range(2))
+    tabs = tab.cuda(), torch.where(tab >= 0, tab + far, tab).cuda()
+    out = []
+    for cache, t in zip((small, big), tabs):
+        ops.kv_append(k, v, cache, t, starts, whole)
+        got = list(ops.kv_read(cache, t, starts, whole, tokens=sum(lens), dtype=dtype))
+        for count in (new, [1, 1, 1]):
+            s = torch.tensor([0] + count).cumsum(0).int().cuda()
+            q = torch.randn(sum(count), 4, dim, generator=torch.Generator().manual_seed(24)).to(dtype).cuda()
+            got.append(ops.paged_attention(q, cache, t, s, whole))
+        out.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and out[0][2].abs().sum() > 0
+    if bits == 16:
+        assert torch.equal(out[1][0], k) and torch.equal(out[1][1], v)
+    assert ops.device_error() == 0
 
 
 @pytest.mark.parametrize("bits", [16, 4])
