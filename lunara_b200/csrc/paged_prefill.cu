@@ -51,7 +51,10 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr int kLaunchRegs = 168;
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
-constexpr int kPolyPairs = 4;            // of 16 exponential pairs on the FMA pipe, as in attention.cu
+// Of 16 exponential pairs these are on the FMA pipe, as in attention.cu: a cubic,
+// off by 7.5e-5 where rounding a probability to 16 bits is by up to 4.9e-4 (f16)
+// or 3.9e-3 (bf16).
+constexpr int kPolyPairs = 4;
 constexpr int kMaskRing = 16;            // blocks whose key masks are kept; more than the ring can run ahead
 constexpr int kItemRing = 4;             // items whose block counts are kept; the copies run one item ahead at most
 
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_dst = (chunk >> 3) * L::kHalfBytes;
     const int boxes = box_rows > 0 ? kBlock / box_rows : 0;
     const CUtensorMap* map = kv == 0 ? &tk : &tv;
-    if (lane == 0) tma_prefetch_desc(map);
+    if (lane == 0 && boxes > 0) tma_prefetch_desc(map);   // (without boxes there is no map)
     const uint32_t page_u = kv == 0 ? p.k_page_u : p.v_page_u;
     bool ok = true;
     Cursor cur = s_cursor;

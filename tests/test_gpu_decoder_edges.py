@@ -321,3 +321,29 @@ def test_a_cache_without_pages(bits):
     assert ops.device_error() == 0x502
     k, v = ops.kv_read(cache, tab, starts, lens, tokens=60, dtype=F16)
     assert ops.device_error() == 0x502 and (k == 0).all() and (v == 0).all()
+
+
+@pytest.mark.parametrize("bits,dim,dtype", [(16, 64, BF16), (4, 128, F16), (16, 20, F16)])
+@pytest.mark.parametrize("lens", [[(1, 17), (1, 300)], [(100, 130), (3, 50)]])
+def test_tokens_before_the_first_sequence(lens, bits, dim, dtype):
+    """Sequences that begin behind the call's first tokens: those rows are left, or zero in a new output, the others as ever."""
+    ops = _ops()
+    p = ref.Paged(lens, 2, dim, 16, dtype, seed=25, bits=bits, extra_tokens=4)
+    q = p.queries(4).cuda()
+    k = torch.randn(p.tokens, 2, dim, generator=p.g).to(dtype).cuda()
+    table = ops.rotary_table(400, 16)
+    tab, starts, seq_lens = where(p)
+    n = p.owned
+    moved = lambda x: torch.cat((x[n:], x[:n]))  # noqa: E731  (the four tokens of no sequence to the front)
+    plain, late = cache_of(p)[0], cache_of(p)[0]
+    want = [ops.kv_append(k, k, plain, tab, starts, seq_lens, table=table, Q=q), *ops.kv_read(plain, tab, starts, seq_lens, p.tokens, dtype),
+            ops.paged_attention(q, plain, tab, starts, seq_lens)]
+    at = starts + 4
+    got = [ops.kv_append(moved(k), moved(k), late, tab, at, seq_lens, table=table, Q=moved(q)), *ops.kv_read(late, tab, at, seq_lens, p.tokens, dtype),
+           ops.paged_attention(moved(q), late, tab, at, seq_lens)]
+    for a, b in zip(want, got):
+        assert torch.equal(a[:n], b[4:]) and (b[:4] == 0).all() and (a[n:] == 0).all()
+    out = torch.full_like(q, 7.0)
+    assert torch.equal(ops.paged_attention(moved(q), late, tab, at, seq_lens, out=out)[4:], got[3][4:]) and (out[:4] == 7).all()
+    assert torch.equal(late.k_pages.view(torch.uint8), plain.k_pages.view(torch.uint8))
+    assert ops.device_error() == 0
