@@ -855,7 +855,8 @@ int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
 int row_tiles_of(const lunarad_paged_attention_args& a) {
   const lunarad_cache& c = *a.cache;
   const int64_t mean = (a.seqs.tokens + a.seqs.batch - 1) / a.seqs.batch;
-  const int64_t rows = (a.max_q_len > 0 ? a.max_q_len : mean) * (a.q_heads / c.kv_heads);
+  const int64_t hint = a.max_q_len < a.seqs.tokens ? a.max_q_len : a.seqs.tokens;
+  const int64_t rows = (hint > 0 ? hint : mean) * (a.q_heads / c.kv_heads);
   const double bytes = 4.0 * static_cast<double>(c.kv_heads * c.dim) * static_cast<double>(c.page_size * a.seqs.max_pages) *
                        static_cast<double>(a.seqs.batch);
   return rows <= (c.kind != LUNARAD_KIND_E2M1 && bytes < 200e6 ? 16 : 8) ? 1 : 2;

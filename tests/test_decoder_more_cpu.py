@@ -111,3 +111,11 @@ def test_yarn_ramp(rot, base, original, factor, fast, slow):
         assert abs(float(got[i]) - want) <= 2.0 ** -24, i
         assert abs(float(t[1, i, 1]) - math.sin(want)) <= 2.0 ** -24 * abs(math.sin(want)) + 1e-15, i
     assert seen == {True, False}
+
+
+def test_a_hint_beyond_the_tokens_counts_as_them():
+    """The kernels that a hint chooses show in the workspace; the hint times the heads of a group passes 64 bits here."""
+    c, lib = cache(), _lib.load()
+    need = [lib.lunarad_paged_attention_workspace(decoder._ATTENTION.pack(*VIEW, *VIEW, c, 16, 16, 16, 8, 8, 2, 64, 8, 0, hint, 0, 0.1), 0)
+            for hint in (64, 65, 1 << 62, (1 << 63) - 1, 1)]
+    assert need[0] == need[1] == need[2] == need[3] > need[4] > 0
