@@ -164,12 +164,16 @@ int lunarad_kv_read(const lunarad_kv_read_args* args, void* stream);
  * them). Q and O [tokens, q_heads, dim] (head_stride, seq_stride); query head h
  * reads key head h / (q_heads / kv_heads). fp32 softmax and sums, one rounding
  * of O (16-bit products round the probabilities to the query dtype as
- * well; with an e2m1 cache the products are f16). A row that sees no key, or
- * whose scores are all -inf, is zero. What the cache holds behind a sequence's
- * end, in other pages and outside every row's window has no influence, NaN
- * included. A value (not a key) that is not finite and that only some of the
- * call's tokens of a sequence see may also reach those that do not. Keys of a page outside the cache
- * (0x502) are left out, and a length outside the page table (0x503) is cut.
+ * well; with an e2m1 cache the products are f16; with many query rows a quarter
+ * of the exponentials are off by up to 7.5e-5). A row that sees no key, or whose
+ * scores are all -inf, is zero; one with a score of +inf or NaN is NaN. The sums
+ * of probabilities times values, before the division by theirs, have to be fp32
+ * numbers. Finite values that a row does not see have no influence on it. What
+ * the cache holds behind a sequence's end, in other pages and outside every
+ * row's window has no influence, NaN included. A value (not a key) that is not
+ * finite and that only some of the call's tokens of a sequence see may also
+ * reach those that do not. Keys of a page outside the cache (0x502) are left
+ * out, and a length outside the page table (0x503) is cut. O may be Q.
  * scale, times the keys' gain of an e2m1 cache and log2(e), is a finite fp32 number.
  * max_q_len: the longest sequence's number of tokens if known (0 = unknown);
  * it only steers the choice of kernels.

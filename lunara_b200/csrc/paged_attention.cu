@@ -10,7 +10,8 @@
 // a persistent grid in equal contiguous runs. Bound by HBM: a decode step reads
 // each cached byte once for group * 4 operations per element. Measured on B200:
 // 64 sequences of up to 8191 keys, 32/8 heads of 128 in bf16, 188 us for 1.18 GB
-// (6.3 TB/s); with 4 bits by issue slots: 438 MB of codes in 108 us (4.0 TB/s).
+// (6.3 TB/s); with 4 bits 438 MB of codes in 108 us (4.0 TB/s, 64 % of the issue
+// slots: conversions and products that wait for one another).
 //   * Every warp works alone (no block barrier after the start): it copies its
 //     tiles with cp.async into a ring of its own in shared memory. The order of
 //     the head dimension inside the scores and of the columns of V is free; it is
@@ -22,7 +23,8 @@
 //     while HBM delivers its 23 bytes per clock and SM; where there are enough
 //     rows for tcgen05, paged_prefill.cu takes them.
 //   * The running maximum is raised only when a row's maximum grows by more
-//     than 2^8 (a warp vote), so O is rescaled a few times per row in all.
+//     than 2^8 (a warp vote), so O is rescaled a few times per row in all. P
+//     rounded to the products' type, as V has it, is off by half a step of it.
 //   * 4-bit caches: codes become f16 pairs by one cvt per pair, times their
 //     e4m3 scale by one half2 product, exactly (6 significant bits; 2^-10 ..
 //     2688); the products run in f16 whatever the queries' type. bf16 queries

@@ -3,10 +3,11 @@
 //
 // The query rows of a sequence and key head (its tokens times the query heads
 // of the group) make items of 256 rows: two tiles of 128 that share every key
-// block. Bound by the tensor and exponential pipes: 4 * 256 * 128 * D
-// operations per 128-key block against 2 * 128 * D cached elements read. Measured
-// on B200: 1024 tokens each of 3 sequences of 4060 to 16384 keys, 32/8 heads of 128
-// in bf16, 0.59 ms for 533 GFLOP (0.90 PFLOP/s), 0.65 ms in a row of calls.
+// block: 4 * 256 * 128 * D operations per 128-key block against 2 * 128 * D cached
+// elements read. Bound by the chain S, softmax, P of a tile, which is longer than
+// the other tile's products (tensor pipe 44 %, exponentials 34 %). Measured on
+// B200: 1024 tokens each of 3 sequences of 4060 to 16384 keys, 32/8 heads of 128 in
+// bf16, 0.59 ms for 533 GFLOP (0.90 PFLOP/s), 0.66 ms in a row of calls.
 //   * Equal runs: the key blocks of all items, in the order (sequence, key head,
 //     row tile, block), are dealt to the persistent CTAs in equal contiguous
 //     runs, so neither ragged lengths nor causal triangles nor few items leave

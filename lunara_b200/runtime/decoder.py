@@ -327,9 +327,10 @@ def paged_attention(Q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     A token at position p sees the keys 0..p of its sequence, with ``window`` > 0 the last
     ``window`` of them; its own key and value must be in the cache (``kv_append`` first). Query
     head h reads key head ``h // (q_heads // kv_heads)``. ``scale`` defaults to ``1 / sqrt(D)``.
-    fp32 softmax; a row that sees no key is zero. Slots that no token sees may hold anything; a
-    value that is not finite may reach the other tokens of its sequence in the call. ``max_q_len``, the most tokens any sequence
-    has here, is a hint that steers the choice of kernels (default: any number)."""
+    fp32 softmax; a row that sees no key is zero, one with a score of +inf or NaN is NaN. Slots
+    that no token sees may hold anything; a value that is not finite may reach the other tokens
+    of its sequence in the call. ``max_q_len``, the most tokens any sequence has here, is a hint
+    that steers the choice of kernels (default: any number). ``out`` may be Q."""
     q, (_, q_heads, tokens, dim) = _rows(Q, "Q")
     assert Q.dim() == 3 and dim == cache.head_dim, f"Q must be [tokens, q_heads, {cache.head_dim}], got {tuple(Q.shape)}"
     assert cache.dtype is None or Q.dtype is cache.dtype, "Q and the cache must share a dtype"

@@ -347,3 +347,16 @@ def test_tokens_before_the_first_sequence(lens, bits, dim, dtype):
     assert torch.equal(ops.paged_attention(moved(q), late, tab, at, seq_lens, out=out)[4:], got[3][4:]) and (out[:4] == 7).all()
     assert torch.equal(late.k_pages.view(torch.uint8), plain.k_pages.view(torch.uint8))
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("bits,dim,dtype", [(16, 128, BF16), (4, 64, F16), (16, 20, F16), (16, 64, F32)])
+def test_the_output_may_be_the_queries(bits, dim, dtype):
+    """In place, where rows are cut between many warps, whole, without keys, and on both kernels."""
+    ops = _ops()
+    p = ref.Paged([(1, 3000), (200, 900), (3, 40), (2, 0), (128, 128)], 2, dim, 16, dtype, seed=26, bits=bits, extra_tokens=2)
+    cache, _ = cache_of(p)
+    q = p.queries(6).cuda()
+    want = ops.paged_attention(q, cache, *where(p))
+    here = q.clone()
+    assert ops.paged_attention(here, cache, *where(p), out=here) is here
+    assert torch.equal(here[:p.owned], want[:p.owned]) and torch.equal(here[p.owned:], q[p.owned:])
