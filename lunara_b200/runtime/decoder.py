@@ -13,11 +13,11 @@ Ragged batches: the tokens of all sequences stand one behind the other;
 [batch] how long each sequence is with them, ``page_table`` int32 [batch, max_pages] which
 page holds its positions ``page_size * i`` onwards. Token ``i`` of ``n`` has position
 ``seq_len - n + i``; a negative one marks padding (written nowhere, zero in outputs).
-Tokens behind ``seq_starts[batch]`` belong to no sequence; their rows are left as they were
-in an output that is given, and zero in one that the call allocates. All three live on the device, so a captured graph follows their contents. What
-is wrong in them (a page outside the cache, a position outside the tables) is kept as a
-device error (``ops.device_error()``) and treated as padding, never as an access out of
-bounds.
+Tokens before ``seq_starts[0]`` and behind ``seq_starts[batch]`` belong to no sequence; their
+rows are left as they were in an output that is given, and zero in one that the call
+allocates. All three live on the device, so a captured graph follows their contents. What is
+wrong in them (a page outside the cache, a position outside the tables) is kept as a device
+error (``ops.device_error()``) and treated as padding, never as an access out of bounds.
 """
 from __future__ import annotations
 
