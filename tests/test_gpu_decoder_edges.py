@@ -360,3 +360,65 @@ def test_the_output_may_be_the_queries(bits, dim, dtype):
     here = q.clone()
     assert ops.paged_attention(here, cache, *where(p), out=here) is here
     assert torch.equal(here[:p.owned], want[:p.owned]) and torch.equal(here[p.owned:], q[p.owned:])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_captured_decode_step_replayed(bits):
+    """Norm, rotation, append and attention of a padded batch as one graph, whose lengths grow on the device, against the same
+    calls outside of it; two graphs over two caches are replayed on two streams at once."""
+    ops = _ops()
+    heads, group, dim, page, batch = 2, 4, 128, 16, 5
+    g = torch.Generator().manual_seed(27)
+    table = ops.rotary_table(200, dim)
+    w = torch.rand(dim, generator=g).bfloat16().cuda() + 0.5
+    first = torch.tensor([0, 15, 16, 90, 47], dtype=torch.int32)
+    starts = torch.arange(batch + 1, dtype=torch.int32, device="cuda")
+    rows = heads * (group + 2)
+
+    class Side:
+        def __init__(self):
+            self.cache = ops.PagedKVCache.allocate(40, heads, page, dim, dtype="e2m1" if bits == 4 else BF16)
+            self.tab = torch.randperm(40, generator=g).int().view(batch, 8).cuda()
+            self.lens = first.clone().cuda()
+            self.qkv = torch.zeros(batch + 2, rows, dim, dtype=BF16, device="cuda")   # two rows of no sequence
+
+        def step(self):
+            self.lens.add_(1)
+            q, k, v = self.qkv.split([heads * group, heads, heads], 1)
+            pos = torch.cat((self.lens - 1, self.lens.new_zeros(2)))
+            nq, nk = ops.qk_norm_rotary(q, k, pos, None, w, w)
+            rq = ops.kv_append(nk, v, self.cache, self.tab, starts, self.lens, table=table, Q=nq)
+            return ops.paged_attention(rq, self.cache, self.tab, starts, self.lens)
+
+    graphed, plain, streams, graphs, outs = [], [], [], [], []
+    for _ in range(2):
+        a, b = Side(), Side()
+        b.tab.copy_(a.tab)
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            a.step()   # (once before the capture)
+        torch.cuda.synchronize()
+        for t in (a.cache.k_pages, a.cache.v_pages) + ((a.cache.k_scales.view(torch.uint8), a.cache.v_scales.view(torch.uint8)) if bits == 4 else ()):
+            t.zero_()
+        a.lens.copy_(first)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = a.step()
+        graphed.append(a), plain.append(b), streams.append(s), graphs.append(graph), outs.append(out)
+    for _ in range(30):
+        for a, b in zip(graphed, plain):
+            b.qkv.copy_(torch.randn(b.qkv.shape, generator=g).bfloat16())
+            a.qkv.copy_(b.qkv)
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, b, a in zip(outs, plain, graphed):
+            want = b.step()
+            assert torch.equal(out, want) and torch.isfinite(out).all() and (out[batch:] == 0).all()
+            assert torch.equal(a.lens, b.lens)
+    for a, b in zip(graphed, plain):
+        assert torch.equal(a.cache.k_pages.view(torch.uint8), b.cache.k_pages.view(torch.uint8))
+    assert ops.device_error() == 0
